@@ -171,6 +171,70 @@ int skhip_attn_varlen_bwd(const void* Q, const void* K, const void* V, const voi
                           float scale, int causal, float p_drop, uint64_t seed,
                           int dtype, void* stream);
 
+/* ---- rotary positions, norms of query and key heads ---------------------------------------
+ * Alternatives to the sinusoid table added to the embeddings (lib/transformer/Models.py:27-46,117-118); the reference
+ * has no counterpart.  Rows are tokens: head h of row t is x[t*ld + h*d .. + d-1].
+ * skhip_qk_rotary: y = R(pos) N(x) for the n_head query heads in q and the n_kv key heads in k (n_kv = 0: k unused).
+ *   R turns the first `rot` elements of a head (even; the others pass) as rot/2 pairs (a, b), pair i by pos * f_i:
+ *   (a cos - b sin, b cos + a sin) * amplitude.  Pairs are (i, i + rot/2), or (2i, 2i + 1) with interleaved != 0.
+ *   turns [rot/2]: f_i / (2 pi) as a 64-bit fraction of a turn (round(f_i / (2 pi) * 2^64) mod 2^64); pos [T] is any
+ *   int64 (the phase pos * turns is exact modulo whole turns).  rot = 0: no turn, pos and turns may be NULL.
+ *   N (gamma_q, gamma_k fp32 [d] given; NULL: identity) is the RMS norm of the head: x / sqrt(mean(x^2) + eps) * gamma.
+ *   inverse != 0 (no norm): the turn by the negative angles, which is the gradient of the turn.
+ *   Outputs may be the inputs.  d <= 256.
+ * skhip_qk_norm_rotary_bwd: from the saved inputs q, k and the output gradients dq_out, dk_out the input gradients
+ *   dq, dk (which may be dq_out, dk_out) and the weights' dgamma_q, dgamma_k [d] (written).  workspace:
+ *   skhip_qk_norm_rotary_bwd_ws_floats(d) floats.  Fixed summation order.                                        */
+int skhip_qk_rotary(const void* q, const void* k, void* q_out, void* k_out, const int64_t* pos, const uint64_t* turns,
+                    float amplitude, const float* gamma_q, const float* gamma_k, float eps, int64_t T, int n_head,
+                    int n_kv, int d, int rot, int64_t ldq, int64_t ldk, int64_t ldq_out, int64_t ldk_out,
+                    int interleaved, int inverse, int dtype, void* stream);
+int64_t skhip_qk_norm_rotary_bwd_ws_floats(int d);
+int skhip_qk_norm_rotary_bwd(const void* q, const void* k, const void* dq_out, const void* dk_out, void* dq, void* dk,
+                             float* dgamma_q, float* dgamma_k, const int64_t* pos, const uint64_t* turns,
+                             float amplitude, const float* gamma_q, const float* gamma_k, float eps, int64_t T,
+                             int n_head, int n_kv, int d, int rot, int64_t ldq, int64_t ldk, int64_t lddq_out,
+                             int64_t lddk_out, int64_t lddq, int64_t lddk, int interleaved, float* workspace,
+                             int64_t workspace_floats, int dtype, void* stream);
+
+/* ---- attention within a window --------------------------------------------------------------
+ * ScaledDotProductAttention (lib/transformer/Modules.py:17-28) with the mask of a sliding window; the reference builds
+ * only pad and causal masks (Models.py:49-69).  Query i of a sequence of Lq queries and Lk keys stands at position
+ * p = i + Lk - Lq and sees key j when
+ *     (p - j < window or j < sinks)  and  (causal ? j <= p : j - p < window)  and not key_pad[b*Lk + j].
+ * The n_head query heads share n_kv key / value heads evenly (head h reads h / (n_head / n_kv)); d <= 128 elements each.
+ * A query that sees nothing gets zeros (LSE -inf) and passes no gradient; keys and values that no query of a tile may
+ * see (padding, rows beyond the sequence) are never used, whatever they hold.
+ * Rows as in skhip_attn_fwd: padded (row b*Lq + i; Tq = B*Lq, Tk = B*Lk) or, with q_off and k_off (int32 [B+1], no
+ * key_pad), packed, Lq and Lk then being at least the longest lengths; rows of a packed tensor outside every sequence get
+ * zeros in O, dQ, dK and dV.  LSE fp32 [n_head][Tq] receives the log-sum-exp of the scaled visible scores.
+ * Backward writes dQ, dK, dV; workspace: skhip_window_attn_bwd_ws_floats() floats.  Fixed summation orders.
+ *
+ * skhip_window_attn_step: the causal form for ONE new query per sequence against a cache.  kv_len[r] positions, the new
+ * one included, the last of which is the query's.  Position j lives in slot  j < sinks ? j : sinks + (j - sinks) %
+ * (cap - sinks)  of  cache[r*row + slot*pos + g*d ..]  (strides in elements): a cache with cap >= kv_len keeps every
+ * position, one with cap = sinks + window is a ring of what can still be seen.  cap - sinks >= window.  k_new, v_new
+ * (optional, [R][ld_new]): the newest position's key and value, which this call uses and stores in its slot.
+ * kv_len[r] <= 0: zeros, nothing stored.  workspace: skhip_window_attn_step_ws_floats() floats (may be 0).       */
+int skhip_window_attn_fwd(const void* Q, const void* K, const void* V, void* O, float* LSE, const uint8_t* key_pad,
+                          const int32_t* q_off, const int32_t* k_off, int B, int n_head, int n_kv, int64_t Tq,
+                          int64_t Tk, int Lq, int Lk, int d, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo,
+                          float scale, int window, int sinks, int causal, int dtype, void* stream);
+int64_t skhip_window_attn_bwd_ws_floats(int B, int n_head, int n_kv, int64_t Tq, int Lq, int Lk, int d, int window,
+                                        int sinks, int causal);
+int skhip_window_attn_bwd(const void* Q, const void* K, const void* V, const void* O, const void* dO, const float* LSE,
+                          void* dQ, void* dK, void* dV, const uint8_t* key_pad, const int32_t* q_off,
+                          const int32_t* k_off, int B, int n_head, int n_kv, int64_t Tq, int64_t Tk, int Lq, int Lk,
+                          int d, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, int64_t lddo, int64_t lddq,
+                          int64_t lddk, int64_t lddv, float scale, int window, int sinks, int causal, float* workspace,
+                          int64_t workspace_floats, int dtype, void* stream);
+int64_t skhip_window_attn_step_ws_floats(int R, int n_head, int n_kv, int d, int cap, int window, int sinks);
+int skhip_window_attn_step(const void* q, const void* k_new, const void* v_new, void* k_cache, void* v_cache, void* out,
+                           const int32_t* kv_len, int R, int n_head, int n_kv, int d, int cap, int64_t ldq,
+                           int64_t ld_new, int64_t ldo, int64_t k_row, int64_t k_pos, int64_t v_row, int64_t v_pos,
+                           float scale, int window, int sinks, float* workspace, int64_t workspace_floats, int dtype,
+                           void* stream);
+
 /* ---- residual + dropout + LayerNorm + pad-row zeroing --------------------------------
  * y = LayerNorm(res + dropout_p(x)) * gamma + beta, rows with row_pad != 0 set to 0.
  * Replaces `self.layer_norm(self.dropout(out) + residual)` (SubLayers.py:62-63,83-84) and

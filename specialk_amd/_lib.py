@@ -5,6 +5,7 @@ passes raw device pointers, sizes and the current HIP stream to the library.  Th
 CPU or torch fallback: if the shared library is missing, or a call is made with non-GPU
 tensors, this module raises.
 """
+import contextlib
 import ctypes
 import os
 
@@ -26,6 +27,9 @@ EXPORTS = [
     "skhip_decode_stack_ws_bytes", "skhip_decode_stack", "skhip_beam_topk_stats", "skhip_beam_step",
     "skhip_softmax_rows", "skhip_conv_windows", "skhip_cnn_head", "skhip_collate", "skhip_set_reserved_cus",
     "skhip_rowpanel_rows", "skhip_rowpanel_pattern_bytes", "skhip_rowpanel_set_stamps", "skhip_rowpanel_gemm", "skhip_rowpanel_gemm_ln",
+    "skhip_qk_rotary", "skhip_qk_norm_rotary_bwd_ws_floats", "skhip_qk_norm_rotary_bwd",
+    "skhip_window_attn_fwd", "skhip_window_attn_bwd_ws_floats", "skhip_window_attn_bwd",
+    "skhip_window_attn_step_ws_floats", "skhip_window_attn_step",
     "skhip_generator_chunk_cols", "skhip_generator_rowstats", "skhip_beam_backtrack",
 ]
 
@@ -90,6 +94,20 @@ def load():
     lib.skhip_rowpanel_gemm_ln.argtypes = [c_p, c_i64, c_p, c_p, c_p, c_i64] + [c_p] * 7 + [c_i64, c_f32, c_f32, c_u64, c_p]
     lib.skhip_generator_rowstats.argtypes = [c_p, c_i64, c_int, c_p, c_p, c_p, c_i64, c_i64, c_i64, c_p]
     lib.skhip_beam_backtrack.argtypes = [c_p] * 4 + [c_int] * 4 + [c_i64, c_p]
+    lib.skhip_qk_rotary.argtypes = [c_p] * 6 + [c_f32, c_p, c_p, c_f32, c_i64] + [c_int] * 4 + [c_i64] * 4 + [c_int] * 3 + [c_p]
+    lib.skhip_qk_norm_rotary_bwd_ws_floats.argtypes = [c_int]
+    lib.skhip_qk_norm_rotary_bwd_ws_floats.restype = c_i64
+    lib.skhip_qk_norm_rotary_bwd.argtypes = ([c_p] * 10 + [c_f32, c_p, c_p, c_f32, c_i64] + [c_int] * 4 + [c_i64] * 6 +
+                                             [c_int, c_p, c_i64, c_int, c_p])
+    lib.skhip_window_attn_fwd.argtypes = ([c_p] * 8 + [c_int] * 3 + [c_i64] * 2 + [c_int] * 3 + [c_i64] * 4 +
+                                          [c_f32] + [c_int] * 4 + [c_p])
+    lib.skhip_window_attn_bwd_ws_floats.argtypes = [c_int] * 3 + [c_i64] + [c_int] * 6
+    lib.skhip_window_attn_bwd_ws_floats.restype = c_i64
+    lib.skhip_window_attn_bwd.argtypes = ([c_p] * 12 + [c_int] * 3 + [c_i64] * 2 + [c_int] * 3 + [c_i64] * 8 +
+                                          [c_f32] + [c_int] * 3 + [c_p, c_i64, c_int, c_p])
+    lib.skhip_window_attn_step_ws_floats.argtypes = [c_int] * 7
+    lib.skhip_window_attn_step_ws_floats.restype = c_i64
+    lib.skhip_window_attn_step.argtypes = ([c_p] * 7 + [c_int] * 5 + [c_i64] * 7 + [c_f32, c_int, c_int, c_p, c_i64, c_int, c_p])
     for name in EXPORTS:
         getattr(lib, name)  # AttributeError here means header and library disagree
     _lib = lib
@@ -304,6 +322,96 @@ def attn_bwd(Q, K, V, O, dO, LSE, dQ, dK, dV, delta, B, H, Lq, Lk, dk, dv, ldq, 
                             lddq, lddk, lddv, float(scale), int(causal), float(p_drop), int(seed), dcode(Q.dtype),
                             _stream())
     _check(rc, "skhip_attn_bwd")
+
+
+# --------------------------------------------------------------------------- rotary positions, norms of heads
+_same_device = contextlib.nullcontext()
+
+
+def on_device(t):
+    """Context in which launches go to the device (and its current stream) that holds t."""
+    if not t.is_cuda:
+        raise RuntimeError("specialk_amd kernels need GPU tensors (there is no CPU path)")
+    here = _raw_device() if _raw_device is not None else torch.cuda.current_device()
+    return _same_device if t.device.index == here else torch.cuda.device(t.device)
+
+
+def qk_rotary(q, k, pos, turns, amplitude, gamma_q, gamma_k, eps, n_head, n_kv, d, rot, interleaved, inverse=False):
+    """(q', k') of the rows q (T, n_head * d) and k (T, n_kv * d) or None; gamma_q / gamma_k None: no norm."""
+    lib = load()
+    T = q.shape[0]
+    qo = torch.empty((T, n_head * d), dtype=q.dtype, device=q.device)
+    ko = None if k is None else torch.empty((T, n_kv * d), dtype=k.dtype, device=k.device)
+    rc = lib.skhip_qk_rotary(_ptr(q), _ptr(k), _ptr(qo), _ptr(ko), _ptr(pos), _ptr(turns), float(amplitude), _ptr(gamma_q),
+                             _ptr(gamma_k), float(eps), T, n_head, 0 if k is None else n_kv, d, rot, q.stride(0),
+                             0 if k is None else k.stride(0), n_head * d, n_kv * d, int(interleaved), int(inverse),
+                             dcode(q.dtype), _stream())
+    _check(rc, "skhip_qk_rotary")
+    return qo, ko
+
+
+def qk_norm_rotary_bwd(q, k, dqo, dko, pos, turns, amplitude, gamma_q, gamma_k, eps, n_head, n_kv, d, rot, interleaved):
+    """(dq, dk, dgamma_q, dgamma_k) from the inputs of qk_rotary and its output gradients."""
+    lib = load()
+    T, dev = q.shape[0], q.device
+    dq = torch.empty((T, n_head * d), dtype=q.dtype, device=dev)
+    dk = None if k is None else torch.empty((T, n_kv * d), dtype=k.dtype, device=dev)
+    dgq = torch.empty(d, dtype=torch.float32, device=dev)
+    dgk = None if k is None else torch.empty(d, dtype=torch.float32, device=dev)
+    n = int(lib.skhip_qk_norm_rotary_bwd_ws_floats(d))
+    ws = torch.empty(n, dtype=torch.float32, device=dev)
+    rc = lib.skhip_qk_norm_rotary_bwd(_ptr(q), _ptr(k), _ptr(dqo), _ptr(dko), _ptr(dq), _ptr(dk), _ptr(dgq), _ptr(dgk),
+                                      _ptr(pos), _ptr(turns), float(amplitude), _ptr(gamma_q), _ptr(gamma_k), float(eps), T,
+                                      n_head, 0 if k is None else n_kv, d, rot, q.stride(0), 0 if k is None else k.stride(0),
+                                      dqo.stride(0), 0 if k is None else dko.stride(0), n_head * d, n_kv * d,
+                                      int(interleaved), _ptr(ws), n, dcode(q.dtype), _stream())
+    _check(rc, "skhip_qk_norm_rotary_bwd")
+    return dq, dk, dgq, dgk
+
+
+# --------------------------------------------------------------------------- attention within a window
+def window_attn_fwd(q, k, v, B, Lq, Lk, n_head, n_kv, d, scale, window, sinks, causal, key_pad=None, q_off=None, k_off=None):
+    """(o (Tq, n_head * d), lse fp32 (n_head, Tq))."""
+    lib = load()
+    o = torch.empty((q.shape[0], n_head * d), dtype=q.dtype, device=q.device)
+    lse = torch.empty((n_head, q.shape[0]), dtype=torch.float32, device=q.device)
+    rc = lib.skhip_window_attn_fwd(_ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse), _ptr(key_pad), _ptr(q_off), _ptr(k_off), B,
+                                   n_head, n_kv, q.shape[0], k.shape[0], Lq, Lk, d, q.stride(0), k.stride(0), v.stride(0),
+                                   n_head * d, float(scale), window, sinks, int(causal), dcode(q.dtype), _stream())
+    _check(rc, "skhip_window_attn_fwd")
+    return o, lse
+
+
+def window_attn_bwd(q, k, v, o, do, lse, B, Lq, Lk, n_head, n_kv, d, scale, window, sinks, causal, key_pad=None, q_off=None,
+                    k_off=None):
+    """(dq, dk, dv), contiguous."""
+    lib = load()
+    dq = torch.empty((q.shape[0], n_head * d), dtype=q.dtype, device=q.device)
+    dk = torch.empty((k.shape[0], n_kv * d), dtype=q.dtype, device=q.device)
+    dv = torch.empty((k.shape[0], n_kv * d), dtype=q.dtype, device=q.device)
+    n = int(lib.skhip_window_attn_bwd_ws_floats(B, n_head, n_kv, q.shape[0], Lq, Lk, d, window, sinks, int(causal)))
+    ws = torch.empty(n, dtype=torch.float32, device=q.device)
+    rc = lib.skhip_window_attn_bwd(_ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(do), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv),
+                                   _ptr(key_pad), _ptr(q_off), _ptr(k_off), B, n_head, n_kv, q.shape[0], k.shape[0], Lq, Lk,
+                                   d, q.stride(0), k.stride(0), v.stride(0), o.stride(0), do.stride(0), n_head * d, n_kv * d,
+                                   n_kv * d, float(scale), window, sinks, int(causal), _ptr(ws), n, dcode(q.dtype), _stream())
+    _check(rc, "skhip_window_attn_bwd")
+    return dq, dk, dv
+
+
+def window_attn_step(q, k_new, v_new, k_cache, v_cache, kv_len, n_head, n_kv, d, scale, window, sinks):
+    """o (R, n_head * d); k_new / v_new (R, n_kv * d; one row stride) or None; caches (R, cap, n_kv * d), written in place."""
+    lib = load()
+    R, cap = k_cache.shape[:2]
+    o = torch.empty((R, n_head * d), dtype=q.dtype, device=q.device)
+    n = int(lib.skhip_window_attn_step_ws_floats(R, n_head, n_kv, d, cap, window, sinks))
+    ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
+    rc = lib.skhip_window_attn_step(_ptr(q), _ptr(k_new), _ptr(v_new), _ptr(k_cache), _ptr(v_cache), _ptr(o), _ptr(kv_len), R,
+                                    n_head, n_kv, d, cap, q.stride(0), 0 if k_new is None else k_new.stride(0), n_head * d,
+                                    k_cache.stride(0), k_cache.stride(1), v_cache.stride(0), v_cache.stride(1), float(scale),
+                                    window, sinks, _ptr(ws), n, dcode(q.dtype), _stream())
+    _check(rc, "skhip_window_attn_step")
+    return o
 
 
 # --------------------------------------------------------------------------- add + LayerNorm

@@ -1,0 +1,510 @@
+// Rotary positions of query and key heads, with an optional RMS norm of every head in the same pass, forward and backward.
+//
+// A head vector x of d elements at position p leaves as  y = R(p) N(x):
+//   N(x) = x * rstd * gamma, rstd = 1 / sqrt(mean(x^2) + eps)      (identity without the norm)
+//   R(p) turns rot / 2 pairs (a, b) of the first rot elements by the angles p f_i and scales them by A:
+//        a' = A (a cos - b sin),  b' = A (b cos + a sin);           elements rot .. d-1 pass through.
+// Pairs are (i, i + rot/2) or, interleaved, (2i, 2i + 1).  Backward, with g = R(p)^T dy (the same turn by -p f_i):
+//   dgamma = sum over rows and heads of g * xhat, xhat = x * rstd;   dx = rstd (g gamma - xhat mean(g gamma xhat)).
+// Without the norm backward IS the forward kernel with the angles negated.
+//
+// Angles: a frequency is a 64-bit fraction of a turn, so  position * frequency mod 2^64  is the exact phase of any 64-bit
+// position in one integer product (in 32-bit floats position 10^6 would already be off by 0.06 rad).  Its top bits give
+// the quadrant and a remainder of at most 1/8 turn, which the Taylor polynomials of sine and cosine take to fp32
+// accuracy.  A block computes the (cos, sin) of its tokens once into LDS and uses them for all heads.
+//
+// Bound by HBM: each element is read and written once (backward of the norm reads x and dy).  A lane owns 8 pairs, or 16
+// of the elements that pass, of one head: two 16-byte loads and stores in bf16, no exchange between lanes but the
+// norm's sum over the lanes of a head.
+#include "common.h"
+#include <algorithm>
+
+namespace {
+
+constexpr int MAX_D = 256;        // at most 16 + 1 owning lanes per head
+constexpr int MAX_TB = 64;        // tokens per group
+constexpr int ANGLES = 2048;      // (cos, sin) pairs per group
+constexpr int UNROLL = 4;         // items a thread has in flight
+constexpr int BWD_BLOCKS = 1024;  // partial dgamma rows of the backward pass
+
+struct RotParams {
+  const void *q, *k;        // forward: inputs; norm backward: the saved inputs
+  const void *dq, *dk;      // norm backward: output gradients
+  void *oq, *ok;            // forward: outputs; backward: input gradients
+  int64_t ldq, ldk, lddq, lddk, ldoq, ldok;
+  const int64_t* pos;
+  const uint64_t* turns;    // [rot / 2]
+  const float *gq, *gk;     // [d]
+  float* partial;           // [blocks][2][d]
+  int64_t T, groups;
+  int H, G, d, rot, lph, tb, width;   // lanes per head (power of two), tokens per group, items per token
+  uint32_t magic;                     // ceil(2^32 / width)
+  float amp, eps;
+  int sign;                           // -1: angles negated
+};
+
+// cos and sin of 2 pi * phase / 2^64
+__device__ __forceinline__ float2 turn_cos_sin(uint64_t phase) {
+  const uint64_t ph = phase + (1ull << 61);
+  const int quad = (int)(ph >> 62);
+  const int32_t v = (int32_t)((uint32_t)(ph >> 30) ^ 0x80000000u);   // remainder in 2^-31 of an eighth of a turn
+  const float x = (float)v * (0.78539816339744831f / 2147483648.f);
+  const float z = x * x;
+  // Taylor series about 0 for |x| <= pi / 4: the first terms left out are below 2e-9 (sine) and 2e-9 (cosine)
+  const float s = x + x * z * (-1.f / 6 + z * (1.f / 120 + z * (-1.f / 5040 + z * (1.f / 362880))));
+  const float c = 1.f + z * (-0.5f + z * (1.f / 24 + z * (-1.f / 720 + z * (1.f / 40320 + z * (-1.f / 3628800)))));
+  float2 r;
+  r.x = (quad & 1) ? s : c;
+  r.y = (quad & 1) ? c : s;
+  if (quad == 1 || quad == 2) r.x = -r.x;
+  if (quad >= 2) r.y = -r.y;
+  return r;
+}
+
+// The 16 elements of lane l of a head: v[j], v[8 + j] = the two halves of pair 8 l + j, or 16 consecutive passing ones.
+template <typename T, bool IL, bool VEC>
+struct Own {
+  static constexpr int VN = Vec16<T>::N;
+  static __device__ __forceinline__ int index(const RotParams& p, int l, int j) {   // j in 0 .. 15; -1: no element
+    const int np = p.rot >> 1, nrl = (np + 7) >> 3;
+    if (l < nrl) {
+      const int pr = 8 * l + (j & 7);
+      if (pr >= np) return -1;
+      return IL ? 2 * pr + (j >> 3) : pr + (j >> 3) * np;
+    }
+    const int e = p.rot + 16 * (l - nrl) + j;
+    return e < p.d ? e : -1;
+  }
+  // base: the head's first element.  Vector form (rot and d multiples of 16, 16-byte rows): two runs of 8 elements.
+  static __device__ __forceinline__ int run(const RotParams& p, int l, int half) {
+    const int np = p.rot >> 1, nrl = np >> 3;
+    if (l < nrl) return IL ? 16 * l + 8 * half : 8 * l + half * np;
+    return p.rot + 16 * (l - nrl) + 8 * half;
+  }
+  // raw[] is the lane's data as loaded
+  typedef decltype(Vec16<T>().v) raw_t;
+  static constexpr int NR = 16 / VN;
+  struct Raw { raw_t r[NR]; };
+  static __device__ __forceinline__ void load(Raw& w, const T* base, const RotParams& p, int l, bool active) {
+    if constexpr (VEC) {
+      if (active) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < NR / 2; ++i) w.r[h * (NR / 2) + i] = *(const raw_t*)(base + run(p, l, h) + i * VN);
+      }
+    } else {
+      T* e = (T*)w.r;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int i = active ? index(p, l, j) : -1;
+        e[j] = i >= 0 ? base[i] : Cvt<T>::from_f32(0.f);
+      }
+    }
+  }
+  // raw order -> pair order (v[j], v[8 + j] = pair j)
+  static __device__ __forceinline__ void unpack(float (&v)[16], const Raw& w, bool rotates) {
+    const T* e = (const T*)w.r;
+    if (VEC && IL && rotates) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { v[j] = Cvt<T>::to_f32(e[2 * j]); v[8 + j] = Cvt<T>::to_f32(e[2 * j + 1]); }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = Cvt<T>::to_f32(e[j]);
+    }
+  }
+  static __device__ __forceinline__ void store(T* base, const float (&v)[16], const RotParams& p, int l, bool rotates) {
+    if constexpr (VEC) {
+      Raw w;
+      T* e = (T*)w.r;
+      if (IL && rotates) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { e[2 * j] = Cvt<T>::from_f32(v[j]); e[2 * j + 1] = Cvt<T>::from_f32(v[8 + j]); }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) e[j] = Cvt<T>::from_f32(v[j]);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < NR / 2; ++i) *(raw_t*)(base + run(p, l, h) + i * VN) = w.r[h * (NR / 2) + i];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int i = index(p, l, j);
+        if (i >= 0) base[i] = Cvt<T>::from_f32(v[j]);
+      }
+    }
+  }
+  // fp32 row vector of d elements (gamma) in pair order
+  static __device__ __forceinline__ void load_row(float (&v)[16], const float* g, const RotParams& p, int l, bool rotates) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      int i;
+      if constexpr (VEC) {
+        if (IL && rotates) i = 16 * l + 2 * (j & 7) + (j >> 3);
+        else i = run(p, l, j >> 3) + (j & 7);
+        if (i >= p.d) i = -1;
+      } else {
+        i = index(p, l, j);
+      }
+      v[j] = i >= 0 ? g[i] : 0.f;
+    }
+  }
+};
+
+__device__ __forceinline__ void group_angles(float2* cs, const RotParams& p, int64_t t0, int nt) {
+  const int np = p.rot >> 1;
+  for (int e = threadIdx.x; e < nt * np; e += 256) {
+    const int t = e / np, i = e - t * np;
+    const int64_t ps = p.pos[t0 + t];
+    float2 r = turn_cos_sin((uint64_t)ps * p.turns[i]);
+    r.x *= p.amp;
+    r.y *= p.sign < 0 ? -p.amp : p.amp;
+    cs[e] = r;
+  }
+}
+
+__device__ __forceinline__ float head_sum(float v, int lph) {
+  for (int o = lph >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// dir > 0: a' = a cos - b sin ...; dir < 0: the turn back
+template <int DIR>
+__device__ __forceinline__ void turn(float (&v)[16], const float2* cs, int valid) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (j >= valid) break;
+    const float2 t = cs[j];
+    const float a = v[j], b = v[8 + j];
+    v[j] = DIR > 0 ? a * t.x - b * t.y : a * t.x + b * t.y;
+    v[8 + j] = DIR > 0 ? b * t.x + a * t.y : b * t.x - a * t.y;
+  }
+}
+
+struct Item { int t, hl, l, head; bool isq, on; };
+__device__ __forceinline__ Item item_of(const RotParams& p, int e, int n, int lanes, int lshift) {
+  Item it;
+  it.t = (int)__umulhi((uint32_t)e, p.magic);
+  if (p.width == 1) it.t = e;
+  it.hl = e - it.t * p.width;
+  it.l = it.hl & (p.lph - 1);
+  it.head = it.hl >> lshift;
+  it.isq = it.head < p.H;
+  it.on = e < n && it.l < lanes;
+  return it;
+}
+
+template <typename T, bool NORM, bool IL, bool VEC>
+__global__ __launch_bounds__(256) void qk_rotary_kernel(RotParams p) {
+  typedef Own<T, IL, VEC> O;
+  __shared__ float2 cs[ANGLES];
+  const int np = p.rot >> 1, nrl = (np + 7) >> 3, lanes = nrl + ((p.d - p.rot + 15) >> 4);
+  const int lshift = __ffs(p.lph) - 1;
+  const int l = threadIdx.x & (p.lph - 1);     // the same for every item of the thread: width and 256 are multiples of lph
+  const bool rotates = l < nrl;
+  const int valid = max(0, min(8, np - 8 * l));
+  float gq[16], gk[16];
+  if (NORM) {
+    const int ll = min(l, lanes - 1);
+    O::load_row(gq, p.gq, p, ll, ll < nrl);
+    O::load_row(gk, p.gk ? p.gk : p.gq, p, ll, ll < nrl);
+  }
+  const float inv_d = 1.f / (float)p.d;
+  for (int64_t grp = blockIdx.x; grp < p.groups; grp += gridDim.x) {
+    const int64_t t0 = grp * p.tb;
+    const int nt = (int)min((int64_t)p.tb, p.T - t0), n = nt * p.width;
+    bool have = false;
+    for (int e0 = 0; e0 < n; e0 += 256 * UNROLL) {
+      typename O::Raw raw[UNROLL];
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        const Item it = item_of(p, e0 + u * 256 + threadIdx.x, n, lanes, lshift);
+        const T* base = it.isq ? (const T*)p.q + (t0 + it.t) * p.ldq + (int64_t)it.head * p.d
+                               : (const T*)p.k + (t0 + it.t) * p.ldk + (int64_t)(it.head - p.H) * p.d;
+        O::load(raw[u], base, p, it.l, it.on);
+      }
+      if (!have) {   // the loads above are in flight meanwhile
+        __syncthreads();
+        group_angles(cs, p, t0, nt);
+        __syncthreads();
+        have = true;
+      }
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        if (e0 + u * 256 >= n) break;   // block-uniform
+        const Item it = item_of(p, e0 + u * 256 + threadIdx.x, n, lanes, lshift);
+        float v[16];
+        O::unpack(v, raw[u], rotates);
+        if (NORM) {
+          float ss = 0.f;
+          if (it.on) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) ss += v[j] * (v[j] * inv_d);   // (the mean, not the sum, has to stay in range)
+          }
+          const float rstd = 1.f / sqrtf(head_sum(ss, p.lph) + p.eps);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = v[j] * rstd * (it.isq ? gq[j] : gk[j]);
+        }
+        if (it.on) {
+          if (rotates) turn<1>(v, cs + it.t * np + 8 * l, VEC ? 8 : valid);
+          T* out = it.isq ? (T*)p.oq + (t0 + it.t) * p.ldoq + (int64_t)it.head * p.d
+                          : (T*)p.ok + (t0 + it.t) * p.ldok + (int64_t)(it.head - p.H) * p.d;
+          O::store(out, v, p, l, rotates);
+        }
+      }
+    }
+  }
+}
+
+// Backward of norm and rotation.  dgamma: every thread sums its own elements of the head over the items it meets, then
+// lanes with the same elements, the waves and (second kernel) the blocks are added in a fixed order: no atomics, results
+// do not change from run to run.
+template <typename T, bool IL, bool VEC>
+__global__ __launch_bounds__(256) void qk_norm_rotary_bwd_kernel(RotParams p) {
+  typedef Own<T, IL, VEC> O;
+  __shared__ float2 cs[ANGLES];
+  __shared__ float red[4][2][MAX_D];
+  const int np = p.rot >> 1, nrl = (np + 7) >> 3, lanes = nrl + ((p.d - p.rot + 15) >> 4);
+  const int lshift = __ffs(p.lph) - 1;
+  const int l = threadIdx.x & (p.lph - 1);
+  const bool rotates = l < nrl;
+  const int valid = max(0, min(8, np - 8 * l));
+  float gq[16], gk[16], aq[16], ak[16];
+  {
+    const int ll = min(l, lanes - 1);
+    O::load_row(gq, p.gq, p, ll, ll < nrl);
+    O::load_row(gk, p.gk ? p.gk : p.gq, p, ll, ll < nrl);
+  }
+#pragma unroll
+  for (int j = 0; j < 16; ++j) aq[j] = ak[j] = 0.f;
+  const float inv_d = 1.f / (float)p.d;
+  constexpr int U = 2;
+  for (int64_t grp = blockIdx.x; grp < p.groups; grp += gridDim.x) {
+    const int64_t t0 = grp * p.tb;
+    const int nt = (int)min((int64_t)p.tb, p.T - t0), n = nt * p.width;
+    bool have = false;
+    for (int e0 = 0; e0 < n; e0 += 256 * U) {
+      typename O::Raw rx[U], rd[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const Item it = item_of(p, e0 + u * 256 + threadIdx.x, n, lanes, lshift);
+        const int64_t t = t0 + it.t, hq = (int64_t)it.head * p.d, hk = (int64_t)(it.head - p.H) * p.d;
+        O::load(rx[u], it.isq ? (const T*)p.q + t * p.ldq + hq : (const T*)p.k + t * p.ldk + hk, p, it.l, it.on);
+        O::load(rd[u], it.isq ? (const T*)p.dq + t * p.lddq + hq : (const T*)p.dk + t * p.lddk + hk, p, it.l, it.on);
+      }
+      if (!have) {
+        __syncthreads();
+        group_angles(cs, p, t0, nt);
+        __syncthreads();
+        have = true;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (e0 + u * 256 >= n) break;   // block-uniform
+        const Item it = item_of(p, e0 + u * 256 + threadIdx.x, n, lanes, lshift);
+        float x[16], g[16];
+        O::unpack(x, rx[u], rotates);
+        O::unpack(g, rd[u], rotates);
+        float ss = 0.f, sg = 0.f;
+        if (it.on) {
+          if (rotates) turn<-1>(g, cs + it.t * np + 8 * l, VEC ? 8 : valid);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            ss += x[j] * (x[j] * inv_d);
+            sg += g[j] * (it.isq ? gq[j] : gk[j]) * x[j];
+          }
+        }
+        const float rstd = 1.f / sqrtf(head_sum(ss, p.lph) + p.eps);
+        const float mean = head_sum(sg, p.lph) * rstd * inv_d;   // mean(g gamma xhat)
+        if (it.on) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float xhat = x[j] * rstd, c = g[j] * xhat;
+            if (it.isq) aq[j] += c; else ak[j] += c;
+            g[j] = rstd * (g[j] * (it.isq ? gq[j] : gk[j]) - xhat * mean);
+          }
+          const int64_t t = t0 + it.t;
+          T* out = it.isq ? (T*)p.oq + t * p.ldoq + (int64_t)it.head * p.d : (T*)p.ok + t * p.ldok + (int64_t)(it.head - p.H) * p.d;
+          O::store(out, g, p, l, rotates);
+        }
+      }
+    }
+  }
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    for (int o = 32; o >= p.lph; o >>= 1) {
+      aq[j] += __shfl_xor(aq[j], o, 64);
+      ak[j] += __shfl_xor(ak[j], o, 64);
+    }
+  if (lane < p.lph && l < lanes) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int i = Own<T, IL, false>::index(p, l, j);
+      if (i >= 0) {
+        // passing elements keep their order; those of pairs are in pair order either way
+        red[wave][0][i] = aq[j];
+        red[wave][1][i] = ak[j];
+      }
+    }
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < 2 * p.d; e += 256) {
+    const int w = e >= p.d, i = e - w * p.d;
+    p.partial[(int64_t)blockIdx.x * 2 * p.d + e] = red[0][w][i] + red[1][w][i] + red[2][w][i] + red[3][w][i];
+  }
+}
+
+// out[c] = sum over blocks of partial[block][c], c < 2 d: one wave per 64 columns and 16 runs of blocks
+__global__ __launch_bounds__(1024) void dgamma_sum_kernel(const float* __restrict__ partial, float* __restrict__ dgq,
+                                                          float* __restrict__ dgk, int blocks, int d) {
+  __shared__ float red[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = blockIdx.x * 64 + lane;
+  float a = 0.f;
+  if (c < 2 * d)
+    for (int b = wave; b < blocks; b += 16) a += partial[(int64_t)b * 2 * d + c];
+  red[wave][lane] = a;
+  __syncthreads();
+  if (wave == 0 && c < 2 * d) {
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) s += red[w][lane];
+    if (c < d) dgq[c] = s;
+    else if (dgk) dgk[c - d] = s;
+  }
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// Lanes per head and tokens per group.
+void plan(RotParams& p) {
+  const int np = p.rot / 2, lanes = (np + 7) / 8 + (p.d - p.rot + 15) / 16;
+  int lph = 1;
+  while (lph < lanes) lph *= 2;
+  p.lph = lph;
+  p.width = (p.H + p.G) * lph;
+  // A group is what a block has between two barriers: four items per thread, fewer where the rows would not give every
+  // CU two blocks (640 rows of 16 heads: 160 blocks of 4 rows instead of 40 of 16).
+  int64_t tb = std::max<int64_t>(1, (256 * UNROLL) / p.width);
+  tb = std::min<int64_t>(tb, std::max<int64_t>(std::max(1, 256 / p.width), p.T / (2 * sk_num_cus())));
+  if (np) tb = std::min<int64_t>(tb, ANGLES / np);
+  p.tb = (int)std::min<int64_t>(tb, MAX_TB);
+  p.groups = (p.T + p.tb - 1) / p.tb;
+  p.magic = (uint32_t)((0x100000000ull + p.width - 1) / p.width);
+}
+
+template <typename T, bool NORM>
+void launch_fwd(const RotParams& p, bool il, bool vec, hipStream_t stream) {
+  const unsigned blocks = (unsigned)std::min<int64_t>(p.groups, (int64_t)sk_num_cus() * 16);
+  if (il) {
+    if (vec) hipLaunchKernelGGL((qk_rotary_kernel<T, NORM, true, true>), dim3(blocks), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((qk_rotary_kernel<T, NORM, true, false>), dim3(blocks), dim3(256), 0, stream, p);
+  } else {
+    if (vec) hipLaunchKernelGGL((qk_rotary_kernel<T, NORM, false, true>), dim3(blocks), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((qk_rotary_kernel<T, NORM, false, false>), dim3(blocks), dim3(256), 0, stream, p);
+  }
+}
+
+template <typename T>
+void launch_bwd(const RotParams& p, bool il, bool vec, unsigned blocks, hipStream_t stream) {
+  if (il) {
+    if (vec) hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, true, true>), dim3(blocks), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, true, false>), dim3(blocks), dim3(256), 0, stream, p);
+  } else {
+    if (vec) hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, false, true>), dim3(blocks), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, false, false>), dim3(blocks), dim3(256), 0, stream, p);
+  }
+}
+
+int check_shape(const char* who, const int64_t* pos, const uint64_t* turns, int64_t T, int n_head, int n_kv, int d, int rot,
+                int dtype) {
+  SK_CHECK_ARG(dtype == SK_F32 || dtype == SK_BF16, "%s: bad dtype %d", who, dtype);
+  SK_CHECK_ARG(T >= 0 && n_head > 0 && n_kv >= 0 && n_head <= 512 && n_kv <= 512, "%s: bad shape (T %lld, heads %d and %d)",
+               who, (long long)T, n_head, n_kv);
+  SK_CHECK_ARG(d > 0 && d <= MAX_D, "%s: head size %d must be in 1..%d", who, d, MAX_D);
+  SK_CHECK_ARG(rot >= 0 && rot % 2 == 0 && rot <= d, "%s: rotated part %d must be even and at most the head size %d", who, rot, d);
+  SK_CHECK_ARG(T == 0 || rot == 0 || (pos && turns), "%s: null pointer", who);
+  return SK_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t skhip_qk_norm_rotary_bwd_ws_floats(int d) { return d > 0 && d <= MAX_D ? (int64_t)BWD_BLOCKS * 2 * d : 0; }
+
+extern "C" int skhip_qk_rotary(const void* q, const void* k, void* q_out, void* k_out, const int64_t* pos,
+                               const uint64_t* turns, float amplitude, const float* gamma_q, const float* gamma_k, float eps,
+                               int64_t T, int n_head, int n_kv, int d, int rot, int64_t ldq, int64_t ldk, int64_t ldq_out,
+                               int64_t ldk_out, int interleaved, int inverse, int dtype, void* stream_) {
+  const char* who = "skhip_qk_rotary";
+  hipStream_t stream = (hipStream_t)stream_;
+  int rc = check_shape(who, pos, turns, T, n_head, n_kv, d, rot, dtype);
+  if (rc) return rc;
+  if (T == 0) return SK_OK;
+  SK_CHECK_ARG(q && q_out && (n_kv == 0 || (k && k_out)), "%s: null pointer", who);
+  SK_CHECK_ARG(!gamma_q || n_kv == 0 || gamma_k, "%s: one norm weight without the other", who);
+  SK_CHECK_ARG(!(gamma_q && inverse), "%s: the inverse turn takes no norm", who);
+  SK_CHECK_ARG(ldq >= (int64_t)n_head * d && ldq_out >= (int64_t)n_head * d && (n_kv == 0 ||
+               (ldk >= (int64_t)n_kv * d && ldk_out >= (int64_t)n_kv * d)), "%s: row stride below the row's length", who);
+  RotParams p = {};
+  p.q = q; p.k = k; p.oq = q_out; p.ok = k_out; p.pos = pos; p.turns = turns; p.amp = amplitude;
+  p.gq = gamma_q; p.gk = gamma_k; p.eps = eps; p.T = T; p.H = n_head; p.G = n_kv; p.d = d; p.rot = rot;
+  p.ldq = ldq; p.ldk = ldk; p.ldoq = ldq_out; p.ldok = ldk_out; p.sign = inverse ? -1 : 1;
+  const int64_t per = dtype == SK_BF16 ? 8 : 4;
+  bool vec = aligned16(q) && aligned16(q_out) && (ldq | ldq_out) % per == 0;
+  if (n_kv) vec = vec && aligned16(k) && aligned16(k_out) && (ldk | ldk_out) % per == 0;
+  vec = vec && rot % 16 == 0 && d % 16 == 0;
+  plan(p);
+  if (dtype == SK_BF16) {
+    if (gamma_q) launch_fwd<bf16_t, true>(p, interleaved, vec, stream);
+    else launch_fwd<bf16_t, false>(p, interleaved, vec, stream);
+  } else {
+    if (gamma_q) launch_fwd<float, true>(p, interleaved, vec, stream);
+    else launch_fwd<float, false>(p, interleaved, vec, stream);
+  }
+  SK_CHECK_LAUNCH(who);
+  return SK_OK;
+}
+
+extern "C" int skhip_qk_norm_rotary_bwd(const void* q, const void* k, const void* dq_out, const void* dk_out, void* dq,
+                                        void* dk, float* dgamma_q, float* dgamma_k, const int64_t* pos,
+                                        const uint64_t* turns, float amplitude, const float* gamma_q, const float* gamma_k,
+                                        float eps, int64_t T, int n_head, int n_kv, int d, int rot, int64_t ldq, int64_t ldk,
+                                        int64_t lddq_out, int64_t lddk_out, int64_t lddq, int64_t lddk, int interleaved,
+                                        float* workspace, int64_t workspace_floats, int dtype, void* stream_) {
+  const char* who = "skhip_qk_norm_rotary_bwd";
+  hipStream_t stream = (hipStream_t)stream_;
+  int rc = check_shape(who, pos, turns, T, n_head, n_kv, d, rot, dtype);
+  if (rc) return rc;
+  SK_CHECK_ARG(gamma_q && dgamma_q && (n_kv == 0 || (gamma_k && dgamma_k)), "%s: null pointer", who);
+  SK_CHECK_ARG(T == 0 || (q && dq_out && dq && (n_kv == 0 || (k && dk_out && dk))), "%s: null pointer", who);
+  const int64_t nq = (int64_t)n_head * d, nk = (int64_t)n_kv * d;
+  SK_CHECK_ARG(T == 0 || (ldq >= nq && lddq_out >= nq && lddq >= nq && ldk >= nk && lddk_out >= nk && lddk >= nk),
+               "%s: row stride below the row's length", who);
+  RotParams p = {};
+  p.q = q; p.k = k; p.dq = dq_out; p.dk = dk_out; p.oq = dq; p.ok = dk; p.pos = pos; p.turns = turns; p.amp = amplitude;
+  p.gq = gamma_q; p.gk = gamma_k; p.eps = eps; p.T = T; p.H = n_head; p.G = n_kv; p.d = d; p.rot = rot;
+  p.ldq = ldq; p.ldk = ldk; p.lddq = lddq_out; p.lddk = lddk_out; p.ldoq = lddq; p.ldok = lddk; p.sign = 1;
+  const int64_t per = dtype == SK_BF16 ? 8 : 4;
+  bool vec = aligned16(q) && aligned16(dq_out) && aligned16(dq) && (ldq | lddq_out | lddq) % per == 0;
+  if (n_kv) vec = vec && aligned16(k) && aligned16(dk_out) && aligned16(dk) && (ldk | lddk_out | lddk) % per == 0;
+  vec = vec && rot % 16 == 0 && d % 16 == 0;
+  plan(p);
+  const int blocks = (int)std::min<int64_t>(p.groups, BWD_BLOCKS);
+  if (!workspace || workspace_floats < (int64_t)blocks * 2 * d) {
+    sk_set_error("%s: workspace of %lld floats needed", who, (long long)blocks * 2 * d);
+    return SK_ERR_WORKSPACE;
+  }
+  p.partial = workspace;
+  if (T > 0) {
+    if (dtype == SK_BF16) launch_bwd<bf16_t>(p, interleaved, vec, (unsigned)blocks, stream);
+    else launch_bwd<float>(p, interleaved, vec, (unsigned)blocks, stream);
+    SK_CHECK_LAUNCH(who);
+  }
+  hipLaunchKernelGGL(dgamma_sum_kernel, dim3((2 * d + 63) / 64), dim3(1024), 0, stream, workspace, dgamma_q,
+                     n_kv ? dgamma_k : nullptr, blocks, d);
+  SK_CHECK_LAUNCH(who);
+  return SK_OK;
+}

@@ -1,0 +1,110 @@
+// Shared parameter block, visibility rule and tile lists of the windowed-attention kernels
+// (window_attn.hip: fp32 arithmetic, any head size; window_attn_mfma.hip: bf16 matrix cores; window_step.hip: one query
+// per sequence over a cache).
+//
+// Query i of a sequence with Lq queries and Lk keys stands at position p = i + Lk - Lq (the last query beside the last
+// key).  It sees key j when  j <= p + right  and  (j >= p - left or j < sinks), and key j is not padding.  left and
+// right are window - 1 (right = 0 in the causal form), clamped by the host to Lq + Lk.  A row that sees nothing has
+// output 0, log-sum-exp -inf and no gradient.
+#pragma once
+#include "common.h"
+
+namespace skwin {
+
+struct WinParams {
+  const void *Q, *K, *V, *O, *dO;
+  void *Oout, *dQ, *dK, *dV;
+  float* LSE;               // [H][Tq]
+  float* delta;             // [H][Tq]
+  float* slabs;             // partial dK, dV of the tiles that hold sinks (see below)
+  const uint8_t* key_pad;   // [B][Lk]; padded batches only
+  const int32_t* q_off;     // packed batches: rows of sequence b are q_off[b] .. q_off[b+1]-1; NULL: (B, Lq) rows
+  const int32_t* k_off;
+  int B, H, G, Lq, Lk, d;   // G key / value heads, head h reads h / (H / G); Lq, Lk: longest sequence when packed
+  int64_t Tq, Tk;           // rows of Q resp. K
+  int64_t ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
+  float scale;
+  int left, right, sinks;
+  // Backward of the keys: queries beyond a key's window see it only if it is a sink, so the few key tiles that hold
+  // sinks would sweep the whole sequence alone.  Their far queries are cut into nch chunks of ch rows, one block each;
+  // window part and chunks leave fp32 partial sums in slabs, which a small kernel adds in a fixed order.
+  int nst, nch, ch;
+};
+
+struct Seq { int64_t qbase, kbase; int Lq, Lk, off; };
+
+__device__ __forceinline__ Seq seq_of(const WinParams& p, int b) {
+  Seq s;
+  if (p.q_off) {   // offsets are device data: clamped to the tensors, lengths to what the grid covers
+    const int64_t q0 = max((int64_t)0, min((int64_t)p.q_off[b], p.Tq)), q1 = max(q0, min((int64_t)p.q_off[b + 1], p.Tq));
+    const int64_t k0 = max((int64_t)0, min((int64_t)p.k_off[b], p.Tk)), k1 = max(k0, min((int64_t)p.k_off[b + 1], p.Tk));
+    s.qbase = q0; s.Lq = (int)min(q1 - q0, (int64_t)p.Lq);
+    s.kbase = k0; s.Lk = (int)min(k1 - k0, (int64_t)p.Lk);
+  } else {
+    s.qbase = (int64_t)b * p.Lq; s.Lq = p.Lq;
+    s.kbase = (int64_t)b * p.Lk; s.Lk = p.Lk;
+  }
+  s.off = s.Lk - s.Lq;
+  return s;
+}
+
+__device__ __forceinline__ bool sees(const WinParams& p, int pos, int j) {
+  return j <= pos + p.right && (j >= pos - p.left || j < p.sinks);
+}
+
+// Keys that queries i0 .. i1-1 see: sinks [0, s_hi) where they lie before the window, and [lo, hi).  Tiles of N keys:
+// the first nst cover the sinks, the others start at w0.
+struct KeyTiles {
+  int lo, hi, s_hi, nst, w0, n;
+  template <int N>
+  static __device__ __forceinline__ KeyTiles of(const WinParams& p, const Seq& sq, int i0, int i1) {
+    KeyTiles t;
+    t.hi = min(sq.Lk, i1 + sq.off + p.right);
+    t.lo = max(0, i0 + sq.off - p.left);
+    t.s_hi = max(0, min(min(p.sinks, t.lo), t.hi));
+    t.nst = (t.s_hi + N - 1) / N;
+    t.w0 = max(t.lo, t.nst * N);
+    t.n = t.nst + max(0, (t.hi - t.w0 + N - 1) / N);
+    return t;
+  }
+  template <int N> __device__ __forceinline__ int start(int t) const { return t < nst ? N * t : w0 + N * (t - nst); }
+  __device__ __forceinline__ bool holds(int j) const { return j < hi && (j >= lo || j < s_hi); }
+};
+
+// Queries that see keys j0 .. j1-1 (rows [i_lo, i_hi)): chunk < 0: through the window; else the given chunk of the
+// queries beyond it, which see only the sinks among the keys.
+__device__ __forceinline__ void query_range(const WinParams& p, const Seq& sq, int j0, int j1, int chunk, int& i_lo, int& i_hi) {
+  const int far = max(0, min(sq.Lq, j1 + p.left - sq.off));
+  if (chunk < 0) {
+    i_lo = max(0, min(sq.Lq, j0 - p.right - sq.off));
+    i_hi = far;
+  } else {
+    i_lo = min(sq.Lq, far + chunk * p.ch);
+    i_hi = min(sq.Lq, i_lo + p.ch);
+  }
+}
+
+// Slab of one (sequence, key head, sink tile, part): [2][tile rows][d] floats; part 0 is the window, 1 + c chunk c.
+__device__ __forceinline__ float* slab(const WinParams& p, int b, int g, int st, int part, int rows) {
+  return p.slabs + ((((int64_t)b * p.G + g) * p.nst + st) * (1 + p.nch) + part) * 2 * rows * p.d;
+}
+
+// Rows of a packed tensor that belong to no sequence become zero: columns col0 .. col0 + d - 1 of rows < off[0] and
+// >= off[B] (called by the blocks of the extra grid layer; `part` of `parts` blocks).
+template <typename T>
+__device__ __forceinline__ void zero_rest(T* out, int64_t ld, int64_t col0, int d, const int32_t* off, int B, int64_t rows,
+                                          int part, int parts) {
+  const int64_t a = max((int64_t)0, min((int64_t)off[0], rows)), z = max(a, min((int64_t)off[B], rows));
+  const int64_t n = a + (rows - z);
+  for (int64_t e = (int64_t)part * 256 + threadIdx.x; e < n * d; e += (int64_t)parts * 256) {
+    const int64_t r = e / d;
+    out[(r < a ? r : z + (r - a)) * ld + col0 + (e - r * d)] = T(0);
+  }
+}
+
+}  // namespace skwin
+
+// bf16 matrix-core path (window_attn_mfma.hip)
+bool sk_window_mfma_supported(const skwin::WinParams& p, int dtype);
+int sk_window_fwd_mfma(const skwin::WinParams& p, hipStream_t stream);
+int sk_window_bwd_mfma(const skwin::WinParams& p, hipStream_t stream);

@@ -1,0 +1,477 @@
+// Attention within a sliding window, with a few first keys that stay visible, forward and backward: fp32 arithmetic on
+// the matrix cores (v_mfma_f32_16x16x4_f32), any head size up to 128, both storage types, any stride and alignment.
+// The bf16 path for aligned heads is window_attn_mfma.hip.
+//
+//   S = scale Q K^T on visible pairs,  P = softmax(S),  O = P V;   with L = log-sum-exp of the rows of S:
+//   P = exp(S - L),  dV = P^T dO,  dP = dO V^T,  dS = scale P (dP - rowsum(dO O)),  dQ = dS K,  dK = dS^T Q.
+//
+// A wave owns 16 rows (queries; keys in the dK / dV kernel) in registers and sweeps the other side in tiles of 64 rows
+// held in LDS as fp32.  Products are D[rho][c] = sum_k X[rho][k] Y[c][k] with X from LDS and the wave's own rows Y on the
+// lanes, so a softmax row is 16 registers and two exchanges, and the accumulators of the scores are the Y operand of the
+// next product as they stand (k = 4 (lane / 16) + r, taken for r = 0 .. 3 in turn).  Scores never reach memory; tiles
+// outside the window are never visited; dQ and dK / dV come from separate launches, so that no sum depends on the order
+// of blocks.  Shared key heads: the dK / dV block walks the query heads of its group.
+// Bound by the fp32 matrix rate (1/16 of bf16's), then by the LDS reads of the column operand.
+#include "window_attn.h"
+#include <algorithm>
+
+using namespace skwin;
+
+namespace {
+
+constexpr int NT = 64;     // rows per LDS tile
+constexpr int MAXD = 128;
+
+template <int D> struct Tile { float a[NT][D + 4]; };
+
+__device__ __forceinline__ f32x4_t mfma4(float x, float y, f32x4_t acc) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(x, y, acc, 0, 0, 0);
+}
+
+// rows r0 .. r0+63 of a matrix as fp32; rows for which ok(row) does not hold and columns beyond d become zero
+template <typename T, int D, class F>
+__device__ __forceinline__ void stage(Tile<D>& t, const T* base, int64_t ld, int r0, int d, F&& ok) {
+  for (int e = threadIdx.x; e < NT * (D / 4); e += 256) {
+    const int r = e / (D / 4), c = (e - r * (D / 4)) * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (c < d && ok(r0 + r)) {
+      const T* s = base + (int64_t)(r0 + r) * ld + c;
+      v.x = Cvt<T>::to_f32(s[0]);
+      if (c + 1 < d) v.y = Cvt<T>::to_f32(s[1]);
+      if (c + 2 < d) v.z = Cvt<T>::to_f32(s[2]);
+      if (c + 3 < d) v.w = Cvt<T>::to_f32(s[3]);
+    }
+    *(float4*)&t.a[r][c] = v;
+  }
+}
+
+// own row: y[s][j] = element 16 s + 4 g + j
+template <typename T, int D>
+__device__ __forceinline__ void load_own(f32x4_t (&y)[D / 16], const T* row, int d, int g, bool ok) {
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = 16 * s + 4 * g + j;
+      y[s][j] = ok && c < d ? Cvt<T>::to_f32(row[c]) : 0.f;
+    }
+}
+
+// D[16 rows of the tile from row0][own] = sum over the head of tile x own
+template <int D>
+__device__ __forceinline__ f32x4_t dot_rows(const Tile<D>& t, int row0, const f32x4_t (&y)[D / 16], int lane) {
+  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) {
+    const float4 x = *(const float4*)&t.a[row0 + (lane & 15)][16 * s + 4 * (lane >> 4)];
+    acc = mfma4(x.x, y[s][0], acc);
+    acc = mfma4(x.y, y[s][1], acc);
+    acc = mfma4(x.z, y[s][2], acc);
+    acc = mfma4(x.w, y[s][3], acc);
+  }
+  return acc;
+}
+
+// out[t][..] (columns 16 t + ..) += sum over tile rows row0 .. row0 + 15 of coef x tile
+template <int D>
+__device__ __forceinline__ void add_cols(f32x4_t (&out)[D / 16], const Tile<D>& t, int row0, const f32x4_t& coef, int lane) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const float* row = t.a[row0 + 4 * (lane >> 4) + r] + (lane & 15);
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) out[c] = mfma4(row[16 * c], coef[r], out[c]);
+  }
+}
+
+__device__ __forceinline__ float quad_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+// own row's columns 16 t + 4 g + r
+template <typename T, int D>
+__device__ __forceinline__ void store_own(T* row, const f32x4_t (&o)[D / 16], float mul, int d, int g) {
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int c = 16 * t + 4 * g + r;
+      if (c < d) row[c] = Cvt<T>::from_f32(o[t][r] * mul);
+    }
+}
+
+__device__ __forceinline__ bool padded(const WinParams& p, int b, int j) {
+  return p.key_pad && p.key_pad[(int64_t)b * p.Lk + j];
+}
+
+// ------------------------------------------------------------------------------ forward
+template <typename T, int D>
+__global__ __launch_bounds__(256) void window_fwd_kernel(WinParams p) {
+  __shared__ __attribute__((aligned(16))) Tile<D> Ks;
+  __shared__ __attribute__((aligned(16))) Tile<D> Vs;
+  __shared__ uint8_t gone[NT];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+  const int b = blockIdx.z, h = blockIdx.y, kh = h / (p.H / p.G);
+  if (b == p.B) {   // packed: rows of no sequence
+    zero_rest<T>((T*)p.Oout, p.ldo, (int64_t)h * p.d, p.d, p.q_off, p.B, p.Tq, blockIdx.x, gridDim.x);
+    return;
+  }
+  const Seq sq = seq_of(p, b);
+  const int i0 = blockIdx.x * 64;
+  if (i0 >= sq.Lq) return;   // block-uniform
+  const int i = i0 + wave * 16 + c, pos = i + sq.off;
+  const KeyTiles kt = KeyTiles::of<NT>(p, sq, i0, min(i0 + 64, sq.Lq));
+  const T* K = (const T*)p.K + sq.kbase * p.ldk + (int64_t)kh * p.d;
+  const T* V = (const T*)p.V + sq.kbase * p.ldv + (int64_t)kh * p.d;
+  f32x4_t fq[D / 16], o[D / 16];
+  load_own<T, D>(fq, (const T*)p.Q + (sq.qbase + min(i, sq.Lq - 1)) * p.ldq + (int64_t)h * p.d, p.d, g, i < sq.Lq);
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  for (int t = 0; t < kt.n; ++t) {
+    const int j0 = kt.start<NT>(t);
+    __syncthreads();
+    if (threadIdx.x < NT) {
+      const int j = j0 + threadIdx.x;
+      gone[threadIdx.x] = !kt.holds(j) || padded(p, b, j);
+    }
+    __syncthreads();
+    auto ok = [&](int j) { return !gone[j - j0]; };
+    stage<T, D>(Ks, K, p.ldk, j0, p.d, ok);
+    stage<T, D>(Vs, V, p.ldv, j0, p.d, ok);
+    __syncthreads();
+    f32x4_t sc[4];
+    float mx = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      sc[k] = dot_rows<D>(Ks, 16 * k, fq, lane);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int jl = 16 * k + 4 * g + r;
+        sc[k][r] = gone[jl] || !sees(p, pos, j0 + jl) ? -INFINITY : sc[k][r] * p.scale;
+        mx = fmaxf(mx, sc[k][r]);
+      }
+    }
+    const float mn = fmaxf(m, quad_max(mx));
+    const bool dead = mn == -INFINITY;
+    const float alpha = dead ? 1.f : expf(m - mn);
+    float rs = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        sc[k][r] = dead ? 0.f : expf(sc[k][r] - mn);
+        rs += sc[k][r];
+      }
+    l = l * alpha + quad_sum(rs);
+    m = mn;
+#pragma unroll
+    for (int x = 0; x < D / 16; ++x) o[x] *= alpha;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) add_cols<D>(o, Vs, 16 * k, sc[k], lane);
+  }
+  if (i < sq.Lq) {
+    store_own<T, D>((T*)p.Oout + (sq.qbase + i) * p.ldo + (int64_t)h * p.d, o, l > 0.f ? 1.f / l : 0.f, p.d, g);
+    if (g == 0) p.LSE[(int64_t)h * p.Tq + sq.qbase + i] = l > 0.f ? m + logf(l) : -INFINITY;
+  }
+}
+
+// ------------------------------------------------------------------------------ dQ, delta
+template <typename T, int D>
+__global__ __launch_bounds__(256) void window_dq_kernel(WinParams p) {
+  __shared__ __attribute__((aligned(16))) Tile<D> Ks;
+  __shared__ __attribute__((aligned(16))) Tile<D> Vs;
+  __shared__ uint8_t gone[NT];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+  const int b = blockIdx.z, h = blockIdx.y, kh = h / (p.H / p.G);
+  if (b == p.B) {
+    zero_rest<T>((T*)p.dQ, p.lddq, (int64_t)h * p.d, p.d, p.q_off, p.B, p.Tq, blockIdx.x, gridDim.x);
+    return;
+  }
+  const Seq sq = seq_of(p, b);
+  const int i0 = blockIdx.x * 64;
+  if (i0 >= sq.Lq) return;
+  const int i = i0 + wave * 16 + c, pos = i + sq.off;
+  const int64_t row = sq.qbase + min(i, sq.Lq - 1), si = (int64_t)h * p.Tq + row;
+  const KeyTiles kt = KeyTiles::of<NT>(p, sq, i0, min(i0 + 64, sq.Lq));
+  const T* K = (const T*)p.K + sq.kbase * p.ldk + (int64_t)kh * p.d;
+  const T* V = (const T*)p.V + sq.kbase * p.ldv + (int64_t)kh * p.d;
+  f32x4_t fq[D / 16], fd[D / 16], dq[D / 16];
+  load_own<T, D>(fq, (const T*)p.Q + row * p.ldq + (int64_t)h * p.d, p.d, g, i < sq.Lq);
+  load_own<T, D>(fd, (const T*)p.O + row * p.ldo + (int64_t)h * p.d, p.d, g, i < sq.Lq);
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t) dq[t] = fd[t];
+  load_own<T, D>(fd, (const T*)p.dO + row * p.lddo + (int64_t)h * p.d, p.d, g, i < sq.Lq);
+  float dl = 0.f;
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) { dl += dq[t][r] * fd[t][r]; dq[t][r] = 0.f; }
+  dl = quad_sum(dl);
+  const float lse = p.LSE[si];
+  if (i < sq.Lq && g == 0) p.delta[si] = dl;
+  for (int t = 0; t < kt.n; ++t) {
+    const int j0 = kt.start<NT>(t);
+    __syncthreads();
+    if (threadIdx.x < NT) {
+      const int j = j0 + threadIdx.x;
+      gone[threadIdx.x] = !kt.holds(j) || padded(p, b, j);
+    }
+    __syncthreads();
+    auto ok = [&](int j) { return !gone[j - j0]; };
+    stage<T, D>(Ks, K, p.ldk, j0, p.d, ok);
+    stage<T, D>(Vs, V, p.ldv, j0, p.d, ok);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const f32x4_t sc = dot_rows<D>(Ks, 16 * k, fq, lane), dp = dot_rows<D>(Vs, 16 * k, fd, lane);
+      f32x4_t ds;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int jl = 16 * k + 4 * g + r;
+        const bool off = gone[jl] || i >= sq.Lq || !sees(p, pos, j0 + jl);
+        ds[r] = off ? 0.f : expf(sc[r] * p.scale - lse) * (dp[r] - dl) * p.scale;
+      }
+      add_cols<D>(dq, Ks, 16 * k, ds, lane);
+    }
+  }
+  if (i < sq.Lq) store_own<T, D>((T*)p.dQ + (sq.qbase + i) * p.lddq + (int64_t)h * p.d, dq, 1.f, p.d, g);
+}
+
+// ------------------------------------------------------------------------------ dK, dV
+template <typename T, int D>
+__global__ __launch_bounds__(256) void window_dkv_kernel(WinParams p) {
+  __shared__ __attribute__((aligned(16))) Tile<D> Qs;
+  __shared__ __attribute__((aligned(16))) Tile<D> Ds;
+  __shared__ float s_lse[NT], s_dl[NT];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+  const int b = blockIdx.z, kh = blockIdx.y, rep = p.H / p.G;
+  const int tiles = (p.Lk + NT - 1) / NT;
+  if (b == p.B) {
+    zero_rest<T>((T*)p.dK, p.lddk, (int64_t)kh * p.d, p.d, p.k_off, p.B, p.Tk, blockIdx.x, gridDim.x);
+    zero_rest<T>((T*)p.dV, p.lddv, (int64_t)kh * p.d, p.d, p.k_off, p.B, p.Tk, blockIdx.x, gridDim.x);
+    return;
+  }
+  const Seq sq = seq_of(p, b);
+  const int extra = (int)blockIdx.x - tiles;                       // >= 0: a chunk of far queries of a sink tile
+  const int tile = extra < 0 ? (int)blockIdx.x : extra / p.nch, chunk = extra < 0 ? -1 : extra % p.nch;
+  const int j0 = tile * NT, j1 = min(j0 + NT, sq.Lk);
+  if (j0 >= sq.Lk) return;
+  const bool partial = tile < p.nst;
+  int i_lo, i_hi;
+  query_range(p, sq, j0, j1, chunk, i_lo, i_hi);
+  if (chunk >= 0 && i_lo >= i_hi) return;   // (the join counts the same chunks)
+  const int j = j0 + wave * 16 + c, jrow = min(j, sq.Lk - 1);
+  const bool alive = j < sq.Lk && !padded(p, b, jrow);
+  const bool busy = chunk < 0 || j0 + wave * 16 < p.sinks;         // wave-uniform
+  f32x4_t fk[D / 16], fv[D / 16], dk[D / 16], dv[D / 16];
+  load_own<T, D>(fk, (const T*)p.K + (sq.kbase + jrow) * p.ldk + (int64_t)kh * p.d, p.d, g, alive);
+  load_own<T, D>(fv, (const T*)p.V + (sq.kbase + jrow) * p.ldv + (int64_t)kh * p.d, p.d, g, alive);
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t) dk[t] = dv[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int hh = 0; hh < rep; ++hh) {
+    const int h = kh * rep + hh;
+    const T* Q = (const T*)p.Q + sq.qbase * p.ldq + (int64_t)h * p.d;
+    const T* dO = (const T*)p.dO + sq.qbase * p.lddo + (int64_t)h * p.d;
+    for (int r0 = i_lo; r0 < i_hi; r0 += NT) {
+      __syncthreads();
+      auto ok = [&](int i) { return i < i_hi; };
+      stage<T, D>(Qs, Q, p.ldq, r0, p.d, ok);
+      stage<T, D>(Ds, dO, p.lddo, r0, p.d, ok);
+      if (threadIdx.x < NT) {
+        const int64_t si = (int64_t)h * p.Tq + sq.qbase + min(r0 + (int)threadIdx.x, sq.Lq - 1);
+        s_lse[threadIdx.x] = p.LSE[si];
+        s_dl[threadIdx.x] = p.delta[si];
+      }
+      __syncthreads();
+      if (!busy) continue;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const f32x4_t sc = dot_rows<D>(Qs, 16 * k, fk, lane), dp = dot_rows<D>(Ds, 16 * k, fv, lane);
+        f32x4_t pr, ds;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int il = 16 * k + 4 * g + r, i = r0 + il;
+          const bool off = !alive || i >= i_hi || !sees(p, i + sq.off, j);
+          pr[r] = off ? 0.f : expf(sc[r] * p.scale - s_lse[il]);
+          ds[r] = off ? 0.f : pr[r] * (dp[r] - s_dl[il]) * p.scale;
+        }
+        add_cols<D>(dv, Ds, 16 * k, pr, lane);
+        add_cols<D>(dk, Qs, 16 * k, ds, lane);
+      }
+    }
+  }
+  if (j >= sq.Lk) return;
+  if (partial) {
+    float* s = slab(p, b, kh, tile, 1 + chunk, NT) + (int64_t)(j - j0) * p.d;
+    store_own<float, D>(s, dk, 1.f, p.d, g);
+    store_own<float, D>(s + (int64_t)NT * p.d, dv, 1.f, p.d, g);
+  } else {
+    store_own<T, D>((T*)p.dK + (sq.kbase + j) * p.lddk + (int64_t)kh * p.d, dk, 1.f, p.d, g);
+    store_own<T, D>((T*)p.dV + (sq.kbase + j) * p.lddv + (int64_t)kh * p.d, dv, 1.f, p.d, g);
+  }
+}
+
+// dK, dV of the tiles that hold sinks: window part and chunks added in this order
+template <typename T>
+__global__ __launch_bounds__(256) void window_join_kernel(WinParams p, int rows) {
+  const int b = blockIdx.z, kh = blockIdx.y, tile = blockIdx.x;
+  const Seq sq = seq_of(p, b);
+  const int j0 = tile * rows, n = min(rows, sq.Lk - j0);
+  int lo, hi, parts = 1;
+  for (; parts <= p.nch; ++parts) {
+    query_range(p, sq, j0, j0 + n, parts - 1, lo, hi);
+    if (lo >= hi) break;
+  }
+  for (int e = threadIdx.x; e < n * p.d; e += 256) {
+    float a = 0.f, v = 0.f;
+    for (int s = 0; s < parts; ++s) {
+      const float* x = slab(p, b, kh, tile, s, rows) + e;
+      a += x[0];
+      v += x[(int64_t)rows * p.d];
+    }
+    const int r = e / p.d, c = e - r * p.d;
+    const int64_t at = sq.kbase + j0 + r;
+    ((T*)p.dK)[at * p.lddk + (int64_t)kh * p.d + c] = Cvt<T>::from_f32(a);
+    ((T*)p.dV)[at * p.lddv + (int64_t)kh * p.d + c] = Cvt<T>::from_f32(v);
+  }
+}
+
+int check(const char* who, const WinParams& p, int window, int dtype) {
+  SK_CHECK_ARG(dtype == SK_F32 || dtype == SK_BF16, "%s: bad dtype %d", who, dtype);
+  SK_CHECK_ARG(p.B >= 0 && p.H > 0 && p.G > 0 && p.Lq >= 0 && p.Lk >= 0 && p.Tq >= 0 && p.Tk >= 0, "%s: bad shape", who);
+  SK_CHECK_ARG(p.H % p.G == 0, "%s: %d query heads do not share %d key heads evenly", who, p.H, p.G);
+  SK_CHECK_ARG(p.d > 0 && p.d <= MAXD, "%s: head size %d must be in 1..%d", who, p.d, MAXD);
+  SK_CHECK_ARG(p.H <= 65535 && p.B <= 65534, "%s: more than 65535 heads or 65534 sequences", who);
+  SK_CHECK_ARG(p.Lq <= (1 << 29) && p.Lk <= (1 << 29), "%s: sequences of more than 2^29 positions", who);
+  SK_CHECK_ARG(window >= 1 && p.sinks >= 0, "%s: window %d must be >= 1 and sinks %d >= 0", who, window, p.sinks);
+  SK_CHECK_ARG(!p.q_off == !p.k_off, "%s: one offset array without the other", who);
+  SK_CHECK_ARG(!(p.q_off && p.key_pad), "%s: packed rows take no padding mask", who);
+  SK_CHECK_ARG(p.q_off || (p.Tq == (int64_t)p.B * p.Lq && p.Tk == (int64_t)p.B * p.Lk), "%s: rows are not B x L", who);
+  const int64_t nq = (int64_t)p.H * p.d, nk = (int64_t)p.G * p.d;
+  SK_CHECK_ARG(p.ldq >= nq && p.ldo >= nq && p.ldk >= nk && p.ldv >= nk, "%s: row stride below the row's length", who);
+  return SK_OK;
+}
+
+void set_window(WinParams& p, int window, int causal) {
+  const int span = p.Lq + p.Lk;
+  p.left = std::min(window - 1, span);
+  p.right = causal ? 0 : p.left;
+  p.sinks = std::min(p.sinks, p.Lk);
+}
+
+// Tiles that hold sinks and the chunks their far queries are cut into: as many rows per chunk as a key tile's own window
+// has, so that these blocks last no longer than the others.
+void plan_sinks(WinParams& p, int rows) {
+  const bool far = p.sinks > 0 && p.left < p.Lk;   // else every query's window reaches key 0
+  p.nst = far ? (p.sinks + rows - 1) / rows : 0;
+  p.ch = std::max(512, (p.left + p.right + rows + 63) / 64 * 64);
+  p.nch = far ? (p.Lq + p.ch - 1) / p.ch : 0;
+}
+
+int64_t slab_floats(const WinParams& p, int rows) {
+  return (int64_t)p.B * p.G * p.nst * (1 + p.nch) * 2 * rows * p.d;
+}
+
+template <typename T, int D>
+void launch_fwd(const WinParams& p, hipStream_t stream) {
+  dim3 grid(std::max(1, (p.Lq + 63) / 64), p.H, p.B + (p.q_off ? 1 : 0));
+  hipLaunchKernelGGL((window_fwd_kernel<T, D>), grid, dim3(256), 0, stream, p);
+}
+template <typename T, int D>
+void launch_bwd(const WinParams& p, hipStream_t stream) {
+  const int layers = p.B + (p.q_off ? 1 : 0);
+  if (p.Tq)
+    hipLaunchKernelGGL((window_dq_kernel<T, D>), dim3(std::max(1, (p.Lq + 63) / 64), p.H, layers), dim3(256), 0, stream, p);
+  if (p.Tk)
+    hipLaunchKernelGGL((window_dkv_kernel<T, D>), dim3(std::max(1, (p.Lk + NT - 1) / NT + p.nst * p.nch), p.G, layers), dim3(256),
+                       0, stream, p);
+}
+
+}  // namespace
+
+int sk_window_join(const WinParams& p, int rows, int dtype, hipStream_t stream) {
+  if (!p.nst) return SK_OK;
+  dim3 grid(p.nst, p.G, p.B);
+  if (dtype == SK_BF16) hipLaunchKernelGGL((window_join_kernel<bf16_t>), grid, dim3(256), 0, stream, p, rows);
+  else hipLaunchKernelGGL((window_join_kernel<float>), grid, dim3(256), 0, stream, p, rows);
+  SK_CHECK_LAUNCH("skhip_window_attn_bwd(join)");
+  return SK_OK;
+}
+
+extern "C" int64_t skhip_window_attn_bwd_ws_floats(int B, int n_head, int n_kv, int64_t Tq, int Lq, int Lk, int d, int window,
+                                                   int sinks, int causal) {
+  if (B < 0 || n_head <= 0 || n_kv <= 0 || Tq < 0 || Lq < 0 || Lk < 0 || d <= 0 || window < 1 || sinks < 0) return 0;
+  WinParams p = {};
+  p.B = B; p.H = n_head; p.G = n_kv; p.Lq = Lq; p.Lk = Lk; p.d = d; p.sinks = sinks;
+  set_window(p, window, causal);
+  plan_sinks(p, NT);
+  return (int64_t)n_head * Tq + slab_floats(p, NT);
+}
+
+extern "C" int skhip_window_attn_fwd(const void* Q, const void* K, const void* V, void* O, float* LSE, const uint8_t* key_pad,
+                                     const int32_t* q_off, const int32_t* k_off, int B, int n_head, int n_kv, int64_t Tq,
+                                     int64_t Tk, int Lq, int Lk, int d, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo,
+                                     float scale, int window, int sinks, int causal, int dtype, void* stream_) {
+  const char* who = "skhip_window_attn_fwd";
+  hipStream_t stream = (hipStream_t)stream_;
+  WinParams p = {};
+  p.Q = Q; p.K = K; p.V = V; p.Oout = O; p.LSE = LSE; p.key_pad = key_pad; p.q_off = q_off; p.k_off = k_off;
+  p.B = B; p.H = n_head; p.G = n_kv; p.Tq = Tq; p.Tk = Tk; p.Lq = Lq; p.Lk = Lk; p.d = d;
+  p.ldq = ldq; p.ldk = ldk; p.ldv = ldv; p.ldo = ldo; p.scale = scale; p.sinks = sinks;
+  int rc = check(who, p, window, dtype);
+  if (rc) return rc;
+  if (Tq == 0) return SK_OK;
+  SK_CHECK_ARG(Q && O && LSE && (Tk == 0 || (K && V)), "%s: null pointer", who);
+  set_window(p, window, causal);
+  if (dtype == SK_BF16) {
+    if (d <= 64) launch_fwd<bf16_t, 64>(p, stream); else launch_fwd<bf16_t, 128>(p, stream);
+  } else {
+    if (d <= 64) launch_fwd<float, 64>(p, stream); else launch_fwd<float, 128>(p, stream);
+  }
+  SK_CHECK_LAUNCH(who);
+  return SK_OK;
+}
+
+extern "C" int skhip_window_attn_bwd(const void* Q, const void* K, const void* V, const void* O, const void* dO,
+                                     const float* LSE, void* dQ, void* dK, void* dV, const uint8_t* key_pad,
+                                     const int32_t* q_off, const int32_t* k_off, int B, int n_head, int n_kv, int64_t Tq,
+                                     int64_t Tk, int Lq, int Lk, int d, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo,
+                                     int64_t lddo, int64_t lddq, int64_t lddk, int64_t lddv, float scale, int window,
+                                     int sinks, int causal, float* workspace, int64_t workspace_floats, int dtype,
+                                     void* stream_) {
+  const char* who = "skhip_window_attn_bwd";
+  hipStream_t stream = (hipStream_t)stream_;
+  WinParams p = {};
+  p.Q = Q; p.K = K; p.V = V; p.O = O; p.dO = dO; p.LSE = (float*)LSE; p.dQ = dQ; p.dK = dK; p.dV = dV;
+  p.key_pad = key_pad; p.q_off = q_off; p.k_off = k_off;
+  p.B = B; p.H = n_head; p.G = n_kv; p.Tq = Tq; p.Tk = Tk; p.Lq = Lq; p.Lk = Lk; p.d = d;
+  p.ldq = ldq; p.ldk = ldk; p.ldv = ldv; p.ldo = ldo; p.lddo = lddo; p.lddq = lddq; p.lddk = lddk; p.lddv = lddv;
+  p.scale = scale; p.sinks = sinks;
+  int rc = check(who, p, window, dtype);
+  if (rc) return rc;
+  const int64_t nq = (int64_t)n_head * d, nk = (int64_t)n_kv * d;
+  SK_CHECK_ARG(lddo >= nq && lddq >= nq && lddk >= nk && lddv >= nk, "%s: row stride below the row's length", who);
+  if (Tq == 0 && Tk == 0) return SK_OK;
+  SK_CHECK_ARG((Tq == 0 || (Q && O && dO && LSE && dQ)) && (Tk == 0 || (K && V && dK && dV)), "%s: null pointer", who);
+  set_window(p, window, causal);
+  plan_sinks(p, NT);
+  const int64_t need = (int64_t)n_head * Tq + slab_floats(p, NT);
+  if (need > 0 && (!workspace || workspace_floats < need)) {
+    sk_set_error("%s: workspace of %lld floats needed", who, (long long)need);
+    return SK_ERR_WORKSPACE;
+  }
+  p.delta = workspace;
+  p.slabs = workspace + (int64_t)n_head * Tq;
+  if (dtype == SK_BF16) {
+    if (d <= 64) launch_bwd<bf16_t, 64>(p, stream); else launch_bwd<bf16_t, 128>(p, stream);
+  } else {
+    if (d <= 64) launch_bwd<float, 64>(p, stream); else launch_bwd<float, 128>(p, stream);
+  }
+  SK_CHECK_LAUNCH(who);
+  return sk_window_join(p, NT, dtype, stream);
+}

@@ -7,6 +7,7 @@ bfloat16 the kernels read bf16 working copies kept by `compute_weight` and weigh
 gradients are produced directly in fp32.
 """
 import itertools
+import math
 import weakref
 
 import contextlib
@@ -962,6 +963,282 @@ class EmbedFn(torch.autograd.Function):
         dW = torch.zeros(ctx.shape, dtype=torch.float32, device=dout.device)
         L.embed_bwd(seq, dout.contiguous(), dW, PAD)
         return None, None, dW, None, None
+
+
+# ----------------------------------------------------------------------------- rotary positions, norms of heads
+class RotaryFrequencies:
+    """The turn per position of each pair of a head's rotated part, for `rotary` and `qk_norm_rotary`.
+
+    Pair i of rot_dim / 2 turns by base^(-2i / rot_dim) radians per position.  scaling stretches this to texts longer than
+    the `trained_len` positions a model was trained on, `factor` times as long:
+      "linear"  every frequency divided by factor (position interpolation);
+      "ntk"     base * factor^(rot_dim / (rot_dim - 2)): the slowest pair is divided by factor, the fastest kept;
+      "yarn"    pairs that turn fewer than once within trained_len are divided by factor, those that turn more than 32
+                times kept, the others blended by their number of turns; rotated pairs are scaled by 0.1 ln(factor) + 1
+                (the attention temperature that goes with it).
+    Frequencies are kept as 64-bit fractions of a turn, so any int64 position has its angle without rounding."""
+
+    def __init__(self, rot_dim, base=10000.0, scaling=None, factor=1.0, trained_len=0, device="cuda"):
+        if rot_dim < 0 or rot_dim % 2:
+            raise ValueError(f"rot_dim must be even and not negative, got {rot_dim}")
+        if scaling not in (None, "linear", "ntk", "yarn"):
+            raise ValueError(f'scaling must be None, "linear", "ntk" or "yarn", got {scaling!r}')
+        if not (base > 0 and math.isfinite(base)) or not (factor > 0 and math.isfinite(factor)):
+            raise ValueError(f"base and factor must be positive, got {base} and {factor}")
+        if scaling == "ntk" and rot_dim <= 2:
+            raise ValueError('"ntk" needs more than one pair')
+        if scaling == "yarn" and trained_len <= 0:
+            raise ValueError('"yarn" needs trained_len')
+        if scaling == "ntk":
+            base = base * factor ** (rot_dim / (rot_dim - 2))
+        radians = [base ** (-2.0 * i / rot_dim) for i in range(rot_dim // 2)]
+        self.rot_dim, self.amplitude = rot_dim, 1.0
+        if scaling == "linear":
+            radians = [f / factor for f in radians]
+        elif scaling == "yarn":
+            keep = [min(1.0, max(0.0, (trained_len * f / (2 * math.pi) - 1.0) / 31.0)) for f in radians]
+            radians = [f / factor * (1.0 - g) + f * g for f, g in zip(radians, keep)]
+            self.amplitude = 0.1 * math.log(factor) + 1.0
+        words = [round(math.fmod(f / (2 * math.pi), 1.0) * 2.0 ** 64) % (1 << 64) for f in radians]
+        self.radians = radians
+        self.turns = torch.tensor([w - (1 << 64) if w >> 63 else w for w in words], dtype=torch.int64).to(device)
+
+
+def _rows(x, width, what):
+    """x as rows (T, width) that kernels can address: unit inner stride, no overlapping rows."""
+    if x.dim() != 2 or x.shape[1] != width:
+        raise ValueError(f"{what} must be (rows, {width}), got {tuple(x.shape)}")
+    return x if x.stride(1) == 1 and x.stride(0) >= width else x.contiguous()
+
+
+def _heads(x, n_head, n_kv_head, most):
+    if n_head <= 0 or n_kv_head <= 0 or n_head % n_kv_head:
+        raise ValueError(f"{n_head} query heads cannot share {n_kv_head} key heads evenly")
+    if x.dim() != 2 or x.shape[1] % n_head or not 0 < x.shape[1] // n_head <= most:
+        raise ValueError(f"q must be (rows, {n_head} heads of 1..{most} elements), got {tuple(x.shape)}")
+    return x.shape[1] // n_head
+
+
+def _same(*tensors):
+    first = tensors[0]
+    for t in tensors[1:]:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on {first.device} and {t.device}")
+
+
+class QKRotaryFn(torch.autograd.Function):
+    """(R(pos) q, R(pos) k); the gradient is the turn by the negative angles."""
+
+    @staticmethod
+    def forward(ctx, q, k, pos, freqs, n_head, n_kv, interleaved):
+        ctx.save_for_backward(pos)
+        ctx.args = (freqs.turns, freqs.amplitude, None, None, 0.0, n_head, n_kv, q.shape[1] // n_head, freqs.rot_dim, interleaved)
+        with L.on_device(q):
+            return L.qk_rotary(q, k, pos, *ctx.args)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        (pos,) = ctx.saved_tensors
+        n_head, n_kv, d = ctx.args[5:8]
+        dq = _rows(dq, n_head * d, "dq")
+        with L.on_device(dq):
+            dq, dk = L.qk_rotary(dq, None if dk is None else _rows(dk, n_kv * d, "dk"), pos, *ctx.args, inverse=True)
+        return dq, dk, None, None, None, None, None
+
+
+class QKNormRotaryFn(torch.autograd.Function):
+    """The RMS norm of every head and the turn in one pass; backward recomputes the norm from the saved inputs."""
+
+    @staticmethod
+    def forward(ctx, q, k, gamma_q, gamma_k, pos, freqs, n_head, n_kv, eps, interleaved):
+        gq, gk = gamma_q.detach(), None if gamma_k is None else gamma_k.detach()
+        rot = 0 if freqs is None else freqs.rot_dim
+        ctx.save_for_backward(q, k, gamma_q, gamma_k, pos)
+        ctx.freqs, ctx.rest = freqs, (eps, n_head, n_kv, q.shape[1] // n_head, rot, interleaved)
+        with L.on_device(q):
+            return L.qk_rotary(q, k, pos, None if freqs is None else freqs.turns, 1.0 if freqs is None else freqs.amplitude,
+                               gq, gk, *ctx.rest)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        q, k, gq, gk, pos = ctx.saved_tensors
+        f, (_, n_head, n_kv, d, _, _) = ctx.freqs, ctx.rest
+        dq = _rows(dq, n_head * d, "dq")
+        with L.on_device(q):
+            out = L.qk_norm_rotary_bwd(q, k, dq, None if k is None else _rows(dk, n_kv * d, "dk"), pos,
+                                       None if f is None else f.turns, 1.0 if f is None else f.amplitude, gq.detach(),
+                                       None if gk is None else gk.detach(), *ctx.rest)
+        return out + (None,) * 6
+
+
+def _rotary_args(q, k, pos, freqs, n_head, n_kv_head):
+    n_kv = n_head if n_kv_head is None else n_kv_head
+    d = _heads(q, n_head, n_kv, 256)
+    q = _rows(q, n_head * d, "q")
+    if k is not None:
+        k = _rows(k, n_kv * d, "k")
+        if k.shape[0] != q.shape[0] or k.dtype != q.dtype:
+            raise ValueError(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} do not go together")
+    L.dcode(q.dtype)
+    if freqs is None:
+        return q, k, None, n_kv
+    if freqs.rot_dim > d:
+        raise ValueError(f"{freqs.rot_dim} rotated elements in a head of {d}")
+    if pos is None or pos.dtype != torch.int64 or pos.numel() != q.shape[0]:
+        raise ValueError(f"pos must hold one int64 position for each of the {q.shape[0]} rows")
+    _same(q, k, pos, freqs.turns)
+    return q, k, pos.reshape(-1).contiguous(), n_kv
+
+
+def rotary(q, k, pos, freqs, n_head, n_kv_head=None, interleaved=False):
+    """Rotary positions: the first freqs.rot_dim elements of every head turned by its row's position, the others passed.
+
+    q (rows, n_head * d), k (rows, n_kv_head * d) or None (slices of a fused projection are read in place), pos int64 one
+    position a row, freqs a RotaryFrequencies.  Pairs are (i, i + rot_dim / 2) or, interleaved, (2i, 2i + 1).  Returns
+    new rows (q', k'), k' None for k None.  Differentiable in q and k."""
+    if freqs is None:
+        raise ValueError("rotary needs a RotaryFrequencies")
+    q, k, pos, n_kv = _rotary_args(q, k, pos, freqs, n_head, n_kv_head)
+    return call(QKRotaryFn, q, k, pos, freqs, n_head, n_kv, bool(interleaved))
+
+
+def qk_norm_rotary(q, k, gamma_q, gamma_k, pos, freqs, n_head, n_kv_head=None, eps=1e-6, interleaved=False):
+    """rotary of x / sqrt(mean(x^2) + eps) * gamma over every head of q and k, in one pass over the rows.
+
+    gamma_q, gamma_k: fp32 (d,), shared by the heads of q resp. k (gamma_k None with k None).  freqs None: the norm alone
+    (pos is not read).  Differentiable in q, k, gamma_q and gamma_k."""
+    q, k, pos, n_kv = _rotary_args(q, k, pos, freqs, n_head, n_kv_head)
+    d = q.shape[1] // n_head
+    if (k is None) != (gamma_k is None):
+        raise ValueError("k and gamma_k go together")
+    for g in (gamma_q, gamma_k):
+        if g is not None and (g.dtype != torch.float32 or g.shape != (d,) or not g.is_contiguous()):
+            raise ValueError(f"a norm weight must be a contiguous fp32 vector of {d}, got {g.dtype} {tuple(g.shape)}")
+    if not eps >= 0:
+        raise ValueError(f"eps {eps} is negative")
+    _same(q, k, gamma_q, gamma_k)
+    return call(QKNormRotaryFn, q, k, gamma_q, gamma_k, pos, freqs, n_head, n_kv, float(eps), bool(interleaved))
+
+
+# ----------------------------------------------------------------------------- attention within a window
+NO_WINDOW = (1 << 31) - 1
+
+
+class WindowAttnFn(torch.autograd.Function):
+    """softmax(scale q k^T on the visible pairs) v over packed or padded rows with shared key heads."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, cfg):
+        with L.on_device(q):
+            o, lse = L.window_attn_fwd(q, k, v, **cfg)
+        ctx.save_for_backward(q, k, v, o, lse)
+        ctx.cfg = cfg
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, lse = ctx.saved_tensors
+        with L.on_device(q):
+            dq, dk, dv = L.window_attn_bwd(q, k, v, o, _rows(do, o.shape[1], "do"), lse, **ctx.cfg)
+        return dq, dk, dv, None
+
+
+def _window(window):
+    if window is None:
+        return NO_WINDOW
+    if window < 1:
+        raise ValueError(f"window {window} must be at least 1")
+    return min(int(window), NO_WINDOW)
+
+
+def window_attention(q, k, v, B, Lq, Lk, n_head, n_kv_head=None, window=None, sinks=0, causal=True, scale=None,
+                     key_pad=None, q_off=None, k_off=None):
+    """Attention within a sliding window, with the first `sinks` keys always visible.
+
+    q (B * Lq, n_head * d), k, v (B * Lk, n_kv_head * d): padded rows; or, with q_off and k_off (int32 (B + 1,) row
+    offsets), packed rows, Lq and Lk then being (at least) the longest lengths.  Query i of a sequence stands at position
+    p = i + Lk - Lq (its own lengths) and sees key j when p - j < window or j < sinks, j <= p (causal) or j - p < window
+    (not causal), and key_pad[b, j] is 0.  window None: no limit.  scale defaults to 1 / sqrt(d).  d <= 128.
+    Returns (rows of q, n_head * d); a query that sees nothing, and a packed row outside every sequence, gets zeros.
+    Differentiable in q, k and v; the result does not depend on what masked keys and values hold unless another query of
+    the sequence sees them."""
+    n_kv = n_head if n_kv_head is None else n_kv_head
+    d = _heads(q, n_head, n_kv, 128)
+    q, k, v = _rows(q, n_head * d, "q"), _rows(k, n_kv * d, "k"), _rows(v, n_kv * d, "v")
+    if k.shape[0] != v.shape[0] or not q.dtype == k.dtype == v.dtype:
+        raise ValueError(f"k {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype} and q of {q.dtype} do not go together")
+    L.dcode(q.dtype)
+    if B < 0 or Lq < 0 or Lk < 0 or sinks < 0:
+        raise ValueError(f"B {B}, Lq {Lq}, Lk {Lk} and sinks {sinks} must not be negative")
+    if (q_off is None) != (k_off is None):
+        raise ValueError("q_off and k_off go together")
+    if q_off is not None:
+        if key_pad is not None:
+            raise ValueError("packed rows take no key_pad")
+        for o in (q_off, k_off):
+            if o.dtype != torch.int32 or o.shape != (B + 1,) or not o.is_contiguous():
+                raise ValueError(f"row offsets must be contiguous int32 ({B + 1},), got {o.dtype} {tuple(o.shape)}")
+    elif q.shape[0] != B * Lq or k.shape[0] != B * Lk:
+        raise ValueError(f"{q.shape[0]} query and {k.shape[0]} key rows are not {B} x {Lq} and {B} x {Lk}")
+    if key_pad is not None:
+        if key_pad.shape != (B, Lk) or key_pad.dtype not in (torch.uint8, torch.bool):
+            raise ValueError(f"key_pad must be uint8 or bool ({B}, {Lk}), got {key_pad.dtype} {tuple(key_pad.shape)}")
+        key_pad = key_pad.contiguous().view(torch.uint8)
+    _same(q, k, v, key_pad, q_off, k_off)
+    cfg = dict(B=B, Lq=Lq, Lk=Lk, n_head=n_head, n_kv=n_kv, d=d, scale=d ** -0.5 if scale is None else float(scale),
+               window=_window(window), sinks=min(int(sinks), NO_WINDOW), causal=bool(causal), key_pad=key_pad, q_off=q_off,
+               k_off=k_off)
+    return call(WindowAttnFn, q, k, v, cfg)
+
+
+def window_attention_step(q, k_new, v_new, k_cache, v_cache, kv_len, n_head, n_kv_head=None, window=None, sinks=0,
+                          scale=None):
+    """window_attention (causal) of one new query per sequence over a cache of keys and values, for generation.
+
+    q (R, n_head * d); k_cache, v_cache (R, cap, n_kv_head * d), any row and position strides; kv_len int32 (R,): positions
+    of each sequence including the new one.  Position j is kept in slot j while j < sinks, else in slot
+    sinks + (j - sinks) % (cap - sinks): a cache with cap >= every kv_len keeps everything, one with cap = sinks + window
+    is a ring that never overflows.  cap - sinks >= window is required; window None takes cap - sinks (every position,
+    while kv_len <= cap).  k_new, v_new (R, n_kv_head * d): the new position's key and value, stored into the caches by
+    this call (both None: the caches hold them already).  Returns (R, n_head * d); sequences with kv_len <= 0 get zeros
+    and store nothing.  No gradient."""
+    n_kv = n_head if n_kv_head is None else n_kv_head
+    d = _heads(q, n_head, n_kv, 128)
+    q = _rows(q, n_head * d, "q")
+    R, w = q.shape[0], n_kv * d
+    L.dcode(q.dtype)
+    if (k_new is None) != (v_new is None):
+        raise ValueError("k_new and v_new go together")
+    if k_cache.dim() != 3 or k_cache.shape[0] != R or k_cache.shape[2] != w or v_cache.shape != k_cache.shape:
+        raise ValueError(f"caches must be ({R}, cap, {w}), got {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
+    cap = k_cache.shape[1]
+    for c in (k_cache, v_cache):
+        s0, s1, s2 = c.stride()
+        if s2 != 1 or s1 < w or s0 < 0 or (R > 1 and s0 < (cap - 1) * s1 + w and (s0 < w or s1 < (R - 1) * s0 + w)):
+            raise ValueError(f"cache rows overlap or are not contiguous (strides {c.stride()})")
+    if k_new is not None:
+        k_new, v_new = _rows(k_new, w, "k_new"), _rows(v_new, w, "v_new")
+        if k_new.stride(0) != v_new.stride(0):
+            k_new, v_new = k_new.contiguous(), v_new.contiguous()
+        if k_new.shape[0] != R or v_new.shape[0] != R:
+            raise ValueError(f"k_new and v_new must have {R} rows")
+    for t in (k_new, v_new, k_cache, v_cache):
+        if t is not None and t.dtype != q.dtype:
+            raise ValueError(f"q is {q.dtype}, a key or value {t.dtype}")
+    if kv_len.dtype != torch.int32 or kv_len.shape != (R,) or not kv_len.is_contiguous():
+        raise ValueError(f"kv_len must be contiguous int32 ({R},), got {kv_len.dtype} {tuple(kv_len.shape)}")
+    window = cap - sinks if window is None else _window(window)
+    if sinks < 0 or window < 1 or cap - sinks < window:
+        raise ValueError(f"a cache of {cap} slots cannot hold {sinks} sinks and a window of {window}")
+    _same(q, k_new, v_new, k_cache, v_cache, kv_len)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k_new, v_new, k_cache, v_cache)):
+        raise RuntimeError("window_attention_step has no gradient: call it under torch.no_grad() or on detached tensors")
+    with L.on_device(q):
+        return L.window_attn_step(q, k_new, v_new, k_cache, v_cache, kv_len, n_head, n_kv, d,
+                                  d ** -0.5 if scale is None else float(scale), window, int(sinks))
 
 
 # ----------------------------------------------------------------------------- loss

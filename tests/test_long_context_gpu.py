@@ -1,0 +1,634 @@
+"""Rotary positions, query / key norms and windowed attention against plain implementations in 64 bits.
+
+Tolerances are bounds per element, from the roundings a result goes through: U = half a step of the storage type (2^-8
+bf16, 2^-24 fp32) for every value that is stored in it, E = 2^-24 for every fp32 operation, multiplied by the absolute
+values that the rounded quantities meet on the way to the element."""
+import math
+
+import pytest
+import torch
+
+from specialk_amd import _lib as L
+from specialk_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+BF, F32 = torch.bfloat16, torch.float32
+E = 2.0 ** -24
+TINY = 1e-30
+
+
+def unit(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def rnd(shape, dtype, g, scale=1.0):
+    return (torch.randn(shape, generator=g) * scale).to(dtype)
+
+
+def check(got, want, bound, what):
+    got, want = got.detach().double().cpu(), want.double().cpu()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    over = (got - want).abs() - bound.cpu()
+    assert bool((over <= 0).all()), f"{what}: off by {(got - want).abs().max():.3g}, worst over its bound by {over.max():.3g}"
+
+
+# ------------------------------------------------------------------------------ rotary and norm
+def turn64(x, pos, f, rot, il, sign=1):
+    """x (T, heads, d) with its first rot elements turned, in 64 bits; also |a| + |b| of every element's pair."""
+    ang = sign * pos.double()[:, None] * torch.tensor(f.radians, dtype=torch.float64)[None]
+    c, s = (torch.cos(ang) * f.amplitude)[:, None], (torch.sin(ang) * f.amplitude)[:, None]
+    h = x[..., :rot]
+    a, b = (h[..., 0::2], h[..., 1::2]) if il else (h[..., :rot // 2], h[..., rot // 2:])
+    y0, y1 = a * c - b * s, b * c + a * s
+    m = a.abs() + b.abs()
+    join = (lambda u, v: torch.stack((u, v), -1).flatten(-2)) if il else (lambda u, v: torch.cat((u, v), -1))
+    return torch.cat((join(y0, y1), x[..., rot:]), -1), torch.cat((join(m, m) * f.amplitude, x[..., rot:].abs()), -1)
+
+
+# cosine and sine: argument rounded twice (2 E x <= 2 E), a polynomial of six terms, two products, one sum
+ROT_E = 12 * E
+
+
+def rotary_case(T, H, G, d, rot, dtype, il, far, gen, **kw):
+    f = ops.RotaryFrequencies(rot, device=DEV, **kw)
+    pos = torch.randint(0, 300, (T,), generator=gen) + far
+    q, k = rnd((T, H * d), dtype, gen, 1.5), rnd((T, G * d), dtype, gen, 1.5)
+    return f, pos, q, k
+
+
+SHAPES = [  # T, H, G, d, rot
+    (1, 1, 1, 64, 64), (640, 8, 8, 64, 64), (37, 8, 2, 128, 64), (5, 3, 1, 80, 80), (19, 4, 4, 96, 48), (1030, 2, 1, 32, 32),
+    (7, 5, 5, 37, 18), (3, 2, 2, 256, 256), (66, 16, 16, 16, 2), (2, 40, 8, 128, 128), (9, 1, 1, 3, 2), (8, 512, 512, 64, 30)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("il", [False, True])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_rotary(shape, il, dtype):
+    T, H, G, d, rot = shape
+    g = torch.Generator().manual_seed(T * 7 + d)
+    f, pos, q, k = rotary_case(T, H, G, d, rot, dtype, il, 0, g)
+    dq, dk = rnd((T, H * d), dtype, g), rnd((T, G * d), dtype, g)
+    qd, kd = q.to(DEV).requires_grad_(), k.to(DEV).requires_grad_()
+    oq, ok = ops.rotary(qd, kd, pos.to(DEV), f, H, G, interleaved=il)
+    gq, gk = torch.autograd.grad((oq, ok), (qd, kd), (dq.to(DEV), dk.to(DEV)))
+    for x, out, dy, dx in ((q, oq, dq, gq), (k, ok, dk, gk)):
+        for src, got, sign, what in ((x, out, 1, "forward"), (dy, dx, -1, "gradient")):
+            want, mag = turn64(src.double().view(T, -1, d), pos, f, rot, il, sign)
+            check(got, want.view(T, -1), (unit(dtype) * want.abs() + ROT_E * mag).view(T, -1) + TINY, what)
+
+
+@pytest.mark.parametrize("scaling", [None, "linear", "ntk", "yarn"])
+@pytest.mark.parametrize("far", [0, 100000, 1 << 31, -70000])
+def test_rotary_far_positions(far, scaling):
+    """Angles of far positions: exact but for the reference's own product pos * f, rounded to 2^-53 of the angle."""
+    g = torch.Generator().manual_seed(3)
+    f, pos, q, k = rotary_case(50, 2, 1, 64, 64, F32, False, far, g, scaling=scaling, factor=8.0, trained_len=4096)
+    out, _ = ops.rotary(q.to(DEV), None, pos.to(DEV), f, 2, interleaved=False)
+    want, mag = turn64(q.double().view(50, 2, 64), pos, f, 64, False)
+    own = pos.abs().max().item() * 2.0 ** -52
+    check(out, want.view(50, -1), (E * want.abs() + (ROT_E + own) * mag).view(50, -1), "far")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_rotary_reads_slices_and_odd_strides(dtype):
+    """Slices of a fused projection (16-byte rows), the same one element off (scalar form), transposed rows: one result."""
+    g = torch.Generator().manual_seed(8)
+    T, H, d = 33, 4, 64
+    f = ops.RotaryFrequencies(64, device=DEV)
+    pos = torch.arange(T, device=DEV)
+    x = rnd((T, H * d), dtype, g).to(DEV)
+    want, _ = ops.rotary(x, None, pos, f, H)
+    wide = torch.zeros((T, 3 * H * d + 8), dtype=dtype, device=DEV)
+    for off in (0, 8, H * d, 1, 3):
+        wide[:, off:off + H * d] = x
+        got, _ = ops.rotary(wide[:, off:off + H * d], None, pos, f, H)
+        assert torch.equal(got, want), off
+    got, _ = ops.rotary(x.t().contiguous().t(), None, pos, f, H)
+    assert torch.equal(got, want)
+    one, _ = ops.rotary(x[:1].expand(T, -1), None, pos, f, H)
+    assert torch.equal(one, ops.rotary(x[:1].repeat(T, 1), None, pos, f, H)[0])
+
+
+def norm64(x, gamma, eps, pos, f, rot, il):
+    y = x / (x.pow(2).mean(-1, keepdim=True) + eps).sqrt() * gamma
+    return (y, y.abs()) if f is None else turn64(y, pos, f, rot, il)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("il", [False, True])
+@pytest.mark.parametrize("shape", SHAPES[:-1] + [(6000, 8, 8, 64, 64), (25, 4, 2, 64, 0)])
+def test_qk_norm_rotary(shape, il, dtype):
+    T, H, G, d, rot = shape
+    g = torch.Generator().manual_seed(T + d)
+    f, pos, q, k = rotary_case(T, H, G, d, max(rot, 2), dtype, il, 5, g)
+    if rot == 0:
+        f = None
+    eps = 1e-5
+    gq, gk = 1 + 0.3 * torch.randn(d, generator=g), 1 + 0.3 * torch.randn(d, generator=g)
+    dq, dk = rnd((T, H * d), dtype, g), rnd((T, G * d), dtype, g)
+    leaves = [t.to(DEV).requires_grad_() for t in (q, k, gq, gk)]
+    out = ops.qk_norm_rotary(*leaves, None if f is None else pos.to(DEV), f, H, G, eps=eps, interleaved=il)
+    grads = torch.autograd.grad(out, leaves, (dq.to(DEV), dk.to(DEV)))
+    # the mean of d squares, root, reciprocal, two products: relative to the normalised value
+    rel = (d + 8) * E
+    for x, gm, dy, y, dx, dg in ((q, gq, dq, out[0], grads[0], grads[2]), (k, gk, dk, out[1], grads[1], grads[3])):
+        x64 = x.double().view(T, -1, d).requires_grad_()
+        g64 = gm.double().requires_grad_()
+        want, mag = norm64(x64, g64, eps, pos, f, rot, il)
+        check(y, want.detach().view(T, -1), (unit(dtype) * want.abs() + (ROT_E + rel) * mag).detach().view(T, -1) + TINY, "forward")
+        dx64, dg64 = torch.autograd.grad(want, (x64, g64), dy.double().view(T, -1, d))
+        # by the formula: r = R^T dy, dx = rstd (r gamma - xhat mean(r gamma xhat))
+        r, rmag = (dy.double().view(T, -1, d),) * 2 if f is None else turn64(dy.double().view(T, -1, d), pos, f, rot, il, -1)
+        rmag = rmag.abs()
+        xd = x.double().view(T, -1, d)
+        rstd = 1 / (xd.pow(2).mean(-1, keepdim=True) + eps).sqrt()
+        xhat = xd * rstd
+        mean = (r * gm.double() * xhat).mean(-1, keepdim=True)
+        formula = rstd * (r * gm.double() - xhat * mean)
+        torch.testing.assert_close(dx64, formula, rtol=1e-9, atol=1e-9)
+        mabs = (rmag * gm.double().abs() * xhat.abs()).mean(-1, keepdim=True)
+        bound = unit(dtype) * formula.abs() + rstd * (rmag * gm.double().abs() + xhat.abs() * mabs) * (ROT_E + (2 * d + 16) * E)
+        check(dx, dx64.view(T, -1), bound.view(T, -1) + TINY, "dx")
+        # dgamma: terms r xhat, added by a thread over its rows, then lanes, waves and blocks: chains of 128 + T / 64 at most
+        terms = (rmag * xhat.abs()).sum((0, 1))
+        check(dg, dg64, terms * (ROT_E + rel + (128 + T / 64) * E) + TINY, "dgamma")
+
+
+def test_qk_norm_rotary_gradient_by_differences():
+    g = torch.Generator().manual_seed(1)
+    T, H, d = 3, 2, 16
+    f = ops.RotaryFrequencies(8, device=DEV)
+    pos = torch.tensor([0, 4, 9], device=DEV)
+    x, w = torch.randn((T, H * d), generator=g), torch.randn((T, H * d), generator=g).to(DEV)
+    gm = (1 + 0.2 * torch.randn(d, generator=g)).to(DEV)
+
+    def loss(t):
+        return (ops.qk_norm_rotary(t, None, gm, None, pos, f, H)[0].double() * w.double()).sum()
+
+    leaf = x.to(DEV).requires_grad_()
+    (grad,) = torch.autograd.grad(loss(leaf), leaf)
+    h = 2.0 ** -7
+    for i, j in ((0, 0), (1, 5), (2, 20), (2, 31)):
+        step = torch.zeros_like(x)
+        step[i, j] = h
+        diff = (loss((x + step).to(DEV)) - loss((x - step).to(DEV))) / (2 * h)
+        # third derivatives of x / rms(x) are below 100 here: 100 h^2 / 6; and 64 outputs rounded to E over 2 h
+        assert abs(diff.item() - grad[i, j].item()) <= 100 * h * h / 6 + 64 * 8 * E / (2 * h), (i, j)
+
+
+def test_norm_row_of_zeros_and_large_values():
+    f = ops.RotaryFrequencies(64, device=DEV)
+    x = torch.zeros((3, 64), device=DEV)
+    x[1] = 3e18      # squares near the largest fp32
+    x[2, 5] = float("inf")
+    out, _ = ops.qk_norm_rotary(x, None, torch.ones(64, device=DEV), None, torch.zeros(3, dtype=torch.int64, device=DEV), f, 1)
+    assert torch.equal(out[0], torch.zeros(64, device=DEV))
+    assert bool((out[1] - 1).abs().max() <= 80 * E)
+    assert bool(torch.isnan(out[2, 5]))
+
+
+def test_empty_rows():
+    f = ops.RotaryFrequencies(64, device=DEV)
+    x = torch.empty((0, 128), device=DEV, requires_grad=True)
+    gm = torch.ones(64, device=DEV, requires_grad=True)
+    out, _ = ops.qk_norm_rotary(x, None, gm, None, torch.empty(0, dtype=torch.int64, device=DEV), f, 2)
+    dx, dg = torch.autograd.grad(out, (x, gm), torch.empty_like(out))
+    assert out.shape == (0, 128) and dx.shape == (0, 128) and torch.equal(dg, torch.zeros(64, device=DEV))
+
+
+# ------------------------------------------------------------------------------ windowed attention
+def visible(n, m, window, sinks, causal, pad=None):
+    p = torch.arange(n)[:, None] + m - n
+    j = torch.arange(m)[None]
+    v = ((p - j < window) | (j < sinks)) & ((j <= p) if causal else (j - p < window))
+    return v if pad is None else v & ~pad.bool()[None]
+
+
+def attention64(q, k, v, do, vis, scale, dtype):
+    """One sequence and query head: (o, dq, dk, dv) in 64 bits and a bound on each (fp32 operations, values rounded to dtype).
+    bf16 products take the probabilities and dS rounded to bf16; delta = rowsum(dO O) takes the rounded output."""
+    q, k, v, do = (t.double() for t in (q, k, v, do))
+    n, d = vis.sum(1).max().item(), q.shape[1]
+    some = vis.any(1, keepdim=True)
+    s = (q @ k.t() * scale).masked_fill(~vis, -math.inf)
+    s = torch.where(some, s, torch.zeros_like(s))
+    p = torch.softmax(s, 1) * vis
+    o = p @ v
+    dp = do @ v.t()
+    delta = (do * o).sum(1, keepdim=True)
+    ds = p * (dp - delta) * scale
+    dq, dk, dv = ds @ k, ds.t() @ q, p.t() @ do
+    ub = unit(dtype) if dtype == BF else 0.0                   # operands of the matrix products
+    u = unit(dtype)
+    smax = (q.abs() @ k.abs().t() * scale * vis).max()
+    rel = (2 * (d + 6) * smax + 2 * n + 16) * E                # of a probability: score, exponential, row sum
+    a = p @ v.abs()
+    eo = u * o.abs() + a * (ub + rel)
+    edelta = (do.abs() * eo).sum(1, keepdim=True) + (d + 2) * E * (do.abs() * o.abs()).sum(1, keepdim=True)
+    edp = (d + 2) * E * (do.abs() @ v.abs().t())
+    eds = ds.abs() * (ub + rel + 4 * E) + p * scale * (edelta + edp)
+    acc = (max(vis.shape) + 8) * E
+    return ((o, eo), (dq, u * dq.abs() + eds @ k.abs() + acc * ds.abs() @ k.abs()),
+            (dk, u * dk.abs() + eds.t() @ q.abs() + acc * ds.abs().t() @ q.abs()),
+            (dv, u * dv.abs() + (p * (ub + rel + acc)).t() @ do.abs()))
+
+
+def run_window(lens_q, lens_k, H, G, d, window, sinks, causal, dtype, layout, seed=0, scale=None, pads=None):
+    """All sequences against attention64; returns nothing, raises where an element leaves its bound."""
+    g = torch.Generator().manual_seed(seed + d)
+    B, Lq, Lk = len(lens_q), max(lens_q), max(lens_k)
+    tq, tk = (sum(lens_q), sum(lens_k)) if layout == "packed" else (B * Lq, B * Lk)
+    q, k, v, do = rnd((tq, H * d), dtype, g), rnd((tk, G * d), dtype, g), rnd((tk, G * d), dtype, g), rnd((tq, H * d), dtype, g)
+    kw = {}
+    if layout == "packed":
+        kw = dict(q_off=torch.tensor([0] + lens_q).cumsum(0).int().to(DEV), k_off=torch.tensor([0] + lens_k).cumsum(0).int().to(DEV))
+    elif pads is not None:
+        kw = dict(key_pad=pads.to(DEV))
+    qd, kd, vd = (t.to(DEV).requires_grad_() for t in (q, k, v))
+    o = ops.window_attention(qd, kd, vd, B, Lq, Lk, H, G, window, sinks, causal, scale, **kw)
+    grads = torch.autograd.grad(o, (qd, kd, vd), do.to(DEV))
+    sc = d ** -0.5 if scale is None else scale
+    want = [torch.zeros((t, w * d), dtype=torch.float64) for t, w in ((tq, H), (tq, H), (tk, G), (tk, G))]
+    bound = [torch.zeros_like(t) + TINY for t in want]
+    q0 = k0 = 0
+    for b in range(B):
+        n, m = (lens_q[b], lens_k[b]) if layout == "packed" else (Lq, Lk)
+        vis = visible(n, m, window or 1 << 30, sinks, causal, None if pads is None else pads[b])
+        for h in range(H if n and m else 0):
+            hs, ks = slice(h * d, h * d + d), slice(h // (H // G) * d, h // (H // G) * d + d)
+            kk = k[k0:k0 + m, ks]
+            vv = v[k0:k0 + m, ks]
+            res = attention64(q[q0:q0 + n, hs], kk, vv, do[q0:q0 + n, hs], vis, sc, dtype)
+            for i, (rs, cs) in enumerate(((slice(q0, q0 + n), hs), (slice(q0, q0 + n), hs), (slice(k0, k0 + m), ks), (slice(k0, k0 + m), ks))):
+                want[i][rs, cs] += res[i][0]
+                bound[i][rs, cs] += res[i][1]
+        q0, k0 = q0 + n, k0 + m
+    for got, w, bd, what in zip((o,) + grads, want, bound, ("o", "dq", "dk", "dv")):
+        check(got, w, bd, what)
+    return o, grads
+
+
+WINDOWS = [  # lens_q, lens_k, H, G, d, window, sinks, causal
+    ([1], [1], 1, 1, 64, 1, 0, True),
+    ([5], [5], 2, 2, 64, 2, 1, True),
+    ([200], [200], 2, 1, 64, 33, 4, True),
+    ([130], [130], 2, 2, 128, 64, 0, False),
+    ([300], [300], 4, 1, 128, 40, 70, True),        # sinks over more than one tile
+    ([257], [257], 2, 2, 32, 1000, 3, True),        # window beyond the text: plain causal
+    ([190], [190], 1, 1, 80, 17, 2, False),
+    ([64], [333], 2, 1, 64, 50, 5, True),           # queries at the end of a longer text
+    ([150], [70], 2, 2, 64, 20, 2, True),           # more queries than keys: the first see nothing
+    ([700], [700], 1, 1, 64, 20, 130, True),        # far queries in chunks, two sink tiles
+    ([100], [100], 2, 2, 40, 10, 1, True),
+    ([90], [90], 3, 3, 37, 12, 3, False),           # odd head size
+    ([65, 1, 129], [65, 1, 129], 2, 1, 96, 30, 2, True)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("case", WINDOWS)
+def test_window_attention(case, dtype):
+    lens_q, lens_k, H, G, d, window, sinks, causal = case
+    layout = "packed" if len(lens_q) > 1 else "dense"
+    run_window(lens_q, lens_k, H, G, d, window, sinks, causal, dtype, layout)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("causal", [True, False])
+def test_window_packed_ragged(causal, dtype):
+    """Sequences of no, one and many rows, queries and keys of different lengths."""
+    run_window([0, 1, 70, 3, 128, 0, 65], [2, 1, 90, 0, 128, 0, 64], 2, 1, 64, 25, 3, causal, dtype, "packed")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("d", [64, 128])
+def test_window_key_padding(d, dtype):
+    """Padding on the right, on the left, everywhere, in the middle: rows that are left with nothing give zeros."""
+    B, n = 5, 150
+    pads = torch.zeros((B, n), dtype=torch.uint8)
+    pads[1, 90:] = 1
+    pads[2, :100] = 1
+    pads[3] = 1
+    pads[4, 40:110:3] = 1
+    o, grads = run_window([n] * B, [n] * B, 2, 2, d, 20, 2, True, dtype, "padded", pads=pads)
+    assert not o.view(B, n, -1)[3].any() and not any(t.view(B, n, -1)[3].any() for t in grads)
+    assert not o.view(B, n, -1)[2, :100].any()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_window_none_and_scale(dtype):
+    run_window([140], [140], 2, 1, 64, None, 0, True, dtype, "dense", scale=0.3)
+    run_window([140], [140], 2, 1, 64, None, 9, False, dtype, "dense")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("d", [64, 128, 80])
+def test_masked_places_may_hold_anything(d, dtype):
+    """Padded keys, keys that no query reaches and rows behind the last sequence hold NaN and infinities."""
+    g = torch.Generator().manual_seed(5)
+    B, n, H = 2, 200, 2
+    q, k, v, do = (rnd((B * n, H * d), dtype, g).to(DEV) for _ in range(4))
+    pads = torch.zeros((B, n), dtype=torch.uint8, device=DEV)
+    pads[0, 120:] = 1
+    pads[1, :33] = 1
+    bad = pads.view(-1).bool()
+
+    def run(k, v):
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        o = ops.window_attention(*leaves, B, n, n, H, H, 40, 4, key_pad=pads)
+        return (o,) + torch.autograd.grad(o, leaves, do)
+
+    want = run(k.masked_fill(bad[:, None], 0.0), v.masked_fill(bad[:, None], 0.0))
+    for fill in (float("nan"), float("inf"), torch.finfo(dtype).min):
+        for a, b in zip(run(k.masked_fill(bad[:, None], fill), v.masked_fill(bad[:, None], fill)), want):
+            assert torch.equal(a, b), fill
+    # the last 20 queries of a text: keys before their windows are out of every query's reach
+    lo = n - 20 - 39
+    kk, vv = k[:n].clone(), v[:n].clone()
+    base = ops.window_attention(q[:20], kk, vv, 1, 20, n, H, H, 40, 4)
+    kk[4:lo], vv[4:lo] = float("nan"), float("-inf")
+    assert torch.equal(ops.window_attention(q[:20], kk, vv, 1, 20, n, H, H, 40, 4), base)
+    # packed rows before the first and behind the last sequence
+    off = torch.tensor([3, 60, 111], dtype=torch.int32, device=DEV)
+    kk, vv, qq, dd = (t[:n].clone() for t in (k, v, q, do))
+    for t in (kk, vv, qq, dd):
+        t[:3], t[111:] = float("nan"), float("inf")
+    leaves = [t.requires_grad_() for t in (qq, kk, vv)]
+    o = ops.window_attention(*leaves, 2, 60, 60, H, H, 40, 4, q_off=off, k_off=off)
+    for t in (o,) + torch.autograd.grad(o, leaves, dd):
+        assert bool(torch.isfinite(t).all()) and not t[:3].any() and not t[111:].any() and bool(t[3:111].any())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_window_strides_and_alignment(dtype):
+    """Heads inside a fused projection, rows one element off, transposed storage: the result of contiguous rows."""
+    g = torch.Generator().manual_seed(2)
+    n, H, G, d = 150, 4, 2, 64
+    q, k, v = rnd((n, H * d), dtype, g).to(DEV), rnd((n, G * d), dtype, g).to(DEV), rnd((n, G * d), dtype, g).to(DEV)
+    do = rnd((n, H * d), dtype, g).to(DEV)
+
+    def run(q, k, v, do):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        o = ops.window_attention(*leaves, 1, n, n, H, G, 30, 2)
+        return (o,) + torch.autograd.grad(o, leaves, do)
+
+    want = run(q, k, v, do)
+    for shift in (0, 8, 1):
+        wide = torch.zeros((n, (H + 2 * G) * d + 16), dtype=dtype, device=DEV)
+        cut = wide[:, shift:shift + (H + 2 * G) * d]
+        cut[:, :H * d], cut[:, H * d:(H + G) * d], cut[:, (H + G) * d:] = q, k, v
+        dw = torch.zeros((n, H * d + 9), dtype=dtype, device=DEV)
+        dw[:, shift:shift + H * d] = do
+        got = run(cut[:, :H * d], cut[:, H * d:(H + G) * d], cut[:, (H + G) * d:], dw[:, shift:shift + H * d])
+        for a, b, name in zip(got, want, ("o", "dq", "dk", "dv")):
+            if shift % 8 == 0 or dtype == F32:
+                assert torch.equal(a, b), (shift, name)
+            else:   # another kernel: same definition, both within the bounds that run_window checks
+                torch.testing.assert_close(a.float(), b.float(), rtol=0.05, atol=0.05)
+    for a, b in zip(run(q.t().contiguous().t(), k, v, do.t().contiguous().t()), want):
+        assert torch.equal(a, b)
+    # a gradient that autograd hands over expanded
+    leaf = q.clone().requires_grad_()
+    (dq,) = torch.autograd.grad(ops.window_attention(leaf, k, v, 1, n, n, H, G, 30, 2).sum(), leaf)
+    assert torch.equal(dq, run(q, k, v, torch.ones_like(do))[1])
+
+
+def test_window_gradient_by_differences():
+    g = torch.Generator().manual_seed(4)
+    n, H, G, d = 40, 2, 1, 16
+    t = [torch.randn((n, w * d), generator=g) for w in (H, G, G)]
+    w = torch.randn((n, H * d), generator=g).to(DEV).double()
+
+    def loss(*x):
+        return (ops.window_attention(*x, 1, n, n, H, G, 7, 2).double() * w).sum()
+
+    leaves = [x.to(DEV).requires_grad_() for x in t]
+    grads = torch.autograd.grad(loss(*leaves), leaves)
+    h = 2.0 ** -6
+    for which in range(3):
+        for i, j in ((0, 0), (1, 3), (17, 9), (39, 15)):
+            step = torch.zeros_like(t[which])
+            step[i, j] = h
+            up = loss(*((x + step if a == which else x).to(DEV) for a, x in enumerate(t)))
+            down = loss(*((x - step if a == which else x).to(DEV) for a, x in enumerate(t)))
+            diff = ((up - down) / (2 * h)).item()
+            # third derivatives along one entry of q or k: up to 80 outputs, each below 2; outputs rounded to 8 E of size 3
+            assert abs(diff - grads[which][i, j].item()) <= 160 * h * h / 6 + n * H * d * 24 * E / (2 * h) / 10, (which, i, j)
+
+
+def test_window_results_repeat_bit_for_bit():
+    g = torch.Generator().manual_seed(6)
+    n, H, G, d = 1500, 4, 1, 64
+    q, k, v, do = (rnd((n, w * d), BF, g).to(DEV) for w in (H, G, G, H))
+    first = None
+    for _ in range(3):
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        o = ops.window_attention(*leaves, 1, n, n, H, G, 100, 4)
+        res = (o,) + torch.autograd.grad(o, leaves, do)
+        first = first or res
+        assert all(torch.equal(a, b) for a, b in zip(res, first))
+
+
+# ------------------------------------------------------------------------------ one step over a cache
+def slot_of(j, cap, sinks):
+    return j if j < sinks else sinks + (j - sinks) % (cap - sinks)
+
+
+def step_case(lens, H, G, d, cap, window, sinks, dtype, seed=0, fill=float("nan")):
+    """Caches filled as a run would have left them (everything else `fill`), new rows, and the 64-bit result with bounds."""
+    g = torch.Generator().manual_seed(seed + d)
+    R = len(lens)
+    q, kn, vn = rnd((R, H * d), dtype, g), rnd((R, G * d), dtype, g), rnd((R, G * d), dtype, g)
+    kc = torch.full((R, cap, G * d), fill, dtype=dtype)
+    vc = kc.clone()
+    want, bound = torch.zeros((R, H * d), dtype=torch.float64), torch.full((R, H * d), TINY, dtype=torch.float64)
+    for r, n in enumerate(lens):
+        if n <= 0:
+            continue
+        pos = [j for j in range(n) if j >= n - window or j < sinks]
+        k, v = rnd((len(pos), G * d), dtype, g), rnd((len(pos), G * d), dtype, g)
+        k[-1], v[-1] = kn[r], vn[r]
+        for i, j in enumerate(pos[:-1]):
+            kc[r, slot_of(j, cap, sinks)], vc[r, slot_of(j, cap, sinks)] = k[i], v[i]
+        for h in range(H):
+            hs, ks = slice(h * d, h * d + d), slice(h // (H // G) * d, h // (H // G) * d + d)
+            vis = torch.ones((1, len(pos)), dtype=torch.bool)
+            (o, eo), *_ = attention64(q[r:r + 1, hs], k[:, ks], v[:, ks], q[r:r + 1, hs], vis, d ** -0.5, dtype)
+            want[r, hs], bound[r, hs] = o[0], bound[r, hs] + eo[0]
+    return q, kn, vn, kc, vc, want, bound
+
+
+STEPS = [  # lens, H, G, d, cap, window, sinks
+    ([1], 1, 1, 64, 8, 8, 0), ([5, 1, 0, 7, -3], 8, 8, 64, 16, 8, 2), ([100, 33], 8, 2, 128, 100, 64, 4),
+    ([70, 69, 68, 300], 4, 1, 64, 68, 64, 4),            # rings, just full, one over, far over
+    ([5000], 8, 8, 64, 5000, 4096, 1), ([4000, 9, 2500], 16, 2, 128, 1030, 1024, 6), ([50, 200], 3, 1, 80, 40, 33, 7),
+    ([90], 2, 2, 37, 95, 40, 3), ([300, 20], 32, 1, 64, 200, 150, 0), ([1000] * 3, 6, 2, 96, 1000, 1000, 0),
+    ([40000], 2, 1, 128, 600, 512, 60)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("case", STEPS)
+def test_window_step(case, dtype):
+    lens, H, G, d, cap, window, sinks = case
+    q, kn, vn, kc, vc, want, bound = step_case(*case, dtype)
+    kd, vd = kc.to(DEV), vc.to(DEV)
+    n = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    o = ops.window_attention_step(q.to(DEV), kn.to(DEV), vn.to(DEV), kd, vd, n, H, G, window, sinks)
+    check(o, want, bound, "o")
+    for r, m in enumerate(lens):   # the new rows are in their slots, nothing else has changed
+        if m > 0:
+            kc[r, slot_of(m - 1, cap, sinks)], vc[r, slot_of(m - 1, cap, sinks)] = kn[r], vn[r]
+    for got, ref in ((kd, kc), (vd, vc)):
+        assert torch.equal(torch.nan_to_num(got.cpu(), 7.0), torch.nan_to_num(ref, 7.0))
+        assert torch.equal(got.cpu().isnan(), ref.isnan())
+    # with the rows in the caches already
+    assert torch.equal(ops.window_attention_step(q.to(DEV), None, None, kd, vd, n, H, G, window, sinks), o)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_step_cache_layouts(dtype):
+    """Keys and values side by side, position-major caches, rows one element off: the result of plain caches."""
+    lens, H, G, d, cap, window, sinks = [100, 40, 260], 4, 2, 64, 104, 100, 4
+    q, kn, vn, kc, vc, _, _ = step_case(lens, H, G, d, cap, window, sinks, dtype, fill=0.0)
+    n = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    args = (q.to(DEV), kn.to(DEV), vn.to(DEV))
+    k0, v0 = kc.to(DEV), vc.to(DEV)
+    want = ops.window_attention_step(*args, k0, v0, n, H, G, window, sinks)
+    both = torch.stack((kc, vc), 2).to(DEV)
+    major = [t.transpose(0, 1).contiguous().to(DEV).transpose(0, 1) for t in (kc, vc)]
+    odd = torch.zeros((2, 3, cap, G * d + 1), dtype=dtype, device=DEV)
+    odd[0, ..., 1:], odd[1, ..., 1:] = kc.to(DEV), vc.to(DEV)
+    for k, v in ((both[:, :, 0], both[:, :, 1]), major, (odd[0, ..., 1:], odd[1, ..., 1:])):
+        got = ops.window_attention_step(*args, k, v, n, H, G, window, sinks)
+        torch.testing.assert_close(got.float(), want.float(), rtol=2.0 ** -6 if dtype == BF else 1e-5,
+                                   atol=2.0 ** -6 if dtype == BF else 1e-5)
+        assert torch.equal(k, k0) and torch.equal(v, v0)
+    wide = torch.zeros((3, 2 * G * d), dtype=dtype, device=DEV)
+    wide[:, :G * d], wide[:, G * d:] = args[1], args[2]
+    got = ops.window_attention_step(args[0], wide[:, :G * d], wide[:, G * d:], k0, v0, n, H, G, window, sinks)
+    assert torch.equal(got, want)
+
+
+def test_step_offsets_beyond_32_bits():
+    """A cache of more than 2^32 elements: the last sequence's rows lie behind the 32-bit range."""
+    R, cap, G, d = 3, 1 << 21, 12, 128     # 3 x 3.2 G elements of bf16, keys only once
+    free, _ = torch.cuda.mem_get_info()
+    if free < 48 << 30:
+        pytest.skip("needs 48 GiB of free memory")
+    g = torch.Generator().manual_seed(9)
+    cache = torch.zeros((R, cap, G * d), dtype=BF, device=DEV)
+    v_small = torch.zeros((R, cap, 1), dtype=BF, device=DEV)
+    del v_small
+    n = torch.tensor([cap, 1, cap - 5], dtype=torch.int32, device=DEV)
+    rowk = rnd((300, G * d), BF, g).to(DEV)
+    cache[2, cap - 5 - 300:cap - 5] = rowk
+    cache[0, cap - 300:] = rowk
+    q = rnd((1, G * d), BF, g).to(DEV).expand(R, -1).contiguous()
+    o = ops.window_attention_step(q, None, None, cache, cache, n, G, G, 300, 0)
+    small = torch.zeros((1, 300, G * d), dtype=BF, device=DEV)
+    small[0] = rowk
+    want = ops.window_attention_step(q[:1], None, None, small, small, torch.tensor([300], dtype=torch.int32, device=DEV), G, G, 300, 0)
+    torch.testing.assert_close(o[2:].float(), want.float(), rtol=2.0 ** -6, atol=2.0 ** -6)
+    torch.testing.assert_close(o[:1].float(), want.float(), rtol=2.0 ** -6, atol=2.0 ** -6)
+
+
+# ------------------------------------------------------------------------------ used together
+def block(x, pos, w, f, H, G, d, gq, gk, **kw):
+    """norm + rotation + windowed attention of the fused projection rows x (T, (H + 2 G) d)."""
+    q, k, v = x[:, :H * d], x[:, H * d:(H + G) * d], x[:, (H + G) * d:]
+    q, k = ops.qk_norm_rotary(q, k, gq, gk, pos, f, H, G)
+    return q, k, v, ops.window_attention(q, k, v, n_head=H, n_kv_head=G, window=w, **kw)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_training_and_generation_agree(dtype):
+    """A text attended as a whole, and the same text token by token over a ring cache of sinks + window slots."""
+    g = torch.Generator().manual_seed(12)
+    n, H, G, d, window, sinks = 180, 4, 2, 64, 48, 4
+    f = ops.RotaryFrequencies(64, device=DEV, scaling="yarn", factor=4.0, trained_len=64)
+    x = rnd((n, (H + 2 * G) * d), dtype, g).to(DEV)
+    gq, gk = (1 + 0.1 * torch.randn(d, generator=g)).to(DEV), (1 + 0.1 * torch.randn(d, generator=g)).to(DEV)
+    pos = torch.arange(n, device=DEV)
+    _, _, v, whole = block(x, pos, window, f, H, G, d, gq, gk, B=1, Lq=n, Lk=n, sinks=sinks)
+    cap = window + sinks
+    kc = torch.full((1, cap, G * d), float("nan"), dtype=dtype, device=DEV)
+    vc = kc.clone()
+    for t in range(n):
+        q1, k1 = ops.qk_norm_rotary(x[t:t + 1, :H * d], x[t:t + 1, H * d:(H + G) * d], gq, gk, pos[t:t + 1], f, H, G)
+        o = ops.window_attention_step(q1, k1, v[t:t + 1].contiguous(), kc, vc, torch.tensor([t + 1], dtype=torch.int32, device=DEV), H, G,
+                                      window, sinks)
+        # same inputs bit for bit; both within the bounds of test_window_attention of one exact value
+        torch.testing.assert_close(o[0].float(), whole[t].float(), rtol=3 * unit(dtype) + 1e-5, atol=4 * unit(dtype) * 3 + 1e-5)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_block_gradients(dtype):
+    """Gradients through norm, rotation and attention against the tape in 64 bits."""
+    g = torch.Generator().manual_seed(13)
+    n, H, G, d, window, sinks = 140, 4, 2, 64, 30, 3
+    f = ops.RotaryFrequencies(32, device=DEV)
+    x, do = rnd((n, (H + 2 * G) * d), dtype, g), rnd((n, H * d), dtype, g)
+    gq, gk = 1 + 0.1 * torch.randn(d, generator=g), 1 + 0.1 * torch.randn(d, generator=g)
+    pos = torch.arange(n) + 1000
+    leaves = [t.to(DEV).requires_grad_() for t in (x, gq, gk)]
+    *_, o = block(leaves[0], pos.to(DEV), window, f, H, G, d, leaves[1], leaves[2], B=1, Lq=n, Lk=n, sinks=sinks)
+    got = (o,) + torch.autograd.grad(o, leaves, do.to(DEV))
+    x64, q64, k64 = (t.double().requires_grad_() for t in (x, gq, gk))
+    y = x64.view(n, -1, d)
+    q, _ = norm64(y[:, :H], q64, 1e-6, pos, f, 32, False)
+    k, _ = norm64(y[:, H:H + G], k64, 1e-6, pos, f, 32, False)
+    v = y[:, H + G:]
+    s = torch.einsum("ihd,jhd->hij", q, k.repeat_interleave(H // G, 1)) * d ** -0.5
+    p = torch.softmax(s.masked_fill(~visible(n, n, window, sinks, True), -math.inf), -1)
+    want = torch.einsum("hij,jhd->ihd", p, v.repeat_interleave(H // G, 1)).reshape(n, -1)
+    ref = (want.detach(),) + torch.autograd.grad(want, (x64, q64, k64), do.double())
+    for a, b, name in zip(got, ref, ("o", "dx", "dgamma_q", "dgamma_k")):
+        # bf16: six roundings (q, k, P, o, dS, dq or dk) of 2^-8 on sums whose terms cancel to about a quarter of their size
+        tol = (6 * 4 * unit(BF) if dtype == BF else 2e-5) * b.abs().max().item()
+        assert (a.double().cpu() - b).abs().max().item() <= tol, name
+
+
+# ------------------------------------------------------------------------------ streams, graphs
+def test_other_stream_and_captured_graph():
+    """Forward, backward and a step captured once and replayed on new inputs, between eager calls on another stream."""
+    g = torch.Generator().manual_seed(14)
+    n, H, G, d, window, sinks, cap = 300, 4, 2, 64, 50, 4, 5000
+    f = ops.RotaryFrequencies(64, device=DEV)
+    pos = torch.arange(n, device=DEV)
+    x = rnd((n, (H + 2 * G) * d), BF, g).to(DEV)
+    do = rnd((n, H * d), BF, g).to(DEV)
+    gq, gk = torch.ones(d, device=DEV), torch.ones(d, device=DEV)
+    kc, vc = rnd((1, cap, G * d), BF, g).to(DEV), rnd((1, cap, G * d), BF, g).to(DEV)
+    length = torch.tensor([4500], dtype=torch.int32, device=DEV)
+
+    def work():
+        leaf = x.detach().requires_grad_()
+        a, b = gq.detach().requires_grad_(), gk.detach().requires_grad_()
+        q, k, v, o = block(leaf, pos, window, f, H, G, d, a, b, B=1, Lq=n, Lk=n, sinks=sinks)
+        grads = torch.autograd.grad(o, (leaf, a, b), do)
+        with torch.no_grad():
+            one = ops.window_attention_step(q[:1], k[:1], v[:1].contiguous(), kc, vc, length, H, G, 4096, sinks)
+        return (o.detach(), one) + grads
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        warm = work()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(warm, work()))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work()
+    for seed in range(3):
+        gen = torch.Generator().manual_seed(100 + seed)
+        x.copy_(rnd(x.shape, BF, gen))
+        length.fill_(4500 + 7 * seed)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        want = work()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), seed
