@@ -21,6 +21,7 @@ namespace {
 
 constexpr int NT = 64;     // rows per LDS tile
 constexpr int MAXD = 128;
+constexpr int MFMA_ROWS = 128;   // key rows of a block of the bf16 path
 
 template <int D> struct Tile { float a[NT][D + 4]; };
 
@@ -409,8 +410,11 @@ extern "C" int64_t skhip_window_attn_bwd_ws_floats(int B, int n_head, int n_kv, 
   WinParams p = {};
   p.B = B; p.H = n_head; p.G = n_kv; p.Lq = Lq; p.Lk = Lk; p.d = d; p.sinks = sinks;
   set_window(p, window, causal);
+  // the larger of the two paths' needs: which one a call takes depends on its pointers and strides
   plan_sinks(p, NT);
-  return (int64_t)n_head * Tq + slab_floats(p, NT);
+  const int64_t plain = ((int64_t)n_head * Tq + 3) / 4 * 4 + slab_floats(p, NT);
+  plan_sinks(p, MFMA_ROWS);
+  return std::max(plain, (2 * (int64_t)n_head * Tq + 3) / 4 * 4 + slab_floats(p, MFMA_ROWS));
 }
 
 extern "C" int skhip_window_attn_fwd(const void* Q, const void* K, const void* V, void* O, float* LSE, const uint8_t* key_pad,
@@ -428,6 +432,7 @@ extern "C" int skhip_window_attn_fwd(const void* Q, const void* K, const void* V
   if (Tq == 0) return SK_OK;
   SK_CHECK_ARG(Q && O && LSE && (Tk == 0 || (K && V)), "%s: null pointer", who);
   set_window(p, window, causal);
+  if (sk_window_mfma_supported(p, dtype)) return sk_window_fwd_mfma(p, stream);
   if (dtype == SK_BF16) {
     if (d <= 64) launch_fwd<bf16_t, 64>(p, stream); else launch_fwd<bf16_t, 128>(p, stream);
   } else {
@@ -459,14 +464,20 @@ extern "C" int skhip_window_attn_bwd(const void* Q, const void* K, const void* V
   if (Tq == 0 && Tk == 0) return SK_OK;
   SK_CHECK_ARG((Tq == 0 || (Q && O && dO && LSE && dQ)) && (Tk == 0 || (K && V && dK && dV)), "%s: null pointer", who);
   set_window(p, window, causal);
-  plan_sinks(p, NT);
-  const int64_t need = (int64_t)n_head * Tq + slab_floats(p, NT);
+  plan_sinks(p, MFMA_ROWS);
+  const bool mfma = sk_window_mfma_supported(p, dtype);
+  if (!mfma) plan_sinks(p, NT);
+  const int64_t head = (mfma ? 2 : 1) * (int64_t)n_head * Tq, need = (head + 3) / 4 * 4 + slab_floats(p, mfma ? MFMA_ROWS : NT);
   if (need > 0 && (!workspace || workspace_floats < need)) {
     sk_set_error("%s: workspace of %lld floats needed", who, (long long)need);
     return SK_ERR_WORKSPACE;
   }
   p.delta = workspace;
-  p.slabs = workspace + (int64_t)n_head * Tq;
+  p.slabs = workspace + (head + 3) / 4 * 4;   // (16-byte stores)
+  if (mfma) {
+    rc = sk_window_bwd_mfma(p, stream);
+    return rc ? rc : sk_window_join(p, MFMA_ROWS, dtype, stream);
+  }
   if (dtype == SK_BF16) {
     if (d <= 64) launch_bwd<bf16_t, 64>(p, stream); else launch_bwd<bf16_t, 128>(p, stream);
   } else {

@@ -179,7 +179,7 @@ def test_entry_points_refuse_before_any_launch():
 
 def test_workspace_sizes():
     lib = L.load()
-    base = 4 * 12
+    base = 2 * 4 * 12
     # no sinks, or a window that reaches the first key from everywhere: the rows' deltas alone
     assert lib.skhip_window_attn_bwd_ws_floats(2, 4, 2, 12, 6, 6, 16, 3, 0, 1) == base
     assert lib.skhip_window_attn_bwd_ws_floats(2, 4, 2, 12, 6, 6, 16, 100, 2, 1) == base

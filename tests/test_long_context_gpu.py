@@ -375,16 +375,17 @@ def test_window_strides_and_alignment(dtype):
         return (o,) + torch.autograd.grad(o, leaves, do)
 
     want = run(q, k, v, do)
-    for shift in (0, 8, 1):
+    for shift, extra in ((0, 9), (8, 9), (1, 9), (0, 16), (8, 16)):
         wide = torch.zeros((n, (H + 2 * G) * d + 16), dtype=dtype, device=DEV)
         cut = wide[:, shift:shift + (H + 2 * G) * d]
         cut[:, :H * d], cut[:, H * d:(H + G) * d], cut[:, (H + G) * d:] = q, k, v
-        dw = torch.zeros((n, H * d + 9), dtype=dtype, device=DEV)
+        dw = torch.zeros((n, H * d + extra), dtype=dtype, device=DEV)
         dw[:, shift:shift + H * d] = do
         got = run(cut[:, :H * d], cut[:, H * d:(H + G) * d], cut[:, (H + G) * d:], dw[:, shift:shift + H * d])
         for a, b, name in zip(got, want, ("o", "dq", "dk", "dv")):
-            if shift % 8 == 0 or dtype == F32:
-                assert torch.equal(a, b), (shift, name)
+            # (rows of 16-byte pieces throughout: the same kernel)
+            if dtype == F32 or (shift % 8 == 0 and (extra % 8 == 0 or name == "o")):
+                assert torch.equal(a, b), (shift, extra, name)
             else:   # another kernel: same definition, both within the bounds that run_window checks
                 torch.testing.assert_close(a.float(), b.float(), rtol=0.05, atol=0.05)
     for a, b in zip(run(q.t().contiguous().t(), k, v, do.t().contiguous().t()), want):
