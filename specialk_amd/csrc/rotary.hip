@@ -15,32 +15,39 @@
 //
 // Bound by HBM: each element is read and written once (backward of the norm reads x and dy).  A lane owns 8 pairs, or 16
 // of the elements that pass, of one head: two 16-byte loads and stores in bf16, no exchange between lanes but the
-// norm's sum over the lanes of a head.
+// norm's sum over the lanes of a head.  Many waves with one item each in flight carry more than few with several: against
+// four items a thread (two backward) at 150 - 176 registers, one item at 60 - 128 takes norm and turn of 65536 rows of 40
+// heads of 128 in bf16 from 280 to 250 us (5.4 TB/s), their backward from 451 to 430 us (4.7 TB/s, three passes over the
+// rows), and the turn alone of 16381 rows of 20 fp32 heads of 128 from 90 to 75 us (4.5 TB/s); a copy reaches 4.9 TB/s.
 #include "common.h"
 #include <algorithm>
 
 namespace {
 
 constexpr int MAX_D = 256;        // at most 16 + 1 owning lanes per head
-constexpr int MAX_TB = 64;        // tokens per group
-constexpr int ANGLES = 2048;      // (cos, sin) pairs per group
-constexpr int UNROLL = 4;         // items a thread has in flight
-constexpr int BWD_BLOCKS = 1024;  // partial dgamma rows of the backward pass
+constexpr int ANGLES = 2048;      // (cos, sin) pairs per group of tokens
+constexpr int BWD_BLOCKS = 1024;  // partial dgamma rows of the backward pass, queries and keys together
 
+// Queries and keys are two sides of a launch, each with blocks of its own: a block then has one set of pointers, one norm
+// weight and one gradient sum.
+struct Side {
+  const void *x, *dy;       // input (backward: the saved one), output gradient
+  void* out;                // forward: output; backward: input gradient
+  int64_t ldx, lddy, ldo;
+  const float* gamma;       // [d]
+  float* partial;           // [blocks][d]
+  int64_t groups;           // of tb tokens
+  int heads, tb, width, blocks;   // width: items (lanes of heads) per token
+  uint32_t magic;                 // ceil(2^32 / width)
+};
 struct RotParams {
-  const void *q, *k;        // forward: inputs; norm backward: the saved inputs
-  const void *dq, *dk;      // norm backward: output gradients
-  void *oq, *ok;            // forward: outputs; backward: input gradients
-  int64_t ldq, ldk, lddq, lddk, ldoq, ldok;
+  Side side[2];
   const int64_t* pos;
   const uint64_t* turns;    // [rot / 2]
-  const float *gq, *gk;     // [d]
-  float* partial;           // [blocks][2][d]
-  int64_t T, groups;
-  int H, G, d, rot, lph, tb, width;   // lanes per head (power of two), tokens per group, items per token
-  uint32_t magic;                     // ceil(2^32 / width)
+  int64_t T;
+  int d, rot, lph;          // lanes per head (power of two)
   float amp, eps;
-  int sign;                           // -1: angles negated
+  int sign;                 // -1: angles negated
 };
 
 // cos and sin of 2 pi * phase / 2^64
@@ -183,16 +190,14 @@ __device__ __forceinline__ void turn(float (&v)[16], const float2* cs, int valid
   }
 }
 
-struct Item { int t, hl, l, head; bool isq, on; };
-__device__ __forceinline__ Item item_of(const RotParams& p, int e, int n, int lanes, int lshift) {
+// item e of a group: token and head (rows and heads are addressed from the group's first token)
+struct Item { int t, head; bool on; };
+__device__ __forceinline__ Item item_of(const RotParams& p, const Side& s, int e, int n, int lanes, int lshift) {
   Item it;
-  it.t = (int)__umulhi((uint32_t)e, p.magic);
-  if (p.width == 1) it.t = e;
-  it.hl = e - it.t * p.width;
-  it.l = it.hl & (p.lph - 1);
-  it.head = it.hl >> lshift;
-  it.isq = it.head < p.H;
-  it.on = e < n && it.l < lanes;
+  it.t = s.width == 1 ? e : (int)__umulhi((uint32_t)e, s.magic);
+  const int hl = e - it.t * s.width;
+  it.head = hl >> lshift;
+  it.on = e < n && (hl & (p.lph - 1)) < lanes;
   return it;
 }
 
@@ -200,59 +205,46 @@ template <typename T, bool NORM, bool IL, bool VEC>
 __global__ __launch_bounds__(256) void qk_rotary_kernel(RotParams p) {
   typedef Own<T, IL, VEC> O;
   __shared__ float2 cs[ANGLES];
+  const bool keys = (int)blockIdx.x >= p.side[0].blocks;
+  const Side s = p.side[keys];
+  const int blk = (int)blockIdx.x - (keys ? p.side[0].blocks : 0);
   const int np = p.rot >> 1, nrl = (np + 7) >> 3, lanes = nrl + ((p.d - p.rot + 15) >> 4);
   const int lshift = __ffs(p.lph) - 1;
   const int l = threadIdx.x & (p.lph - 1);     // the same for every item of the thread: width and 256 are multiples of lph
   const bool rotates = l < nrl;
   const int valid = max(0, min(8, np - 8 * l));
-  float gq[16], gk[16];
-  if (NORM) {
-    const int ll = min(l, lanes - 1);
-    O::load_row(gq, p.gq, p, ll, ll < nrl);
-    O::load_row(gk, p.gk ? p.gk : p.gq, p, ll, ll < nrl);
-  }
+  float gm[16];
+  if (NORM) O::load_row(gm, s.gamma, p, min(l, lanes - 1), min(l, lanes - 1) < nrl);
   const float inv_d = 1.f / (float)p.d;
-  for (int64_t grp = blockIdx.x; grp < p.groups; grp += gridDim.x) {
-    const int64_t t0 = grp * p.tb;
-    const int nt = (int)min((int64_t)p.tb, p.T - t0), n = nt * p.width;
-    bool have = false;
-    for (int e0 = 0; e0 < n; e0 += 256 * UNROLL) {
-      typename O::Raw raw[UNROLL];
-#pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        const Item it = item_of(p, e0 + u * 256 + threadIdx.x, n, lanes, lshift);
-        const T* base = it.isq ? (const T*)p.q + (t0 + it.t) * p.ldq + (int64_t)it.head * p.d
-                               : (const T*)p.k + (t0 + it.t) * p.ldk + (int64_t)(it.head - p.H) * p.d;
-        O::load(raw[u], base, p, it.l, it.on);
-      }
-      if (!have) {   // the loads above are in flight meanwhile
+  for (int64_t grp = blk; grp < s.groups; grp += s.blocks) {
+    const int64_t t0 = grp * s.tb;
+    const int nt = (int)min((int64_t)s.tb, p.T - t0), n = nt * s.width;
+    const T* x = (const T*)s.x + t0 * s.ldx;
+    T* out = (T*)s.out + t0 * s.ldo;
+    for (int e0 = 0; e0 < n; e0 += 256) {
+      const Item it = item_of(p, s, e0 + threadIdx.x, n, lanes, lshift);
+      typename O::Raw raw;
+      O::load(raw, x + it.t * s.ldx + it.head * p.d, p, l, it.on);
+      if (e0 == 0) {   // the first load is in flight meanwhile
         __syncthreads();
         group_angles(cs, p, t0, nt);
         __syncthreads();
-        have = true;
       }
-#pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        if (e0 + u * 256 >= n) break;   // block-uniform
-        const Item it = item_of(p, e0 + u * 256 + threadIdx.x, n, lanes, lshift);
-        float v[16];
-        O::unpack(v, raw[u], rotates);
-        if (NORM) {
-          float ss = 0.f;
-          if (it.on) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) ss += v[j] * (v[j] * inv_d);   // (the mean, not the sum, has to stay in range)
-          }
-          const float rstd = 1.f / sqrtf(head_sum(ss, p.lph) + p.eps);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = v[j] * rstd * (it.isq ? gq[j] : gk[j]);
-        }
+      float v[16];
+      O::unpack(v, raw, rotates);
+      if (NORM) {
+        float ss = 0.f;
         if (it.on) {
-          if (rotates) turn<1>(v, cs + it.t * np + 8 * l, VEC ? 8 : valid);
-          T* out = it.isq ? (T*)p.oq + (t0 + it.t) * p.ldoq + (int64_t)it.head * p.d
-                          : (T*)p.ok + (t0 + it.t) * p.ldok + (int64_t)(it.head - p.H) * p.d;
-          O::store(out, v, p, l, rotates);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) ss += v[j] * (v[j] * inv_d);   // (the mean, not the sum, has to stay in range)
         }
+        const float rstd = 1.f / sqrtf(head_sum(ss, p.lph) + p.eps);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = v[j] * rstd * gm[j];
+      }
+      if (it.on) {
+        if (rotates) turn<1>(v, cs + it.t * np + 8 * l, VEC ? 8 : valid);
+        O::store(out + it.t * s.ldo + it.head * p.d, v, p, l, rotates);
       }
     }
   }
@@ -262,160 +254,155 @@ __global__ __launch_bounds__(256) void qk_rotary_kernel(RotParams p) {
 // lanes with the same elements, the waves and (second kernel) the blocks are added in a fixed order: no atomics, results
 // do not change from run to run.
 template <typename T, bool IL, bool VEC>
-__global__ __launch_bounds__(256) void qk_norm_rotary_bwd_kernel(RotParams p) {
+__global__ __launch_bounds__(256, 4) void qk_norm_rotary_bwd_kernel(RotParams p) {
   typedef Own<T, IL, VEC> O;
   __shared__ float2 cs[ANGLES];
-  __shared__ float red[4][2][MAX_D];
+  __shared__ float red[4][MAX_D];
+  const bool keys = (int)blockIdx.x >= p.side[0].blocks;
+  const Side s = p.side[keys];
+  const int blk = (int)blockIdx.x - (keys ? p.side[0].blocks : 0);
   const int np = p.rot >> 1, nrl = (np + 7) >> 3, lanes = nrl + ((p.d - p.rot + 15) >> 4);
   const int lshift = __ffs(p.lph) - 1;
   const int l = threadIdx.x & (p.lph - 1);
   const bool rotates = l < nrl;
   const int valid = max(0, min(8, np - 8 * l));
-  float gq[16], gk[16], aq[16], ak[16];
-  {
-    const int ll = min(l, lanes - 1);
-    O::load_row(gq, p.gq, p, ll, ll < nrl);
-    O::load_row(gk, p.gk ? p.gk : p.gq, p, ll, ll < nrl);
-  }
+  float gm[16], acc[16];
+  O::load_row(gm, s.gamma, p, min(l, lanes - 1), min(l, lanes - 1) < nrl);
 #pragma unroll
-  for (int j = 0; j < 16; ++j) aq[j] = ak[j] = 0.f;
+  for (int j = 0; j < 16; ++j) acc[j] = 0.f;
   const float inv_d = 1.f / (float)p.d;
-  constexpr int U = 2;
-  for (int64_t grp = blockIdx.x; grp < p.groups; grp += gridDim.x) {
-    const int64_t t0 = grp * p.tb;
-    const int nt = (int)min((int64_t)p.tb, p.T - t0), n = nt * p.width;
-    bool have = false;
-    for (int e0 = 0; e0 < n; e0 += 256 * U) {
-      typename O::Raw rx[U], rd[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const Item it = item_of(p, e0 + u * 256 + threadIdx.x, n, lanes, lshift);
-        const int64_t t = t0 + it.t, hq = (int64_t)it.head * p.d, hk = (int64_t)(it.head - p.H) * p.d;
-        O::load(rx[u], it.isq ? (const T*)p.q + t * p.ldq + hq : (const T*)p.k + t * p.ldk + hk, p, it.l, it.on);
-        O::load(rd[u], it.isq ? (const T*)p.dq + t * p.lddq + hq : (const T*)p.dk + t * p.lddk + hk, p, it.l, it.on);
-      }
-      if (!have) {
+  for (int64_t grp = blk; grp < s.groups; grp += s.blocks) {
+    const int64_t t0 = grp * s.tb;
+    const int nt = (int)min((int64_t)s.tb, p.T - t0), n = nt * s.width;
+    const T* x = (const T*)s.x + t0 * s.ldx;
+    const T* dy = (const T*)s.dy + t0 * s.lddy;
+    T* out = (T*)s.out + t0 * s.ldo;
+    for (int e0 = 0; e0 < n; e0 += 256) {
+      const Item it = item_of(p, s, e0 + threadIdx.x, n, lanes, lshift);
+      typename O::Raw rx, rd;
+      O::load(rx, x + it.t * s.ldx + it.head * p.d, p, l, it.on);
+      O::load(rd, dy + it.t * s.lddy + it.head * p.d, p, l, it.on);
+      if (e0 == 0) {
         __syncthreads();
         group_angles(cs, p, t0, nt);
         __syncthreads();
-        have = true;
       }
+      float v[16], g[16];
+      O::unpack(v, rx, rotates);
+      O::unpack(g, rd, rotates);
+      float ss = 0.f, sg = 0.f;
+      if (it.on) {
+        if (rotates) turn<-1>(g, cs + it.t * np + 8 * l, VEC ? 8 : valid);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (e0 + u * 256 >= n) break;   // block-uniform
-        const Item it = item_of(p, e0 + u * 256 + threadIdx.x, n, lanes, lshift);
-        float x[16], g[16];
-        O::unpack(x, rx[u], rotates);
-        O::unpack(g, rd[u], rotates);
-        float ss = 0.f, sg = 0.f;
-        if (it.on) {
-          if (rotates) turn<-1>(g, cs + it.t * np + 8 * l, VEC ? 8 : valid);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            ss += x[j] * (x[j] * inv_d);
-            sg += g[j] * (it.isq ? gq[j] : gk[j]) * x[j];
-          }
+        for (int j = 0; j < 16; ++j) {
+          ss += v[j] * (v[j] * inv_d);
+          sg += g[j] * gm[j] * v[j];
         }
-        const float rstd = 1.f / sqrtf(head_sum(ss, p.lph) + p.eps);
-        const float mean = head_sum(sg, p.lph) * rstd * inv_d;   // mean(g gamma xhat)
-        if (it.on) {
+      }
+      const float rstd = 1.f / sqrtf(head_sum(ss, p.lph) + p.eps);
+      const float mean = head_sum(sg, p.lph) * rstd * inv_d;   // mean(g gamma xhat)
+      if (it.on) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float xhat = x[j] * rstd, c = g[j] * xhat;
-            if (it.isq) aq[j] += c; else ak[j] += c;
-            g[j] = rstd * (g[j] * (it.isq ? gq[j] : gk[j]) - xhat * mean);
-          }
-          const int64_t t = t0 + it.t;
-          T* out = it.isq ? (T*)p.oq + t * p.ldoq + (int64_t)it.head * p.d : (T*)p.ok + t * p.ldok + (int64_t)(it.head - p.H) * p.d;
-          O::store(out, g, p, l, rotates);
+        for (int j = 0; j < 16; ++j) {
+          const float xhat = v[j] * rstd;
+          acc[j] += g[j] * xhat;
+          g[j] = rstd * (g[j] * gm[j] - xhat * mean);
         }
+        O::store(out + it.t * s.ldo + it.head * p.d, g, p, l, rotates);
       }
     }
   }
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
 #pragma unroll
   for (int j = 0; j < 16; ++j)
-    for (int o = 32; o >= p.lph; o >>= 1) {
-      aq[j] += __shfl_xor(aq[j], o, 64);
-      ak[j] += __shfl_xor(ak[j], o, 64);
-    }
+    for (int o = 32; o >= p.lph; o >>= 1) acc[j] += __shfl_xor(acc[j], o, 64);
   if (lane < p.lph && l < lanes) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
+    for (int j = 0; j < 16; ++j) {   // (sums are in pair order whatever the storage order)
       const int i = Own<T, IL, false>::index(p, l, j);
-      if (i >= 0) {
-        // passing elements keep their order; those of pairs are in pair order either way
-        red[wave][0][i] = aq[j];
-        red[wave][1][i] = ak[j];
-      }
+      if (i >= 0) red[wave][i] = acc[j];
     }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < 2 * p.d; e += 256) {
-    const int w = e >= p.d, i = e - w * p.d;
-    p.partial[(int64_t)blockIdx.x * 2 * p.d + e] = red[0][w][i] + red[1][w][i] + red[2][w][i] + red[3][w][i];
-  }
+  for (int i = threadIdx.x; i < p.d; i += 256)
+    s.partial[(int64_t)blk * p.d + i] = red[0][i] + red[1][i] + red[2][i] + red[3][i];
 }
 
-// out[c] = sum over blocks of partial[block][c], c < 2 d: one wave per 64 columns and 16 runs of blocks
-__global__ __launch_bounds__(1024) void dgamma_sum_kernel(const float* __restrict__ partial, float* __restrict__ dgq,
-                                                          float* __restrict__ dgk, int blocks, int d) {
-  __shared__ float red[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = blockIdx.x * 64 + lane;
+// dgamma[c] = sum over blocks of partial[block][c]: a block adds 16 columns, 64 runs of partial rows side by side
+__global__ __launch_bounds__(1024) void dgamma_sum_kernel(const float* __restrict__ part_q, const float* __restrict__ part_k,
+                                                          float* __restrict__ dgq, float* __restrict__ dgk, int blocks_q,
+                                                          int blocks_k, int d) {
+  __shared__ float red[64][17];
+  const float* part = blockIdx.y ? part_k : part_q;
+  const int blocks = blockIdx.y ? blocks_k : blocks_q;
+  const int c = threadIdx.x & 15, run = threadIdx.x >> 4, col = blockIdx.x * 16 + c;
   float a = 0.f;
-  if (c < 2 * d)
-    for (int b = wave; b < blocks; b += 16) a += partial[(int64_t)b * 2 * d + c];
-  red[wave][lane] = a;
+  if (col < d) {
+#pragma unroll 8
+    for (int b = run; b < blocks; b += 64) a += part[(int64_t)b * d + col];
+  }
+  red[run][c] = a;
   __syncthreads();
-  if (wave == 0 && c < 2 * d) {
-    float s = 0.f;
+  if (run < 8) {
+    float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < 16; ++w) s += red[w][lane];
-    if (c < d) dgq[c] = s;
-    else if (dgk) dgk[c - d] = s;
+    for (int i = 0; i < 8; ++i) v += red[8 * run + i][c];
+    red[8 * run][c] = v;
+  }
+  __syncthreads();
+  if (run == 0 && col < d) {
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v += red[8 * i][c];
+    (blockIdx.y ? dgk : dgq)[col] = v;
   }
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-// Lanes per head and tokens per group.
-void plan(RotParams& p) {
+// Lanes per head, tokens per group and blocks of each side; `most`: blocks of both sides.
+void plan(RotParams& p, int n_head, int n_kv, int rounds, int64_t most) {
   const int np = p.rot / 2, lanes = (np + 7) / 8 + (p.d - p.rot + 15) / 16;
-  int lph = 1;
-  while (lph < lanes) lph *= 2;
-  p.lph = lph;
-  p.width = (p.H + p.G) * lph;
-  // A group is what a block has between two barriers: four items per thread, fewer where the rows would not give every
-  // CU two blocks (640 rows of 16 heads: 160 blocks of 4 rows instead of 40 of 16).
-  int64_t tb = std::max<int64_t>(1, (256 * UNROLL) / p.width);
-  tb = std::min<int64_t>(tb, std::max<int64_t>(std::max(1, 256 / p.width), p.T / (2 * sk_num_cus())));
-  if (np) tb = std::min<int64_t>(tb, ANGLES / np);
-  p.tb = (int)std::min<int64_t>(tb, MAX_TB);
-  p.groups = (p.T + p.tb - 1) / p.tb;
-  p.magic = (uint32_t)((0x100000000ull + p.width - 1) / p.width);
+  p.lph = 1;
+  while (p.lph < lanes) p.lph *= 2;
+  for (int i = 0; i < 2; ++i) {
+    Side& s = p.side[i];
+    s.heads = i ? n_kv : n_head;
+    s.width = std::max(1, s.heads * p.lph);
+    // A group is what a block has between two barriers: `rounds` items of each thread, fewer where the rows would not
+    // give every CU two blocks (640 rows of 8 heads: 80 blocks of 8 rows a side instead of 10 of 64).
+    int64_t tb = std::max<int64_t>(1, 256 * rounds / s.width);
+    tb = std::min<int64_t>(tb, std::max<int64_t>(std::max(1, 256 / s.width), p.T / (2 * sk_num_cus())));
+    if (np) tb = std::min<int64_t>(tb, ANGLES / np);
+    s.tb = (int)tb;
+    s.groups = s.heads ? (p.T + tb - 1) / tb : 0;
+    s.magic = (uint32_t)((0x100000000ull + s.width - 1) / s.width);
+    const int64_t share = std::max<int64_t>(1, most * s.heads / (n_head + n_kv));
+    s.blocks = (int)std::min<int64_t>(s.groups, share);
+  }
 }
 
 template <typename T, bool NORM>
 void launch_fwd(const RotParams& p, bool il, bool vec, hipStream_t stream) {
-  const unsigned blocks = (unsigned)std::min<int64_t>(p.groups, (int64_t)sk_num_cus() * 16);
+  const dim3 grid((unsigned)(p.side[0].blocks + p.side[1].blocks));
   if (il) {
-    if (vec) hipLaunchKernelGGL((qk_rotary_kernel<T, NORM, true, true>), dim3(blocks), dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((qk_rotary_kernel<T, NORM, true, false>), dim3(blocks), dim3(256), 0, stream, p);
+    if (vec) hipLaunchKernelGGL((qk_rotary_kernel<T, NORM, true, true>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((qk_rotary_kernel<T, NORM, true, false>), grid, dim3(256), 0, stream, p);
   } else {
-    if (vec) hipLaunchKernelGGL((qk_rotary_kernel<T, NORM, false, true>), dim3(blocks), dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((qk_rotary_kernel<T, NORM, false, false>), dim3(blocks), dim3(256), 0, stream, p);
+    if (vec) hipLaunchKernelGGL((qk_rotary_kernel<T, NORM, false, true>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((qk_rotary_kernel<T, NORM, false, false>), grid, dim3(256), 0, stream, p);
   }
 }
 
 template <typename T>
-void launch_bwd(const RotParams& p, bool il, bool vec, unsigned blocks, hipStream_t stream) {
+void launch_bwd(const RotParams& p, bool il, bool vec, hipStream_t stream) {
+  const dim3 grid((unsigned)(p.side[0].blocks + p.side[1].blocks));
   if (il) {
-    if (vec) hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, true, true>), dim3(blocks), dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, true, false>), dim3(blocks), dim3(256), 0, stream, p);
+    if (vec) hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, true, true>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, true, false>), grid, dim3(256), 0, stream, p);
   } else {
-    if (vec) hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, false, true>), dim3(blocks), dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, false, false>), dim3(blocks), dim3(256), 0, stream, p);
+    if (vec) hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, false, true>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, false, false>), grid, dim3(256), 0, stream, p);
   }
 }
 
@@ -432,7 +419,7 @@ int check_shape(const char* who, const int64_t* pos, const uint64_t* turns, int6
 
 }  // namespace
 
-extern "C" int64_t skhip_qk_norm_rotary_bwd_ws_floats(int d) { return d > 0 && d <= MAX_D ? (int64_t)BWD_BLOCKS * 2 * d : 0; }
+extern "C" int64_t skhip_qk_norm_rotary_bwd_ws_floats(int d) { return d > 0 && d <= MAX_D ? (int64_t)(BWD_BLOCKS + 1) * d : 0; }
 
 extern "C" int skhip_qk_rotary(const void* q, const void* k, void* q_out, void* k_out, const int64_t* pos,
                                const uint64_t* turns, float amplitude, const float* gamma_q, const float* gamma_k, float eps,
@@ -449,14 +436,14 @@ extern "C" int skhip_qk_rotary(const void* q, const void* k, void* q_out, void* 
   SK_CHECK_ARG(ldq >= (int64_t)n_head * d && ldq_out >= (int64_t)n_head * d && (n_kv == 0 ||
                (ldk >= (int64_t)n_kv * d && ldk_out >= (int64_t)n_kv * d)), "%s: row stride below the row's length", who);
   RotParams p = {};
-  p.q = q; p.k = k; p.oq = q_out; p.ok = k_out; p.pos = pos; p.turns = turns; p.amp = amplitude;
-  p.gq = gamma_q; p.gk = gamma_k; p.eps = eps; p.T = T; p.H = n_head; p.G = n_kv; p.d = d; p.rot = rot;
-  p.ldq = ldq; p.ldk = ldk; p.ldoq = ldq_out; p.ldok = ldk_out; p.sign = inverse ? -1 : 1;
+  p.pos = pos; p.turns = turns; p.amp = amplitude; p.eps = eps; p.T = T; p.d = d; p.rot = rot; p.sign = inverse ? -1 : 1;
+  p.side[0].x = q; p.side[0].out = q_out; p.side[0].ldx = ldq; p.side[0].ldo = ldq_out; p.side[0].gamma = gamma_q;
+  p.side[1].x = k; p.side[1].out = k_out; p.side[1].ldx = ldk; p.side[1].ldo = ldk_out; p.side[1].gamma = gamma_k;
   const int64_t per = dtype == SK_BF16 ? 8 : 4;
   bool vec = aligned16(q) && aligned16(q_out) && (ldq | ldq_out) % per == 0;
   if (n_kv) vec = vec && aligned16(k) && aligned16(k_out) && (ldk | ldk_out) % per == 0;
   vec = vec && rot % 16 == 0 && d % 16 == 0;
-  plan(p);
+  plan(p, n_head, n_kv, gamma_q ? 2 : 1, (int64_t)sk_num_cus() * 64);
   if (dtype == SK_BF16) {
     if (gamma_q) launch_fwd<bf16_t, true>(p, interleaved, vec, stream);
     else launch_fwd<bf16_t, false>(p, interleaved, vec, stream);
@@ -484,27 +471,29 @@ extern "C" int skhip_qk_norm_rotary_bwd(const void* q, const void* k, const void
   SK_CHECK_ARG(T == 0 || (ldq >= nq && lddq_out >= nq && lddq >= nq && ldk >= nk && lddk_out >= nk && lddk >= nk),
                "%s: row stride below the row's length", who);
   RotParams p = {};
-  p.q = q; p.k = k; p.dq = dq_out; p.dk = dk_out; p.oq = dq; p.ok = dk; p.pos = pos; p.turns = turns; p.amp = amplitude;
-  p.gq = gamma_q; p.gk = gamma_k; p.eps = eps; p.T = T; p.H = n_head; p.G = n_kv; p.d = d; p.rot = rot;
-  p.ldq = ldq; p.ldk = ldk; p.lddq = lddq_out; p.lddk = lddk_out; p.ldoq = lddq; p.ldok = lddk; p.sign = 1;
+  p.pos = pos; p.turns = turns; p.amp = amplitude; p.eps = eps; p.T = T; p.d = d; p.rot = rot; p.sign = 1;
+  Side &sq = p.side[0], &sk = p.side[1];
+  sq.x = q; sq.dy = dq_out; sq.out = dq; sq.ldx = ldq; sq.lddy = lddq_out; sq.ldo = lddq; sq.gamma = gamma_q;
+  sk.x = k; sk.dy = dk_out; sk.out = dk; sk.ldx = ldk; sk.lddy = lddk_out; sk.ldo = lddk; sk.gamma = gamma_k;
   const int64_t per = dtype == SK_BF16 ? 8 : 4;
   bool vec = aligned16(q) && aligned16(dq_out) && aligned16(dq) && (ldq | lddq_out | lddq) % per == 0;
   if (n_kv) vec = vec && aligned16(k) && aligned16(dk_out) && aligned16(dk) && (ldk | lddk_out | lddk) % per == 0;
   vec = vec && rot % 16 == 0 && d % 16 == 0;
-  plan(p);
-  const int blocks = (int)std::min<int64_t>(p.groups, BWD_BLOCKS);
-  if (!workspace || workspace_floats < (int64_t)blocks * 2 * d) {
-    sk_set_error("%s: workspace of %lld floats needed", who, (long long)blocks * 2 * d);
+  plan(p, n_head, n_kv, 2, BWD_BLOCKS);
+  const int64_t need = (int64_t)(sq.blocks + sk.blocks) * d;
+  if (need > 0 && (!workspace || workspace_floats < need)) {
+    sk_set_error("%s: workspace of %lld floats needed", who, (long long)need);
     return SK_ERR_WORKSPACE;
   }
-  p.partial = workspace;
+  sq.partial = workspace;
+  sk.partial = workspace + (int64_t)sq.blocks * d;
   if (T > 0) {
-    if (dtype == SK_BF16) launch_bwd<bf16_t>(p, interleaved, vec, (unsigned)blocks, stream);
-    else launch_bwd<float>(p, interleaved, vec, (unsigned)blocks, stream);
+    if (dtype == SK_BF16) launch_bwd<bf16_t>(p, interleaved, vec, stream);
+    else launch_bwd<float>(p, interleaved, vec, stream);
     SK_CHECK_LAUNCH(who);
   }
-  hipLaunchKernelGGL(dgamma_sum_kernel, dim3((2 * d + 63) / 64), dim3(1024), 0, stream, workspace, dgamma_q,
-                     n_kv ? dgamma_k : nullptr, blocks, d);
+  hipLaunchKernelGGL(dgamma_sum_kernel, dim3((d + 15) / 16, n_kv ? 2 : 1), dim3(1024), 0, stream, sq.partial, sk.partial, dgamma_q,
+                     dgamma_k, sq.blocks, sk.blocks, d);
   SK_CHECK_LAUNCH(who);
   return SK_OK;
 }

@@ -262,7 +262,6 @@ __global__ __launch_bounds__(256) void window_dkv_kernel(WinParams p) {
   const int tile = extra < 0 ? (int)blockIdx.x : extra / p.nch, chunk = extra < 0 ? -1 : extra % p.nch;
   const int j0 = tile * NT, j1 = min(j0 + NT, sq.Lk);
   if (j0 >= sq.Lk) return;
-  const bool partial = tile < p.nst;
   int i_lo, i_hi;
   query_range(p, sq, j0, j1, chunk, i_lo, i_hi);
   if (chunk >= 0 && i_lo >= i_hi) return;   // (the join counts the same chunks)
@@ -307,39 +306,37 @@ __global__ __launch_bounds__(256) void window_dkv_kernel(WinParams p) {
     }
   }
   if (j >= sq.Lk) return;
-  if (partial) {
+  if (j < p.sinks && p.nst) {   // (a sink's sum has further parts)
     float* s = slab(p, b, kh, tile, 1 + chunk, NT) + (int64_t)(j - j0) * p.d;
     store_own<float, D>(s, dk, 1.f, p.d, g);
     store_own<float, D>(s + (int64_t)NT * p.d, dv, 1.f, p.d, g);
-  } else {
+  } else if (chunk < 0) {
     store_own<T, D>((T*)p.dK + (sq.kbase + j) * p.lddk + (int64_t)kh * p.d, dk, 1.f, p.d, g);
     store_own<T, D>((T*)p.dV + (sq.kbase + j) * p.lddv + (int64_t)kh * p.d, dv, 1.f, p.d, g);
   }
 }
 
-// dK, dV of the tiles that hold sinks: window part and chunks added in this order
+// dK, dV of the sinks: window part and chunks added in this order.  `rows`: key rows of a tile.
 template <typename T>
 __global__ __launch_bounds__(256) void window_join_kernel(WinParams p, int rows) {
-  const int b = blockIdx.z, kh = blockIdx.y, tile = blockIdx.x;
+  const int b = blockIdx.z, kh = blockIdx.y;
   const Seq sq = seq_of(p, b);
-  const int j0 = tile * rows, n = min(rows, sq.Lk - j0);
+  const int e = (int)blockIdx.x * 256 + threadIdx.x, j = e / p.d, c = e - j * p.d;
+  if (j >= min(p.sinks, sq.Lk)) return;
+  const int tile = j / rows, j0 = tile * rows;
   int lo, hi, parts = 1;
-  for (; parts <= p.nch; ++parts) {
-    query_range(p, sq, j0, j0 + n, parts - 1, lo, hi);
-    if (lo >= hi) break;
+  query_range(p, sq, j0, min(j0 + rows, sq.Lk), 0, lo, hi);
+  if (lo < hi) parts += (sq.Lq - lo + p.ch - 1) / p.ch;
+  const float* x = slab(p, b, kh, tile, 0, rows) + (int64_t)(j - j0) * p.d + c;
+  const int64_t step = (int64_t)2 * rows * p.d;
+  float a = 0.f, v = 0.f;
+#pragma unroll 8
+  for (int s = 0; s < parts; ++s) {
+    a += x[s * step];
+    v += x[s * step + (int64_t)rows * p.d];
   }
-  for (int e = threadIdx.x; e < n * p.d; e += 256) {
-    float a = 0.f, v = 0.f;
-    for (int s = 0; s < parts; ++s) {
-      const float* x = slab(p, b, kh, tile, s, rows) + e;
-      a += x[0];
-      v += x[(int64_t)rows * p.d];
-    }
-    const int r = e / p.d, c = e - r * p.d;
-    const int64_t at = sq.kbase + j0 + r;
-    ((T*)p.dK)[at * p.lddk + (int64_t)kh * p.d + c] = Cvt<T>::from_f32(a);
-    ((T*)p.dV)[at * p.lddv + (int64_t)kh * p.d + c] = Cvt<T>::from_f32(v);
-  }
+  ((T*)p.dK)[(sq.kbase + j) * p.lddk + (int64_t)kh * p.d + c] = Cvt<T>::from_f32(a);
+  ((T*)p.dV)[(sq.kbase + j) * p.lddv + (int64_t)kh * p.d + c] = Cvt<T>::from_f32(v);
 }
 
 int check(const char* who, const WinParams& p, int window, int dtype) {
@@ -396,8 +393,8 @@ void launch_bwd(const WinParams& p, hipStream_t stream) {
 }  // namespace
 
 int sk_window_join(const WinParams& p, int rows, int dtype, hipStream_t stream) {
-  if (!p.nst) return SK_OK;
-  dim3 grid(p.nst, p.G, p.B);
+  if (!p.nst || !p.Tk) return SK_OK;
+  dim3 grid((unsigned)(((int64_t)p.sinks * p.d + 255) / 256), p.G, p.B);
   if (dtype == SK_BF16) hipLaunchKernelGGL((window_join_kernel<bf16_t>), grid, dim3(256), 0, stream, p, rows);
   else hipLaunchKernelGGL((window_join_kernel<float>), grid, dim3(256), 0, stream, p, rows);
   SK_CHECK_LAUNCH("skhip_window_attn_bwd(join)");

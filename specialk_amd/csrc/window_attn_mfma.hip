@@ -482,16 +482,15 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(WinParams p, int ktiles) {
       }
     }
   }
-  if (tile < p.nst) {
-    if (j < sq.Lk) {
-      float* s = slab(p, b, kh, tile, 1 + chunk, OWN) + (int64_t)(j - j0) * p.d;
-      store_own_f32<D>(s, dk, p.scale, p.d, hf);
-      store_own_f32<D>(s + (int64_t)OWN * p.d, dv, 1.f, p.d, hf);
-    }
-    return;
+  const bool sink = p.nst && j < p.sinks;   // (a sink's sum has further parts)
+  if (sink && j < sq.Lk) {
+    float* s = slab(p, b, kh, tile, 1 + chunk, OWN) + (int64_t)(j - j0) * p.d;
+    store_own_f32<D>(s, dk, p.scale, p.d, hf);
+    store_own_f32<D>(s + (int64_t)OWN * p.d, dv, 1.f, p.d, hf);
   }
-  store_own<D>((bf16_t*)p.dK + (sq.kbase + jrow) * p.lddk + (int64_t)kh * p.d, dk, p.scale, p.d, hf, j < sq.Lk);
-  store_own<D>((bf16_t*)p.dV + (sq.kbase + jrow) * p.lddv + (int64_t)kh * p.d, dv, 1.f, p.d, hf, j < sq.Lk);
+  if (chunk >= 0) return;
+  store_own<D>((bf16_t*)p.dK + (sq.kbase + jrow) * p.lddk + (int64_t)kh * p.d, dk, p.scale, p.d, hf, j < sq.Lk && !sink);
+  store_own<D>((bf16_t*)p.dV + (sq.kbase + jrow) * p.lddv + (int64_t)kh * p.d, dv, 1.f, p.d, hf, j < sq.Lk && !sink);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }

@@ -1019,11 +1019,26 @@ def _heads(x, n_head, n_kv_head, most):
     return x.shape[1] // n_head
 
 
-def _same(*tensors):
-    first = tensors[0]
-    for t in tensors[1:]:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"tensors on {first.device} and {t.device}")
+def _same(first, *tensors):
+    dev = first.device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}")
+
+
+def _run(fn, *args):
+    """call(fn, *args), without the tape where no tensor among the arguments asks for it."""
+    if torch.is_grad_enabled():
+        for a in args:
+            if isinstance(a, torch.Tensor) and a.requires_grad:
+                return fn.apply(*args)
+    return fn.forward(_InferCtx(), *args)
+
+
+def _once():
+    """First thing in a backward pass whose results are not on the tape: grad mode is only on there for create_graph."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("this operator has no second derivative (create_graph=True)")
 
 
 class QKRotaryFn(torch.autograd.Function):
@@ -1037,8 +1052,8 @@ class QKRotaryFn(torch.autograd.Function):
             return L.qk_rotary(q, k, pos, *ctx.args)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
+        _once()
         (pos,) = ctx.saved_tensors
         n_head, n_kv, d = ctx.args[5:8]
         dq = _rows(dq, n_head * d, "dq")
@@ -1061,8 +1076,8 @@ class QKNormRotaryFn(torch.autograd.Function):
                                gq, gk, *ctx.rest)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
+        _once()
         q, k, gq, gk, pos = ctx.saved_tensors
         f, (_, n_head, n_kv, d, _, _) = ctx.freqs, ctx.rest
         dq = _rows(dq, n_head * d, "dq")
@@ -1101,7 +1116,7 @@ def rotary(q, k, pos, freqs, n_head, n_kv_head=None, interleaved=False):
     if freqs is None:
         raise ValueError("rotary needs a RotaryFrequencies")
     q, k, pos, n_kv = _rotary_args(q, k, pos, freqs, n_head, n_kv_head)
-    return call(QKRotaryFn, q, k, pos, freqs, n_head, n_kv, bool(interleaved))
+    return _run(QKRotaryFn, q, k, pos, freqs, n_head, n_kv, bool(interleaved))
 
 
 def qk_norm_rotary(q, k, gamma_q, gamma_k, pos, freqs, n_head, n_kv_head=None, eps=1e-6, interleaved=False):
@@ -1119,7 +1134,7 @@ def qk_norm_rotary(q, k, gamma_q, gamma_k, pos, freqs, n_head, n_kv_head=None, e
     if not eps >= 0:
         raise ValueError(f"eps {eps} is negative")
     _same(q, k, gamma_q, gamma_k)
-    return call(QKNormRotaryFn, q, k, gamma_q, gamma_k, pos, freqs, n_head, n_kv, float(eps), bool(interleaved))
+    return _run(QKNormRotaryFn, q, k, gamma_q, gamma_k, pos, freqs, n_head, n_kv, float(eps), bool(interleaved))
 
 
 # ----------------------------------------------------------------------------- attention within a window
@@ -1138,8 +1153,8 @@ class WindowAttnFn(torch.autograd.Function):
         return o
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, do):
+        _once()
         q, k, v, o, lse = ctx.saved_tensors
         with L.on_device(q):
             dq, dk, dv = L.window_attn_bwd(q, k, v, o, _rows(do, o.shape[1], "do"), lse, **ctx.cfg)
@@ -1191,7 +1206,7 @@ def window_attention(q, k, v, B, Lq, Lk, n_head, n_kv_head=None, window=None, si
     cfg = dict(B=B, Lq=Lq, Lk=Lk, n_head=n_head, n_kv=n_kv, d=d, scale=d ** -0.5 if scale is None else float(scale),
                window=_window(window), sinks=min(int(sinks), NO_WINDOW), causal=bool(causal), key_pad=key_pad, q_off=q_off,
                k_off=k_off)
-    return call(WindowAttnFn, q, k, v, cfg)
+    return _run(WindowAttnFn, q, k, v, cfg)
 
 
 def window_attention_step(q, k_new, v_new, k_cache, v_cache, kv_len, n_head, n_kv_head=None, window=None, sinks=0,
@@ -1216,7 +1231,7 @@ def window_attention_step(q, k_new, v_new, k_cache, v_cache, kv_len, n_head, n_k
         raise ValueError(f"caches must be ({R}, cap, {w}), got {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
     cap = k_cache.shape[1]
     for c in (k_cache, v_cache):
-        s0, s1, s2 = c.stride()
+        s0, s1, s2 = c.stride()   # sequence by sequence, or position by position
         if s2 != 1 or s1 < w or s0 < 0 or (R > 1 and s0 < (cap - 1) * s1 + w and (s0 < w or s1 < (R - 1) * s0 + w)):
             raise ValueError(f"cache rows overlap or are not contiguous (strides {c.stride()})")
     if k_new is not None:
@@ -1225,16 +1240,18 @@ def window_attention_step(q, k_new, v_new, k_cache, v_cache, kv_len, n_head, n_k
             k_new, v_new = k_new.contiguous(), v_new.contiguous()
         if k_new.shape[0] != R or v_new.shape[0] != R:
             raise ValueError(f"k_new and v_new must have {R} rows")
-    for t in (k_new, v_new, k_cache, v_cache):
-        if t is not None and t.dtype != q.dtype:
-            raise ValueError(f"q is {q.dtype}, a key or value {t.dtype}")
+        if k_new.dtype != q.dtype or v_new.dtype != q.dtype:
+            raise ValueError(f"q is {q.dtype}, k_new and v_new {k_new.dtype} and {v_new.dtype}")
+    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise ValueError(f"q is {q.dtype}, the caches {k_cache.dtype} and {v_cache.dtype}")
     if kv_len.dtype != torch.int32 or kv_len.shape != (R,) or not kv_len.is_contiguous():
         raise ValueError(f"kv_len must be contiguous int32 ({R},), got {kv_len.dtype} {tuple(kv_len.shape)}")
     window = cap - sinks if window is None else _window(window)
     if sinks < 0 or window < 1 or cap - sinks < window:
         raise ValueError(f"a cache of {cap} slots cannot hold {sinks} sinks and a window of {window}")
     _same(q, k_new, v_new, k_cache, v_cache, kv_len)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k_new, v_new, k_cache, v_cache)):
+    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or
+                                    (k_new is not None and (k_new.requires_grad or v_new.requires_grad))):
         raise RuntimeError("window_attention_step has no gradient: call it under torch.no_grad() or on detached tensors")
     with L.on_device(q):
         return L.window_attn_step(q, k_new, v_new, k_cache, v_cache, kv_len, n_head, n_kv, d,
