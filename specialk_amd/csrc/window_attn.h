@@ -25,6 +25,7 @@ struct WinParams {
   int64_t ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
   float scale;
   int left, right, sinks;
+  bool vec;                 // fp32 path: rows are read in pieces of 4 elements
   // Backward of the keys: queries beyond a key's window see it only if it is a sink, so the few key tiles that hold
   // sinks would sweep the whole sequence alone.  Their far queries are cut into nch chunks of ch rows, one block each;
   // window part and chunks leave fp32 partial sums in slabs, which a small kernel adds in a fixed order.
@@ -48,8 +49,22 @@ __device__ __forceinline__ Seq seq_of(const WinParams& p, int b) {
   return s;
 }
 
-__device__ __forceinline__ bool sees(const WinParams& p, int pos, int j) {
-  return j <= pos + p.right && (j >= pos - p.left || j < p.sinks);
+// bits a .. b-1 of 64 (any a, b)
+__device__ __forceinline__ uint64_t bits(int a, int b) {
+  a = min(max(a, 0), 64);
+  b = min(max(b, 0), 64);
+  const uint64_t hi = b == 64 ? ~0ull : (1ull << b) - 1, lo = a == 64 ? ~0ull : (1ull << a) - 1;
+  return hi & ~lo;
+}
+
+// Of keys j0 .. j0+63, those that a query at position pos sees; `use`: the ones that may be used at all.
+__device__ __forceinline__ uint64_t keys_seen(const WinParams& p, int pos, int j0, uint64_t use) {
+  const int end = pos + p.right + 1 - j0;
+  return (bits(pos - p.left - j0, end) | bits(0, min(p.sinks - j0, end))) & use;
+}
+// Of queries at positions p0 .. p0+63, the first n of which exist, those that see key j.
+__device__ __forceinline__ uint64_t queries_seeing(const WinParams& p, int j, int p0, int n) {
+  return bits(j - p.right - p0, min(n, j < p.sinks ? 64 : j + p.left + 1 - p0));
 }
 
 // Keys that queries i0 .. i1-1 see: sinks [0, s_hi) where they lie before the window, and [lo, hi).  Tiles of N keys:
@@ -87,6 +102,36 @@ __device__ __forceinline__ void query_range(const WinParams& p, const Seq& sq, i
 // Slab of one (sequence, key head, sink tile, part): [2][tile rows][d] floats; part 0 is the window, 1 + c chunk c.
 __device__ __forceinline__ float* slab(const WinParams& p, int b, int g, int st, int part, int rows) {
   return p.slabs + ((((int64_t)b * p.G + g) * p.nst + st) * (1 + p.nch) + part) * 2 * rows * p.d;
+}
+
+// The work of a block: tile `tile` of query head h (or key head, where `rep` is 1) of sequence b.  Blocks of one XCD
+// (blockIdx mod 8) should meet in their L2 on the keys and values that the tiles and query heads of a (sequence, key head)
+// share, and each XCD should get the same work.  With a multiple of 8 such units, or many, unit u goes to XCD u mod 8,
+// which spreads a ragged batch evenly (16 packed sequences of 100 to 1000 tokens: dispatched in grid order the XCDs were
+// 62 % busy); else an XCD takes a contiguous run of all tiles.  b == B: the layer that zeroes rows of no sequence.
+struct Work { int tile, h, b; bool none; };
+__host__ __device__ inline bool by_unit(int units) { return units % 8 == 0 || units >= 64; }
+__device__ __forceinline__ Work work_of_block(const WinParams& p, int tiles, int rep) {
+  const int units = (p.B + (p.q_off ? 1 : 0)) * p.G, m = tiles * rep, x = blockIdx.x & 7, s = blockIdx.x >> 3;
+  int u, r;
+  Work w;
+  if (by_unit(units)) {
+    u = (s / m) * 8 + x;
+    r = s % m;
+  } else {
+    const int per = (units * m + 7) >> 3, item = x * per + s;
+    u = s < per ? item / m : units;
+    r = item % m;
+  }
+  w.none = u >= units;
+  w.b = u / p.G;
+  w.h = (u - w.b * p.G) * rep + r / tiles;
+  w.tile = r % tiles;
+  return w;
+}
+inline unsigned work_blocks(const WinParams& p, int tiles, int rep) {
+  const int64_t units = (int64_t)(p.B + (p.q_off ? 1 : 0)) * p.G, m = (int64_t)tiles * rep;
+  return (unsigned)(8 * (by_unit((int)units) ? (units + 7) / 8 * m : (units * m + 7) / 8));
 }
 
 // Rows of a packed tensor that belong to no sequence become zero: columns col0 .. col0 + d - 1 of rows < off[0] and

@@ -21,6 +21,7 @@ namespace {
 
 constexpr int NT = 64;     // rows per LDS tile
 constexpr int MAXD = 128;
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr int MFMA_ROWS = 128;   // key rows of a block of the bf16 path
 
 template <int D> struct Tile { float a[NT][D + 4]; };
@@ -29,22 +30,45 @@ __device__ __forceinline__ f32x4_t mfma4(float x, float y, f32x4_t acc) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(x, y, acc, 0, 0, 0);
 }
 
-// rows r0 .. r0+63 of a matrix as fp32; rows for which ok(row) does not hold and columns beyond d become zero
-template <typename T, int D, class F>
-__device__ __forceinline__ void stage(Tile<D>& t, const T* base, int64_t ld, int r0, int d, F&& ok) {
-  for (int e = threadIdx.x; e < NT * (D / 4); e += 256) {
-    const int r = e / (D / 4), c = (e - r * (D / 4)) * 4;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (c < d && ok(r0 + r)) {
-      const T* s = base + (int64_t)(r0 + r) * ld + c;
-      v.x = Cvt<T>::to_f32(s[0]);
-      if (c + 1 < d) v.y = Cvt<T>::to_f32(s[1]);
-      if (c + 2 < d) v.z = Cvt<T>::to_f32(s[2]);
-      if (c + 3 < d) v.w = Cvt<T>::to_f32(s[3]);
+// A tile of 64 rows on its way: loaded into registers while the tile before is multiplied, converted and written to LDS
+// between two barriers.  Rows are clamped to the matrix; those whose bit in `ok` is clear, and columns beyond d, are
+// written as zeros whatever they hold.
+template <typename T> struct Load4;
+template <> struct Load4<float> { typedef float4 raw; };
+template <> struct Load4<bf16_t> { typedef uint2 raw; };
+template <typename T, int D> struct Stage {
+  typedef typename Load4<T>::raw raw;
+  static constexpr int N = NT * (D / 4) / 256;
+  raw r[N];
+  __device__ __forceinline__ void load(const T* base, int64_t ld, int r0, int rows, int d, bool vec) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int e = threadIdx.x + 256 * k, row = e / (D / 4), c = (e - row * (D / 4)) * 4;
+      const T* s = base + (int64_t)min(r0 + row, rows - 1) * ld;
+      if (vec) {
+        r[k] = *(const raw*)(s + (c < d ? c : 0));
+      } else {
+        T* w = (T*)&r[k];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) w[x] = s[c + x < d ? c + x : 0];
+      }
     }
-    *(float4*)&t.a[r][c] = v;
   }
-}
+  __device__ __forceinline__ void store(Tile<D>& t, uint64_t ok, int d) const {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int e = threadIdx.x + 256 * k, row = e / (D / 4), c = (e - row * (D / 4)) * 4;
+      const T* w = (const T*)&r[k];
+      const bool use = (ok >> row) & 1;
+      float4 v;
+      v.x = use && c < d ? Cvt<T>::to_f32(w[0]) : 0.f;
+      v.y = use && c + 1 < d ? Cvt<T>::to_f32(w[1]) : 0.f;
+      v.z = use && c + 2 < d ? Cvt<T>::to_f32(w[2]) : 0.f;
+      v.w = use && c + 3 < d ? Cvt<T>::to_f32(w[3]) : 0.f;
+      *(float4*)&t.a[row][c] = v;
+    }
+  }
+};
 
 // own row: y[s][j] = element 16 s + 4 g + j
 template <typename T, int D>
@@ -105,67 +129,100 @@ __device__ __forceinline__ void store_own(T* row, const f32x4_t (&o)[D / 16], fl
     }
 }
 
-__device__ __forceinline__ bool padded(const WinParams& p, int b, int j) {
-  return p.key_pad && p.key_pad[(int64_t)b * p.Lk + j];
+// v where the lane's bit 16 k + r of a row mask (shifted right by 4 g) is set, else `other`
+__device__ __forceinline__ float keep_or(float v, uint64_t mask, int k, int r, uint32_t other) {
+  const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)(uint32_t)(mask >> (32 * (k >> 1))), 16 * (k & 1) + r, 1);
+  return __uint_as_float((__float_as_uint(v) & m) | (other & ~m));
 }
+
+// Keys of a sequence as tiles: what forward and dQ sweep.
+template <typename T, int D> struct KeySweep {
+  const WinParams& p;
+  const Seq& sq;
+  const KeyTiles kt;
+  const T *K, *V;
+  const uint8_t* pad;
+  Stage<T, D> k, v;
+  int gone;
+  __device__ __forceinline__ KeySweep(const WinParams& p_, const Seq& sq_, int b, int kh, int i0)
+      : p(p_), sq(sq_), kt(KeyTiles::of<NT>(p_, sq_, i0, min(i0 + 64, sq_.Lq))) {
+    K = (const T*)p.K + sq.kbase * p.ldk + (int64_t)kh * p.d;
+    V = (const T*)p.V + sq.kbase * p.ldv + (int64_t)kh * p.d;
+    pad = p.key_pad ? p.key_pad + (int64_t)b * p.Lk : nullptr;
+    gone = 0;
+    if (kt.n > 0) load(0);
+  }
+  __device__ __forceinline__ int start(int t) const { return kt.start<NT>(t); }
+  __device__ __forceinline__ void load(int t) {
+    const int j0 = start(t);
+    if (pad) gone = pad[min(j0 + (int)(threadIdx.x & 63), sq.Lk - 1)];
+    k.load(K, p.ldk, j0, sq.Lk, p.d, p.vec);
+    v.load(V, p.ldv, j0, sq.Lk, p.d, p.vec);
+  }
+  // tile t into LDS; the next one on its way.  Returns the keys that may be used.
+  __device__ __forceinline__ uint64_t next(int t, Tile<D>& Ks, Tile<D>& Vs) {
+    const uint64_t ok = __ballot(kt.holds(start(t) + (int)(threadIdx.x & 63)) && !gone);
+    __syncthreads();
+    k.store(Ks, ok, p.d);
+    v.store(Vs, ok, p.d);
+    __syncthreads();
+    if (t + 1 < kt.n) load(t + 1);
+    return ok;
+  }
+};
+
+// whether any row of the wave has a bit among the 16 of piece k
+__device__ __forceinline__ bool piece(uint64_t see, int k) { return __any(((see >> (16 * k)) & 0xffff) != 0); }
 
 // ------------------------------------------------------------------------------ forward
 template <typename T, int D>
-__global__ __launch_bounds__(256) void window_fwd_kernel(WinParams p) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 1) void window_fwd_kernel(WinParams p) {
   __shared__ __attribute__((aligned(16))) Tile<D> Ks;
   __shared__ __attribute__((aligned(16))) Tile<D> Vs;
-  __shared__ uint8_t gone[NT];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-  const int b = blockIdx.z, h = blockIdx.y, kh = h / (p.H / p.G);
+  const int qtiles = max(1, (p.Lq + 63) / 64);
+  const Work work = work_of_block(p, qtiles, p.H / p.G);
+  if (work.none) return;
+  const int b = work.b, h = work.h, kh = h / (p.H / p.G);
   if (b == p.B) {   // packed: rows of no sequence
-    zero_rest<T>((T*)p.Oout, p.ldo, (int64_t)h * p.d, p.d, p.q_off, p.B, p.Tq, blockIdx.x, gridDim.x);
+    zero_rest<T>((T*)p.Oout, p.ldo, (int64_t)h * p.d, p.d, p.q_off, p.B, p.Tq, work.tile, qtiles);
     return;
   }
   const Seq sq = seq_of(p, b);
-  const int i0 = blockIdx.x * 64;
+  const int i0 = work.tile * 64;
   if (i0 >= sq.Lq) return;   // block-uniform
   const int i = i0 + wave * 16 + c, pos = i + sq.off;
-  const KeyTiles kt = KeyTiles::of<NT>(p, sq, i0, min(i0 + 64, sq.Lq));
-  const T* K = (const T*)p.K + sq.kbase * p.ldk + (int64_t)kh * p.d;
-  const T* V = (const T*)p.V + sq.kbase * p.ldv + (int64_t)kh * p.d;
+  KeySweep<T, D> keys(p, sq, b, kh, i0);
   f32x4_t fq[D / 16], o[D / 16];
   load_own<T, D>(fq, (const T*)p.Q + (sq.qbase + min(i, sq.Lq - 1)) * p.ldq + (int64_t)h * p.d, p.d, g, i < sq.Lq);
 #pragma unroll
   for (int t = 0; t < D / 16; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const float cs = p.scale * LOG2E;   // scores in units of log 2: exp2 is one instruction, exp a dozen
   float m = -INFINITY, l = 0.f;
-  for (int t = 0; t < kt.n; ++t) {
-    const int j0 = kt.start<NT>(t);
-    __syncthreads();
-    if (threadIdx.x < NT) {
-      const int j = j0 + threadIdx.x;
-      gone[threadIdx.x] = !kt.holds(j) || padded(p, b, j);
-    }
-    __syncthreads();
-    auto ok = [&](int j) { return !gone[j - j0]; };
-    stage<T, D>(Ks, K, p.ldk, j0, p.d, ok);
-    stage<T, D>(Vs, V, p.ldv, j0, p.d, ok);
-    __syncthreads();
+  for (int t = 0; t < keys.kt.n; ++t) {
+    const uint64_t ok = keys.next(t, Ks, Vs), see = i < sq.Lq ? keys_seen(p, pos, keys.start(t), ok) : 0;
+    const uint64_t mk = see >> (4 * g);
     f32x4_t sc[4];
     float mx = -INFINITY;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      sc[k] = dot_rows<D>(Ks, 16 * k, fq, lane);
+      sc[k] = f32x4_t{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      if (!piece(see, k)) continue;
+      sc[k] = dot_rows<D>(Ks, 16 * k, fq, lane) * cs;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int jl = 16 * k + 4 * g + r;
-        sc[k][r] = gone[jl] || !sees(p, pos, j0 + jl) ? -INFINITY : sc[k][r] * p.scale;
+        sc[k][r] = keep_or(sc[k][r], mk, k, r, 0xff800000u);   // -inf
         mx = fmaxf(mx, sc[k][r]);
       }
     }
-    const float mn = fmaxf(m, quad_max(mx));
-    const bool dead = mn == -INFINITY;
-    const float alpha = dead ? 1.f : expf(m - mn);
+    const float mn = fmaxf(m, quad_max(mx)), base = mn == -INFINITY ? 0.f : mn;
+    const float alpha = __builtin_amdgcn_exp2f(m - base);
     float rs = 0.f;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        sc[k][r] = dead ? 0.f : expf(sc[k][r] - mn);
+        sc[k][r] = __builtin_amdgcn_exp2f(sc[k][r] - base);
         rs += sc[k][r];
       }
     l = l * alpha + quad_sum(rs);
@@ -173,145 +230,144 @@ __global__ __launch_bounds__(256) void window_fwd_kernel(WinParams p) {
 #pragma unroll
     for (int x = 0; x < D / 16; ++x) o[x] *= alpha;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) add_cols<D>(o, Vs, 16 * k, sc[k], lane);
+    for (int k = 0; k < 4; ++k)
+      if (piece(see, k)) add_cols<D>(o, Vs, 16 * k, sc[k], lane);
   }
   if (i < sq.Lq) {
-    store_own<T, D>((T*)p.Oout + (sq.qbase + i) * p.ldo + (int64_t)h * p.d, o, l > 0.f ? 1.f / l : 0.f, p.d, g);
-    if (g == 0) p.LSE[(int64_t)h * p.Tq + sq.qbase + i] = l > 0.f ? m + logf(l) : -INFINITY;
+    store_own<T, D>((T*)p.Oout + (sq.qbase + i) * p.ldo + (int64_t)h * p.d, o, l > 0.f || l != l ? 1.f / l : 0.f, p.d, g);
+    if (g == 0) p.LSE[(int64_t)h * p.Tq + sq.qbase + i] = l > 0.f ? m * LN2 + logf(l) : (l != l ? l : -INFINITY);
   }
 }
 
 // ------------------------------------------------------------------------------ dQ, delta
 template <typename T, int D>
-__global__ __launch_bounds__(256) void window_dq_kernel(WinParams p) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 1) void window_dq_kernel(WinParams p) {
   __shared__ __attribute__((aligned(16))) Tile<D> Ks;
   __shared__ __attribute__((aligned(16))) Tile<D> Vs;
-  __shared__ uint8_t gone[NT];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-  const int b = blockIdx.z, h = blockIdx.y, kh = h / (p.H / p.G);
+  const int qtiles = max(1, (p.Lq + 63) / 64);
+  const Work work = work_of_block(p, qtiles, p.H / p.G);
+  if (work.none) return;
+  const int b = work.b, h = work.h, kh = h / (p.H / p.G);
   if (b == p.B) {
-    zero_rest<T>((T*)p.dQ, p.lddq, (int64_t)h * p.d, p.d, p.q_off, p.B, p.Tq, blockIdx.x, gridDim.x);
+    zero_rest<T>((T*)p.dQ, p.lddq, (int64_t)h * p.d, p.d, p.q_off, p.B, p.Tq, work.tile, qtiles);
     return;
   }
   const Seq sq = seq_of(p, b);
-  const int i0 = blockIdx.x * 64;
+  const int i0 = work.tile * 64;
   if (i0 >= sq.Lq) return;
   const int i = i0 + wave * 16 + c, pos = i + sq.off;
   const int64_t row = sq.qbase + min(i, sq.Lq - 1), si = (int64_t)h * p.Tq + row;
-  const KeyTiles kt = KeyTiles::of<NT>(p, sq, i0, min(i0 + 64, sq.Lq));
-  const T* K = (const T*)p.K + sq.kbase * p.ldk + (int64_t)kh * p.d;
-  const T* V = (const T*)p.V + sq.kbase * p.ldv + (int64_t)kh * p.d;
+  KeySweep<T, D> keys(p, sq, b, kh, i0);
   f32x4_t fq[D / 16], fd[D / 16], dq[D / 16];
-  load_own<T, D>(fq, (const T*)p.Q + row * p.ldq + (int64_t)h * p.d, p.d, g, i < sq.Lq);
-  load_own<T, D>(fd, (const T*)p.O + row * p.ldo + (int64_t)h * p.d, p.d, g, i < sq.Lq);
-#pragma unroll
-  for (int t = 0; t < D / 16; ++t) dq[t] = fd[t];
+  load_own<T, D>(fq, (const T*)p.O + row * p.ldo + (int64_t)h * p.d, p.d, g, i < sq.Lq);
   load_own<T, D>(fd, (const T*)p.dO + row * p.lddo + (int64_t)h * p.d, p.d, g, i < sq.Lq);
   float dl = 0.f;
 #pragma unroll
-  for (int t = 0; t < D / 16; ++t)
+  for (int t = 0; t < D / 16; ++t) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) { dl += dq[t][r] * fd[t][r]; dq[t][r] = 0.f; }
+    for (int r = 0; r < 4; ++r) dl += fq[t][r] * fd[t][r];
+    dq[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
   dl = quad_sum(dl);
-  const float lse = p.LSE[si];
+  load_own<T, D>(fq, (const T*)p.Q + row * p.ldq + (int64_t)h * p.d, p.d, g, i < sq.Lq);
+  const float cs = p.scale * LOG2E, lse2 = p.LSE[si] * LOG2E;
   if (i < sq.Lq && g == 0) p.delta[si] = dl;
-  for (int t = 0; t < kt.n; ++t) {
-    const int j0 = kt.start<NT>(t);
-    __syncthreads();
-    if (threadIdx.x < NT) {
-      const int j = j0 + threadIdx.x;
-      gone[threadIdx.x] = !kt.holds(j) || padded(p, b, j);
-    }
-    __syncthreads();
-    auto ok = [&](int j) { return !gone[j - j0]; };
-    stage<T, D>(Ks, K, p.ldk, j0, p.d, ok);
-    stage<T, D>(Vs, V, p.ldv, j0, p.d, ok);
-    __syncthreads();
+  for (int t = 0; t < keys.kt.n; ++t) {
+    const uint64_t ok = keys.next(t, Ks, Vs), see = i < sq.Lq ? keys_seen(p, pos, keys.start(t), ok) : 0;
+    const uint64_t mk = see >> (4 * g);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const f32x4_t sc = dot_rows<D>(Ks, 16 * k, fq, lane), dp = dot_rows<D>(Vs, 16 * k, fd, lane);
-      f32x4_t ds;
+      if (!piece(see, k)) continue;
+      f32x4_t ds = dot_rows<D>(Ks, 16 * k, fq, lane);
+      const f32x4_t dp = dot_rows<D>(Vs, 16 * k, fd, lane);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int jl = 16 * k + 4 * g + r;
-        const bool off = gone[jl] || i >= sq.Lq || !sees(p, pos, j0 + jl);
-        ds[r] = off ? 0.f : expf(sc[r] * p.scale - lse) * (dp[r] - dl) * p.scale;
-      }
+      for (int r = 0; r < 4; ++r)
+        ds[r] = keep_or(__builtin_amdgcn_exp2f(fmaf(ds[r], cs, -lse2)) * (dp[r] - dl), mk, k, r, 0u);
       add_cols<D>(dq, Ks, 16 * k, ds, lane);
     }
   }
-  if (i < sq.Lq) store_own<T, D>((T*)p.dQ + (sq.qbase + i) * p.lddq + (int64_t)h * p.d, dq, 1.f, p.d, g);
+  if (i < sq.Lq) store_own<T, D>((T*)p.dQ + (sq.qbase + i) * p.lddq + (int64_t)h * p.d, dq, p.scale, p.d, g);
 }
 
 // ------------------------------------------------------------------------------ dK, dV
 template <typename T, int D>
-__global__ __launch_bounds__(256) void window_dkv_kernel(WinParams p) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 1) void window_dkv_kernel(WinParams p) {
   __shared__ __attribute__((aligned(16))) Tile<D> Qs;
   __shared__ __attribute__((aligned(16))) Tile<D> Ds;
   __shared__ float s_lse[NT], s_dl[NT];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-  const int b = blockIdx.z, kh = blockIdx.y, rep = p.H / p.G;
-  const int tiles = (p.Lk + NT - 1) / NT;
+  const int ktiles = max(1, (p.Lk + NT - 1) / NT), tiles = ktiles + p.nst * p.nch;
+  const Work work = work_of_block(p, tiles, 1);
+  if (work.none) return;
+  const int b = work.b, kh = work.h, rep = p.H / p.G;
   if (b == p.B) {
-    zero_rest<T>((T*)p.dK, p.lddk, (int64_t)kh * p.d, p.d, p.k_off, p.B, p.Tk, blockIdx.x, gridDim.x);
-    zero_rest<T>((T*)p.dV, p.lddv, (int64_t)kh * p.d, p.d, p.k_off, p.B, p.Tk, blockIdx.x, gridDim.x);
+    zero_rest<T>((T*)p.dK, p.lddk, (int64_t)kh * p.d, p.d, p.k_off, p.B, p.Tk, work.tile, tiles);
+    zero_rest<T>((T*)p.dV, p.lddv, (int64_t)kh * p.d, p.d, p.k_off, p.B, p.Tk, work.tile, tiles);
     return;
   }
   const Seq sq = seq_of(p, b);
-  const int extra = (int)blockIdx.x - tiles;                       // >= 0: a chunk of far queries of a sink tile
-  const int tile = extra < 0 ? (int)blockIdx.x : extra / p.nch, chunk = extra < 0 ? -1 : extra % p.nch;
+  const int extra = work.tile - ktiles;                            // >= 0: a chunk of far queries of a sink tile
+  const int tile = extra < 0 ? work.tile : extra / p.nch, chunk = extra < 0 ? -1 : extra % p.nch;
   const int j0 = tile * NT, j1 = min(j0 + NT, sq.Lk);
   if (j0 >= sq.Lk) return;
   int i_lo, i_hi;
   query_range(p, sq, j0, j1, chunk, i_lo, i_hi);
   if (chunk >= 0 && i_lo >= i_hi) return;   // (the join counts the same chunks)
   const int j = j0 + wave * 16 + c, jrow = min(j, sq.Lk - 1);
-  const bool alive = j < sq.Lk && !padded(p, b, jrow);
-  const bool busy = chunk < 0 || j0 + wave * 16 < p.sinks;         // wave-uniform
+  const bool alive = j < sq.Lk && !(p.key_pad && p.key_pad[(int64_t)b * p.Lk + jrow]);
+  const bool sink = p.nst && j < p.sinks;   // (a sink's sum has further parts)
   f32x4_t fk[D / 16], fv[D / 16], dk[D / 16], dv[D / 16];
   load_own<T, D>(fk, (const T*)p.K + (sq.kbase + jrow) * p.ldk + (int64_t)kh * p.d, p.d, g, alive);
   load_own<T, D>(fv, (const T*)p.V + (sq.kbase + jrow) * p.ldv + (int64_t)kh * p.d, p.d, g, alive);
 #pragma unroll
   for (int t = 0; t < D / 16; ++t) dk[t] = dv[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  for (int hh = 0; hh < rep; ++hh) {
-    const int h = kh * rep + hh;
-    const T* Q = (const T*)p.Q + sq.qbase * p.ldq + (int64_t)h * p.d;
-    const T* dO = (const T*)p.dO + sq.qbase * p.lddo + (int64_t)h * p.d;
-    for (int r0 = i_lo; r0 < i_hi; r0 += NT) {
-      __syncthreads();
-      auto ok = [&](int i) { return i < i_hi; };
-      stage<T, D>(Qs, Q, p.ldq, r0, p.d, ok);
-      stage<T, D>(Ds, dO, p.lddo, r0, p.d, ok);
-      if (threadIdx.x < NT) {
-        const int64_t si = (int64_t)h * p.Tq + sq.qbase + min(r0 + (int)threadIdx.x, sq.Lq - 1);
-        s_lse[threadIdx.x] = p.LSE[si];
-        s_dl[threadIdx.x] = p.delta[si];
-      }
-      __syncthreads();
-      if (!busy) continue;
+  const int per = (i_hi - i_lo + NT - 1) / NT, n = per * rep;
+  const float cs = p.scale * LOG2E;
+  Stage<T, D> stage_q, stage_d;
+  float row_lse = 0.f, row_dl = 0.f;
+  auto load = [&](int t) {
+    const int hh = t / per, r0 = i_lo + (t - hh * per) * NT, h = kh * rep + hh;
+    stage_q.load((const T*)p.Q + sq.qbase * p.ldq + (int64_t)h * p.d, p.ldq, r0, sq.Lq, p.d, p.vec);
+    stage_d.load((const T*)p.dO + sq.qbase * p.lddo + (int64_t)h * p.d, p.lddo, r0, sq.Lq, p.d, p.vec);
+    const int64_t si = (int64_t)h * p.Tq + sq.qbase + min(r0 + (int)(threadIdx.x & 63), sq.Lq - 1);
+    row_lse = p.LSE[si];
+    row_dl = p.delta[si];
+  };
+  if (n > 0) load(0);
+  for (int t = 0; t < n; ++t) {
+    const int r0 = i_lo + (t % per) * NT;
+    const uint64_t ok = bits(0, i_hi - r0);
+    __syncthreads();
+    stage_q.store(Qs, ok, p.d);
+    stage_d.store(Ds, ok, p.d);
+    if (threadIdx.x < NT) { s_lse[threadIdx.x] = row_lse * LOG2E; s_dl[threadIdx.x] = row_dl; }
+    __syncthreads();
+    if (t + 1 < n) load(t + 1);
+    const uint64_t see = alive ? queries_seeing(p, j, r0 + sq.off, i_hi - r0) : 0;
+    const uint64_t mk = see >> (4 * g);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const f32x4_t sc = dot_rows<D>(Qs, 16 * k, fk, lane), dp = dot_rows<D>(Ds, 16 * k, fv, lane);
-        f32x4_t pr, ds;
+    for (int k = 0; k < 4; ++k) {
+      if (!piece(see, k)) continue;
+      f32x4_t pr = dot_rows<D>(Qs, 16 * k, fk, lane), ds = dot_rows<D>(Ds, 16 * k, fv, lane);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int il = 16 * k + 4 * g + r, i = r0 + il;
-          const bool off = !alive || i >= i_hi || !sees(p, i + sq.off, j);
-          pr[r] = off ? 0.f : expf(sc[r] * p.scale - s_lse[il]);
-          ds[r] = off ? 0.f : pr[r] * (dp[r] - s_dl[il]) * p.scale;
-        }
-        add_cols<D>(dv, Ds, 16 * k, pr, lane);
-        add_cols<D>(dk, Qs, 16 * k, ds, lane);
+      for (int r = 0; r < 4; ++r) {
+        const int il = 16 * k + 4 * g + r;
+        const float e = __builtin_amdgcn_exp2f(fmaf(pr[r], cs, -s_lse[il]));
+        ds[r] = keep_or(e * (ds[r] - s_dl[il]), mk, k, r, 0u);
+        pr[r] = keep_or(e, mk, k, r, 0u);
       }
+      add_cols<D>(dv, Ds, 16 * k, pr, lane);
+      add_cols<D>(dk, Qs, 16 * k, ds, lane);
     }
   }
   if (j >= sq.Lk) return;
-  if (j < p.sinks && p.nst) {   // (a sink's sum has further parts)
+  if (sink) {
     float* s = slab(p, b, kh, tile, 1 + chunk, NT) + (int64_t)(j - j0) * p.d;
-    store_own<float, D>(s, dk, 1.f, p.d, g);
+    store_own<float, D>(s, dk, p.scale, p.d, g);
     store_own<float, D>(s + (int64_t)NT * p.d, dv, 1.f, p.d, g);
   } else if (chunk < 0) {
-    store_own<T, D>((T*)p.dK + (sq.kbase + j) * p.lddk + (int64_t)kh * p.d, dk, 1.f, p.d, g);
+    store_own<T, D>((T*)p.dK + (sq.kbase + j) * p.lddk + (int64_t)kh * p.d, dk, p.scale, p.d, g);
     store_own<T, D>((T*)p.dV + (sq.kbase + j) * p.lddv + (int64_t)kh * p.d, dv, 1.f, p.d, g);
   }
 }
@@ -337,6 +393,13 @@ __global__ __launch_bounds__(256) void window_join_kernel(WinParams p, int rows)
   }
   ((T*)p.dK)[(sq.kbase + j) * p.lddk + (int64_t)kh * p.d + c] = Cvt<T>::from_f32(a);
   ((T*)p.dV)[(sq.kbase + j) * p.lddv + (int64_t)kh * p.d + c] = Cvt<T>::from_f32(v);
+}
+
+// whether every row of the operands that go through LDS is made of whole 4-element pieces
+bool whole_pieces(const WinParams& p, int dtype) {
+  const int64_t size = dtype == SK_BF16 ? 2 : 4;
+  return p.d % 4 == 0 && (p.ldq | p.ldk | p.ldv | p.lddo) % 4 == 0 &&
+         (((uintptr_t)p.Q | (uintptr_t)p.K | (uintptr_t)p.V | (uintptr_t)p.dO) & (4 * size - 1)) == 0;
 }
 
 int check(const char* who, const WinParams& p, int window, int dtype) {
@@ -377,17 +440,15 @@ int64_t slab_floats(const WinParams& p, int rows) {
 
 template <typename T, int D>
 void launch_fwd(const WinParams& p, hipStream_t stream) {
-  dim3 grid(std::max(1, (p.Lq + 63) / 64), p.H, p.B + (p.q_off ? 1 : 0));
+  const dim3 grid(work_blocks(p, std::max(1, (p.Lq + 63) / 64), p.H / p.G));
   hipLaunchKernelGGL((window_fwd_kernel<T, D>), grid, dim3(256), 0, stream, p);
 }
 template <typename T, int D>
 void launch_bwd(const WinParams& p, hipStream_t stream) {
-  const int layers = p.B + (p.q_off ? 1 : 0);
-  if (p.Tq)
-    hipLaunchKernelGGL((window_dq_kernel<T, D>), dim3(std::max(1, (p.Lq + 63) / 64), p.H, layers), dim3(256), 0, stream, p);
-  if (p.Tk)
-    hipLaunchKernelGGL((window_dkv_kernel<T, D>), dim3(std::max(1, (p.Lk + NT - 1) / NT + p.nst * p.nch), p.G, layers), dim3(256),
-                       0, stream, p);
+  const dim3 gq(work_blocks(p, std::max(1, (p.Lq + 63) / 64), p.H / p.G));
+  const dim3 gk(work_blocks(p, std::max(1, (p.Lk + NT - 1) / NT) + p.nst * p.nch, 1));
+  if (p.Tq) hipLaunchKernelGGL((window_dq_kernel<T, D>), gq, dim3(256), 0, stream, p);
+  if (p.Tk) hipLaunchKernelGGL((window_dkv_kernel<T, D>), gk, dim3(256), 0, stream, p);
 }
 
 }  // namespace
@@ -430,6 +491,7 @@ extern "C" int skhip_window_attn_fwd(const void* Q, const void* K, const void* V
   SK_CHECK_ARG(Q && O && LSE && (Tk == 0 || (K && V)), "%s: null pointer", who);
   set_window(p, window, causal);
   if (sk_window_mfma_supported(p, dtype)) return sk_window_fwd_mfma(p, stream);
+  p.vec = whole_pieces(p, dtype);
   if (dtype == SK_BF16) {
     if (d <= 64) launch_fwd<bf16_t, 64>(p, stream); else launch_fwd<bf16_t, 128>(p, stream);
   } else {
@@ -471,6 +533,7 @@ extern "C" int skhip_window_attn_bwd(const void* Q, const void* K, const void* V
   }
   p.delta = workspace;
   p.slabs = workspace + (head + 3) / 4 * 4;   // (16-byte stores)
+  p.vec = whole_pieces(p, dtype);
   if (mfma) {
     rc = sk_window_bwd_mfma(p, stream);
     return rc ? rc : sk_window_join(p, MFMA_ROWS, dtype, stream);

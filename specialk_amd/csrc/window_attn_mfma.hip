@@ -16,6 +16,7 @@
 // wholly invisible to it are skipped but for the barrier.
 #include "window_attn.h"
 #include <algorithm>
+#include <type_traits>
 
 using namespace skwin;
 
@@ -140,19 +141,13 @@ __device__ __forceinline__ void store_own_f32(float* row, const f32x16_t (&o)[D 
     }
 }
 
-// bits a .. b-1 of 64 (any a, b)
-__device__ __forceinline__ uint64_t bits(int a, int b) {
-  a = min(max(a, 0), 64);
-  b = min(max(b, 0), 64);
-  const uint64_t hi = b == 64 ? ~0ull : (1ull << b) - 1, lo = a == 64 ? ~0ull : (1ull << a) - 1;
-  return hi & ~lo;
-}
-
-// Work item of a block: blocks of one XCD (blockIdx mod 8) take a contiguous run of items, so that neighbouring tiles of a
-// sequence, which read the same rows of the other side, meet in one L2.
-__device__ __forceinline__ int item_of_block(int n) {
-  const int per = (n + 7) >> 3, w = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-  return (int)(blockIdx.x >> 3) < per && w < n ? w : -1;
+// All ones where register r's bit of the row mask is set, else 0: mk is the tile half's 32 bits, shifted by 4 h.
+__device__ __forceinline__ uint32_t lane_bit(uint32_t mk, int r) { return (uint32_t)__builtin_amdgcn_sbfe((int)mk, 8 * (r >> 2) + (r & 3), 1); }
+// (opaque(mk) inside a wave-uniform `if` keeps that a branch: hoisted and turned into selects, the masks of the few partly
+// visible tiles would cost every tile three instructions a score)
+__device__ __forceinline__ void opaque(uint32_t& mk) { asm volatile("" : "+v"(mk)); }
+__device__ __forceinline__ float keep_or(float v, uint32_t m, uint32_t other) {
+  return __uint_as_float((__float_as_uint(v) & m) | (other & ~m));
 }
 
 // ------------------------------------------------------------------------------ forward
@@ -164,9 +159,9 @@ template <int D>
 __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void fwd_kernel(WinParams p, int qtiles) {
   __shared__ __attribute__((aligned(1024))) char lds[2][2 * tile_bytes<D>()];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, hf = lane >> 5;
-  const int layers = p.B + (p.q_off ? 1 : 0), item = item_of_block(qtiles * p.H * layers);
-  if (item < 0) return;
-  const int tile = item % qtiles, h = (item / qtiles) % p.H, b = item / (qtiles * p.H), kh = h / (p.H / p.G);
+  const Work work = work_of_block(p, qtiles, p.H / p.G);
+  if (work.none) return;
+  const int tile = work.tile, h = work.h, b = work.b, kh = h / (p.H / p.G);
   if (b == p.B) {
     zero_rest<bf16_t>((bf16_t*)p.Oout, p.ldo, (int64_t)h * p.d, p.d, p.q_off, p.B, p.Tq, tile, qtiles);
     return;
@@ -219,7 +214,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void fwd_kernel(WinParams p, 
       gone = padding(t + 2);
     }
     const int j0 = kt.start<NT>(t);
-    if (pmax < pmin || j0 > pmax + p.right || (j0 + NT - 1 < pmin - p.left && j0 >= p.sinks)) continue;   // wave-uniform
+    if (use == 0 || pmax < pmin || j0 > pmax + p.right || (j0 + NT - 1 < pmin - p.left && j0 >= p.sinks)) continue;   // wave-uniform
     const char* Ks = lds[t & 1];
     const char* Vs = Ks + tile_bytes<D>();
     f32x16_t sc[2];
@@ -231,13 +226,14 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void fwd_kernel(WinParams p, 
     }
     const bool whole = use == ~0ull && j0 + NT - 1 <= pmin + p.right && (j0 >= pmax - p.left || j0 + NT <= p.sinks);
     if (!whole) {
-      const uint64_t see = (bits(pos - p.left - j0, pos + p.right + 1 - j0) | (bits(0, p.sinks - j0) & bits(0, pos + p.right + 1 - j0))) & use;
+      const uint64_t see = keys_seen(p, pos, j0, use);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const uint32_t mk = (uint32_t)(see >> (32 * k)) >> (4 * hf);
+        uint32_t mk = (uint32_t)(see >> (32 * k)) >> (4 * hf);
+        opaque(mk);
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (!((mk >> (8 * (r >> 2) + (r & 3))) & 1)) sc[k][r] = -INFINITY;
+          sc[k][r] = keep_or(sc[k][r], lane_bit(mk, r), 0xff800000u);   // -inf
       }
     }
     float mx = sc[0][0];
@@ -283,13 +279,18 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void fwd_kernel(WinParams p, 
 // ------------------------------------------------------------------------------ dQ, delta
 // Also leaves the rows' log-sum-exp in units of log 2 and delta = rowsum(dO O) for the dK / dV kernel.  dS is rounded to
 // bf16 without the scale, which multiplies the fp32 sums at the end.
+// O carries two roundings to 2^-8 (the probabilities', its own), and delta inherits them: against the rounding of dS
+// itself that is 1 / sqrt(n) as much for a row that sees n keys alike.  Blocks with a row of at most FEW keys (the
+// first rows of a text, rows behind it, small windows) take delta = sum_j P dP in fp32 from a sweep of its own: with four
+// visible keys dQ and dK are then 1.4 instead of 1.65 times as far from the exact values as a result rounded once.
+constexpr int FEW = 32;
 template <int D>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dq_kernel(WinParams p, int qtiles) {
   __shared__ __attribute__((aligned(1024))) char lds[2][2 * tile_bytes<D>()];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, hf = lane >> 5;
-  const int layers = p.B + (p.q_off ? 1 : 0), item = item_of_block(qtiles * p.H * layers);
-  if (item < 0) return;
-  const int tile = item % qtiles, h = (item / qtiles) % p.H, b = item / (qtiles * p.H), kh = h / (p.H / p.G);
+  const Work work = work_of_block(p, qtiles, p.H / p.G);
+  if (work.none) return;
+  const int tile = work.tile, h = work.h, b = work.b, kh = h / (p.H / p.G);
   if (b == p.B) {
     zero_rest<bf16_t>((bf16_t*)p.dQ, p.lddq, (int64_t)h * p.d, p.d, p.q_off, p.B, p.Tq, tile, qtiles);
     return;
@@ -316,10 +317,6 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dq_kernel(WinParams p, i
   dl = other_sum(dl);
   load_own<D>(q, (const bf16_t*)p.Q + row * p.ldq + (int64_t)h * p.d, p.d, hf, i < sq.Lq);
   const float lse2 = p.LSE[si] * LOG2E;
-  if (i < sq.Lq && hf == 0) {
-    p.delta[si] = dl;
-    p.delta[(int64_t)p.H * p.Tq + si] = lse2;
-  }
   f32x16_t dq[D / 32];
 #pragma unroll
   for (int t = 0; t < D / 32; ++t) dq[t] = zero16();
@@ -333,46 +330,36 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dq_kernel(WinParams p, i
     load_tile<D>(buf, K + j0 * p.ldk, p.ldk, p.d, ok, wave, lane);
     load_tile<D>(buf + tile_bytes<D>(), V + j0 * p.ldv, p.ldv, p.d, ok, wave, lane);
   };
-  uint64_t ok = 0;
-  int gone = padding(0);
-  if (kt.n > 0) { ok = usable(0, gone); fetch(0, ok); }
-  gone = padding(1);
-  for (int t = 0; t < kt.n; ++t) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    const uint64_t use = ok;
-    if (t + 1 < kt.n) {
-      ok = usable(t + 1, gone);
-      fetch(t + 1, ok);
-      gone = padding(t + 2);
+  int count = 0;
+  for (int t = kt.n - 1; t >= 0; --t) {
+    count += __popcll(keys_seen(p, pos, kt.start<NT>(t), usable(t, padding(t))));
+    if (__all(count > FEW || i >= sq.Lq)) break;
+  }
+  const bool few = __syncthreads_or(i < sq.Lq && count <= FEW);
+  // one half tile: scores and dP; then the half's part of delta, or dS and its product
+  auto half_tile = [&](auto delta_only, bool whole, const char* Ks, const char* Vs, int k, uint32_t mk) {
+    f32x16_t sc = zero16(), dp = zero16();
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      sc = mfma(x_rows<D>(Ks, 32 * k, s, lane), q[s], sc);
+      dp = mfma(x_rows<D>(Vs, 32 * k, s, lane), g[s], dp);
     }
-    const int j0 = kt.start<NT>(t);
-    if (pmax < pmin || j0 > pmax + p.right || (j0 + NT - 1 < pmin - p.left && j0 >= p.sinks)) continue;
-    const char* Ks = lds[t & 1];
-    const char* Vs = Ks + tile_bytes<D>();
-    const bool whole = use == ~0ull && j0 + NT - 1 <= pmin + p.right && (j0 >= pmax - p.left || j0 + NT <= p.sinks);
-    uint64_t see = ~0ull;
-    if (!whole)
-      see = (bits(pos - p.left - j0, pos + p.right + 1 - j0) | (bits(0, p.sinks - j0) & bits(0, pos + p.right + 1 - j0))) & use;
+    float part = 0.f;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      f32x16_t sc = zero16(), dp = zero16();
+    for (int r = 0; r < 16; ++r) {
+      const float pr = __builtin_amdgcn_exp2f(fmaf(sc[r], cs, -lse2));
+      sc[r] = pr * (delta_only ? dp[r] : dp[r] - dl);
+    }
+    if (!whole) {
+      opaque(mk);
 #pragma unroll
-      for (int s = 0; s < D / 16; ++s) {
-        sc = mfma(x_rows<D>(Ks, 32 * k, s, lane), q[s], sc);
-        dp = mfma(x_rows<D>(Vs, 32 * k, s, lane), g[s], dp);
-      }
-      const uint32_t mk = (uint32_t)(see >> (32 * k)) >> (4 * hf);
+      for (int r = 0; r < 16; ++r) sc[r] = keep_or(sc[r], lane_bit(mk, r), 0u);
+    }
+    if (delta_only) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float pr = __builtin_amdgcn_exp2f(fmaf(sc[r], cs, -lse2));
-        sc[r] = pr * (dp[r] - dl);
-      }
-      if (!whole) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (!((mk >> (8 * (r >> 2) + (r & 3))) & 1)) sc[r] = 0.f;
-      }
+      for (int r = 0; r < 16; ++r) part += sc[r];
+    }
+    if constexpr (!delta_only) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const bf16x8_t y = pack_y(sc, s);
@@ -380,23 +367,64 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dq_kernel(WinParams p, i
         for (int x = 0; x < D / 32; ++x) dq[x] = mfma(x_cols<D>(Ks, 32 * x, 32 * k + 16 * s, lane), y, dq[x]);
       }
     }
+    return part;
+  };
+  auto sweep = [&](auto delta_only) {
+    uint64_t ok = 0;
+    int gone = padding(0);
+    float sum = 0.f;
+    if (kt.n > 0) { ok = usable(0, gone); fetch(0, ok); }
+    gone = padding(1);
+    for (int t = 0; t < kt.n; ++t) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      const uint64_t use = ok;
+      if (t + 1 < kt.n) {
+        ok = usable(t + 1, gone);
+        fetch(t + 1, ok);
+        gone = padding(t + 2);
+      }
+      const int j0 = kt.start<NT>(t);
+      if (use == 0 || pmax < pmin || j0 > pmax + p.right || (j0 + NT - 1 < pmin - p.left && j0 >= p.sinks)) continue;
+      const char* Ks = lds[t & 1];
+      const char* Vs = Ks + tile_bytes<D>();
+      const bool whole = use == ~0ull && j0 + NT - 1 <= pmin + p.right && (j0 >= pmax - p.left || j0 + NT <= p.sinks);
+      const uint64_t see = whole ? 0 : keys_seen(p, pos, j0, use);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) sum += half_tile(delta_only, whole, Ks, Vs, k, (uint32_t)(see >> (32 * k)) >> (4 * hf));
+    }
+    return sum;
+  };
+  if (few) {
+    dl = other_sum(sweep(std::true_type{}));
+    __syncthreads();   // every wave is done with the tiles
+  }
+  sweep(std::false_type{});
+  if (i < sq.Lq && hf == 0) {
+    p.delta[si] = dl;
+    p.delta[(int64_t)p.H * p.Tq + si] = lse2;
   }
   store_own<D>((bf16_t*)p.dQ + row * p.lddq + (int64_t)h * p.d, dq, p.scale, p.d, hf, i < sq.Lq);
 }
 
 // ------------------------------------------------------------------------------ dK, dV
 // Own rows are keys; the tiles hold 64 queries and their output gradients, head after head of the group that shares them.
-template <int D>
+// WHAT: 1 = dK, 2 = dV, 3 = both.  At a width of 64 one launch computes both.  At 128 the two sums and the own rows alone
+// are 192 registers, and with them only one wave fits a SIMD: dK and dV as launches of their own cost the scores twice
+// (10 instead of 8 products) but keep two (16384 tokens, causal, 16 heads: 3.73 ms together, 1.67 + 1.25 ms apart).
+template <int D, int WHAT>
 __global__ __launch_bounds__(256, 2) void dkv_kernel(WinParams p, int ktiles) {
+  constexpr bool DK = WHAT & 1, DV = WHAT & 2;
   __shared__ __attribute__((aligned(1024))) char lds[2][2 * tile_bytes<D>()];
   __shared__ __attribute__((aligned(16))) float rowv[2][2][NT];   // log-sum-exp (log 2 units), delta
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, hf = lane >> 5;
-  const int tiles = ktiles + p.nst * p.nch, layers = p.B + (p.q_off ? 1 : 0), item = item_of_block(tiles * p.G * layers);
-  if (item < 0) return;
-  const int work = item % tiles, kh = (item / tiles) % p.G, b = item / (tiles * p.G), rep = p.H / p.G;
+  const int tiles = ktiles + p.nst * p.nch;
+  const Work item = work_of_block(p, tiles, 1);
+  if (item.none) return;
+  const int work = item.tile, kh = item.h, b = item.b, rep = p.H / p.G;
   if (b == p.B) {
-    zero_rest<bf16_t>((bf16_t*)p.dK, p.lddk, (int64_t)kh * p.d, p.d, p.k_off, p.B, p.Tk, work, tiles);
-    zero_rest<bf16_t>((bf16_t*)p.dV, p.lddv, (int64_t)kh * p.d, p.d, p.k_off, p.B, p.Tk, work, tiles);
+    if (DK) zero_rest<bf16_t>((bf16_t*)p.dK, p.lddk, (int64_t)kh * p.d, p.d, p.k_off, p.B, p.Tk, work, tiles);
+    if (DV) zero_rest<bf16_t>((bf16_t*)p.dV, p.lddv, (int64_t)kh * p.d, p.d, p.k_off, p.B, p.Tk, work, tiles);
     return;
   }
   const Seq sq = seq_of(p, b);
@@ -411,7 +439,7 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(WinParams p, int ktiles) {
   const bool all_alive = __all(alive), busy = jw < sq.Lk && (chunk < 0 || jw < p.sinks);   // wave-uniform
   bf16x8_t fk[D / 16], fv[D / 16];
   load_own<D>(fk, (const bf16_t*)p.K + (sq.kbase + jrow) * p.ldk + (int64_t)kh * p.d, p.d, hf, alive);
-  load_own<D>(fv, (const bf16_t*)p.V + (sq.kbase + jrow) * p.ldv + (int64_t)kh * p.d, p.d, hf, alive);
+  if (DK) load_own<D>(fv, (const bf16_t*)p.V + (sq.kbase + jrow) * p.ldv + (int64_t)kh * p.d, p.d, hf, alive);
   const float cs = p.scale * LOG2E;
   f32x16_t dk[D / 32], dv[D / 32];
 #pragma unroll
@@ -430,6 +458,43 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(WinParams p, int ktiles) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)rowv[t & 1][wave], 4, r0 + lane < i_hi ? lane * 4 : NOWHERE, 0, 0, 0);
     }
   };
+  auto half_tile = [&](bool whole, const char* Qs, const char* Gs, const float (*rv)[NT], int k, uint32_t mk) {
+    f32x16_t sc = zero16(), dp = zero16();
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      sc = mfma(x_rows<D>(Qs, 32 * k, s, lane), fk[s], sc);
+      if (DK) dp = mfma(x_rows<D>(Gs, 32 * k, s, lane), fv[s], dp);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float4 ls = *(const float4*)&rv[0][32 * k + 8 * u + 4 * hf], de = *(const float4*)&rv[1][32 * k + 8 * u + 4 * hf];
+      const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, ev[4] = {de.x, de.y, de.z, de.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 4 * u + e;
+        sc[r] = __builtin_amdgcn_exp2f(fmaf(sc[r], cs, -lv[e]));
+        dp[r] = sc[r] * (dp[r] - ev[e]);
+      }
+    }
+    if (!whole) {
+      opaque(mk);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const uint32_t m = lane_bit(mk, r);
+        sc[r] = keep_or(sc[r], m, 0u);
+        dp[r] = keep_or(dp[r], m, 0u);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const bf16x8_t yp = pack_y(sc, s), ys = pack_y(dp, s);
+#pragma unroll
+      for (int x = 0; x < D / 32; ++x) {
+        if (DV) dv[x] = mfma(x_cols<D>(Gs, 32 * x, 32 * k + 16 * s, lane), yp, dv[x]);
+        if (DK) dk[x] = mfma(x_cols<D>(Qs, 32 * x, 32 * k + 16 * s, lane), ys, dk[x]);
+      }
+    }
+  };
   if (n > 0) fetch(0);
   for (int t = 0; t < n; ++t) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -441,56 +506,20 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(WinParams p, int ktiles) {
     const char* Gs = Qs + tile_bytes<D>();
     const float (*rv)[NT] = rowv[t & 1];
     const bool whole = all_alive && r0 + NT <= i_hi && jl <= p0 + p.right && (jw >= p1 - p.left || jl < p.sinks);
-    uint64_t see = ~0ull;
-    if (!whole) {
-      see = bits(j - p.right - p0, j < p.sinks ? NT : j + p.left + 1 - p0) & bits(0, i_hi - r0);
-      if (!alive) see = 0;
-    }
+    uint64_t see = 0;
+    if (!whole && alive) see = queries_seeing(p, j, p0, i_hi - r0);
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      f32x16_t sc = zero16(), dp = zero16();
-#pragma unroll
-      for (int s = 0; s < D / 16; ++s) {
-        sc = mfma(x_rows<D>(Qs, 32 * k, s, lane), fk[s], sc);
-        dp = mfma(x_rows<D>(Gs, 32 * k, s, lane), fv[s], dp);
-      }
-      const uint32_t mk = (uint32_t)(see >> (32 * k)) >> (4 * hf);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const float4 ls = *(const float4*)&rv[0][32 * k + 8 * u + 4 * hf], de = *(const float4*)&rv[1][32 * k + 8 * u + 4 * hf];
-        const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, ev[4] = {de.x, de.y, de.z, de.w};
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float pr = __builtin_amdgcn_exp2f(fmaf(sc[4 * u + r], cs, -lv[r]));
-          sc[4 * u + r] = pr;
-          dp[4 * u + r] = pr * (dp[4 * u + r] - ev[r]);
-        }
-      }
-      if (!whole) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (!((mk >> (8 * (r >> 2) + (r & 3))) & 1)) { sc[r] = 0.f; dp[r] = 0.f; }
-      }
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const bf16x8_t yp = pack_y(sc, s), ys = pack_y(dp, s);
-#pragma unroll
-        for (int x = 0; x < D / 32; ++x) {
-          dv[x] = mfma(x_cols<D>(Gs, 32 * x, 32 * k + 16 * s, lane), yp, dv[x]);
-          dk[x] = mfma(x_cols<D>(Qs, 32 * x, 32 * k + 16 * s, lane), ys, dk[x]);
-        }
-      }
-    }
+    for (int k = 0; k < 2; ++k) half_tile(whole, Qs, Gs, rv, k, (uint32_t)(see >> (32 * k)) >> (4 * hf));
   }
   const bool sink = p.nst && j < p.sinks;   // (a sink's sum has further parts)
   if (sink && j < sq.Lk) {
     float* s = slab(p, b, kh, tile, 1 + chunk, OWN) + (int64_t)(j - j0) * p.d;
-    store_own_f32<D>(s, dk, p.scale, p.d, hf);
-    store_own_f32<D>(s + (int64_t)OWN * p.d, dv, 1.f, p.d, hf);
+    if (DK) store_own_f32<D>(s, dk, p.scale, p.d, hf);
+    if (DV) store_own_f32<D>(s + (int64_t)OWN * p.d, dv, 1.f, p.d, hf);
   }
   if (chunk >= 0) return;
-  store_own<D>((bf16_t*)p.dK + (sq.kbase + jrow) * p.lddk + (int64_t)kh * p.d, dk, p.scale, p.d, hf, j < sq.Lk && !sink);
-  store_own<D>((bf16_t*)p.dV + (sq.kbase + jrow) * p.lddv + (int64_t)kh * p.d, dv, 1.f, p.d, hf, j < sq.Lk && !sink);
+  if (DK) store_own<D>((bf16_t*)p.dK + (sq.kbase + jrow) * p.lddk + (int64_t)kh * p.d, dk, p.scale, p.d, hf, j < sq.Lk && !sink);
+  if (DV) store_own<D>((bf16_t*)p.dV + (sq.kbase + jrow) * p.lddv + (int64_t)kh * p.d, dv, 1.f, p.d, hf, j < sq.Lk && !sink);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -511,11 +540,9 @@ bool sk_window_mfma_supported(const WinParams& p, int dtype) {
   return tiles * p.H * (p.B + 1) < (1ll << 30);
 }
 
-static unsigned grid_of(int64_t items) { return (unsigned)(8 * ((items + 7) / 8)); }
-
 int sk_window_fwd_mfma(const WinParams& p, hipStream_t stream) {
-  const int layers = p.B + (p.q_off ? 1 : 0), qtiles = std::max(1, (p.Lq + OWN - 1) / OWN);
-  const dim3 grid(grid_of((int64_t)qtiles * p.H * layers));
+  const int qtiles = std::max(1, (p.Lq + OWN - 1) / OWN);
+  const dim3 grid(work_blocks(p, qtiles, p.H / p.G));
   if (p.d <= 64) hipLaunchKernelGGL((fwd_kernel<64>), grid, dim3(256), 0, stream, p, qtiles);
   else hipLaunchKernelGGL((fwd_kernel<128>), grid, dim3(256), 0, stream, p, qtiles);
   SK_CHECK_LAUNCH("skhip_window_attn_fwd(mfma)");
@@ -523,15 +550,15 @@ int sk_window_fwd_mfma(const WinParams& p, hipStream_t stream) {
 }
 
 int sk_window_bwd_mfma(const WinParams& p, hipStream_t stream) {
-  const int layers = p.B + (p.q_off ? 1 : 0), qtiles = std::max(1, (p.Lq + OWN - 1) / OWN);
-  const int ktiles = std::max(1, (p.Lk + OWN - 1) / OWN);
-  const dim3 gq(grid_of((int64_t)qtiles * p.H * layers)), gk(grid_of((int64_t)(ktiles + p.nst * p.nch) * p.G * layers));
+  const int qtiles = std::max(1, (p.Lq + OWN - 1) / OWN), ktiles = std::max(1, (p.Lk + OWN - 1) / OWN);
+  const dim3 gq(work_blocks(p, qtiles, p.H / p.G)), gk(work_blocks(p, ktiles + p.nst * p.nch, 1));
   if (p.d <= 64) {
     if (p.Tq) hipLaunchKernelGGL((dq_kernel<64>), gq, dim3(256), 0, stream, p, qtiles);
-    if (p.Tk) hipLaunchKernelGGL((dkv_kernel<64>), gk, dim3(256), 0, stream, p, ktiles);
+    if (p.Tk) hipLaunchKernelGGL((dkv_kernel<64, 3>), gk, dim3(256), 0, stream, p, ktiles);
   } else {
     if (p.Tq) hipLaunchKernelGGL((dq_kernel<128>), gq, dim3(256), 0, stream, p, qtiles);
-    if (p.Tk) hipLaunchKernelGGL((dkv_kernel<128>), gk, dim3(256), 0, stream, p, ktiles);
+    if (p.Tk) hipLaunchKernelGGL((dkv_kernel<128, 1>), gk, dim3(256), 0, stream, p, ktiles);
+    if (p.Tk) hipLaunchKernelGGL((dkv_kernel<128, 2>), gk, dim3(256), 0, stream, p, ktiles);
   }
   SK_CHECK_LAUNCH("skhip_window_attn_bwd(mfma)");
   return SK_OK;
