@@ -104,34 +104,54 @@ __device__ __forceinline__ float* slab(const WinParams& p, int b, int g, int st,
   return p.slabs + ((((int64_t)b * p.G + g) * p.nst + st) * (1 + p.nch) + part) * 2 * rows * p.d;
 }
 
-// The work of a block: tile `tile` of query head h (or key head, where `rep` is 1) of sequence b.  Blocks of one XCD
-// (blockIdx mod 8) should meet in their L2 on the keys and values that the tiles and query heads of a (sequence, key head)
-// share, and each XCD should get the same work.  With a multiple of 8 such units, or many, unit u goes to XCD u mod 8,
-// which spreads a ragged batch evenly (16 packed sequences of 100 to 1000 tokens: dispatched in grid order the XCDs were
-// 62 % busy); else an XCD takes a contiguous run of all tiles.  b == B: the layer that zeroes rows of no sequence.
+// The work of a block: tile `tile` of query head h (or key head, where `rep` is 1) of sequence b; the last blocks of a packed
+// batch's grid (b == B) zero rows of no sequence, TAIL parts a head.
+//  * A (sequence, key head) is a unit, whose keys and values its tiles and query heads share in the L2 of one XCD
+//    (blockIdx mod 8).  Every row of 8 units gives each XCD one, turned by one from row to row: with 8 key heads an XCD
+//    that kept the same head would read one 128-byte piece of every row, an eighth of its L2's channels (256 sequences of
+//    200 tokens: dQ 96 us, turned 88).  Few units that do not fill rows are dealt tile by tile instead.
+//  * Within an XCD the tile is the slowest index.  With the tiles of a sequence side by side, a batch where half of them
+//    are empty repeats "two full, two empty", and the dispatcher, which deals blocks to 4 shader engines in turn, leaves
+//    two engines without work (256 x 200 tokens given as at most 400: forward 81 instead of 55 us).
+//  * Late tiles first where they are the long ones (queries of a causal text), early ones first for keys.
 struct Work { int tile, h, b; bool none; };
+constexpr int TAIL = 8;
 __host__ __device__ inline bool by_unit(int units) { return units % 8 == 0 || units >= 64; }
-__device__ __forceinline__ Work work_of_block(const WinParams& p, int tiles, int rep) {
-  const int units = (p.B + (p.q_off ? 1 : 0)) * p.G, m = tiles * rep, x = blockIdx.x & 7, s = blockIdx.x >> 3;
-  int u, r;
+__host__ __device__ inline int main_blocks(int units, int tiles, int rep) {
+  return by_unit(units) ? 8 * ((units + 7) / 8) * tiles * rep : units * tiles * rep;
+}
+__device__ __forceinline__ Work work_of_block(const WinParams& p, int tiles, int rep, bool late_first) {
+  const int units = p.B * p.G, main = main_blocks(units, tiles, rep), i = blockIdx.x;
   Work w;
+  w.none = false;
+  if (i >= main) {
+    w.b = p.B;
+    w.tile = (i - main) / (p.G * rep);
+    w.h = (i - main) - w.tile * (p.G * rep);
+    return w;
+  }
+  int u, r;
   if (by_unit(units)) {
-    u = (s / m) * 8 + x;
-    r = s % m;
+    const int rows = (units + 7) >> 3, x = i & 7, s = i >> 3;
+    w.tile = s / (rows * rep);
+    r = s - w.tile * (rows * rep);
+    const int row = r / rep;
+    u = row * 8 + ((x - row) & 7);
+    r -= row * rep;
   } else {
-    const int per = (units * m + 7) >> 3, item = x * per + s;
-    u = s < per ? item / m : units;
-    r = item % m;
+    w.tile = i / (units * rep);
+    r = i - w.tile * (units * rep);
+    u = r / rep;
+    r -= u * rep;
   }
   w.none = u >= units;
   w.b = u / p.G;
-  w.h = (u - w.b * p.G) * rep + r / tiles;
-  w.tile = r % tiles;
+  w.h = (u - w.b * p.G) * rep + r;
+  if (late_first) w.tile = tiles - 1 - w.tile;
   return w;
 }
 inline unsigned work_blocks(const WinParams& p, int tiles, int rep) {
-  const int64_t units = (int64_t)(p.B + (p.q_off ? 1 : 0)) * p.G, m = (int64_t)tiles * rep;
-  return (unsigned)(8 * (by_unit((int)units) ? (units + 7) / 8 * m : (units * m + 7) / 8));
+  return (unsigned)(main_blocks(p.B * p.G, tiles, rep) + (p.q_off ? TAIL * p.G * rep : 0));
 }
 
 // Rows of a packed tensor that belong to no sequence become zero: columns col0 .. col0 + d - 1 of rows < off[0] and

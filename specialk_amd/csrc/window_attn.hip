@@ -181,11 +181,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 1) void window_fwd_kernel(WinPar
   __shared__ __attribute__((aligned(16))) Tile<D> Vs;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
   const int qtiles = max(1, (p.Lq + 63) / 64);
-  const Work work = work_of_block(p, qtiles, p.H / p.G);
+  const Work work = work_of_block(p, qtiles, p.H / p.G, true);
   if (work.none) return;
   const int b = work.b, h = work.h, kh = h / (p.H / p.G);
   if (b == p.B) {   // packed: rows of no sequence
-    zero_rest<T>((T*)p.Oout, p.ldo, (int64_t)h * p.d, p.d, p.q_off, p.B, p.Tq, work.tile, qtiles);
+    zero_rest<T>((T*)p.Oout, p.ldo, (int64_t)h * p.d, p.d, p.q_off, p.B, p.Tq, work.tile, TAIL);
     return;
   }
   const Seq sq = seq_of(p, b);
@@ -246,11 +246,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 1) void window_dq_kernel(WinPara
   __shared__ __attribute__((aligned(16))) Tile<D> Vs;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
   const int qtiles = max(1, (p.Lq + 63) / 64);
-  const Work work = work_of_block(p, qtiles, p.H / p.G);
+  const Work work = work_of_block(p, qtiles, p.H / p.G, true);
   if (work.none) return;
   const int b = work.b, h = work.h, kh = h / (p.H / p.G);
   if (b == p.B) {
-    zero_rest<T>((T*)p.dQ, p.lddq, (int64_t)h * p.d, p.d, p.q_off, p.B, p.Tq, work.tile, qtiles);
+    zero_rest<T>((T*)p.dQ, p.lddq, (int64_t)h * p.d, p.d, p.q_off, p.B, p.Tq, work.tile, TAIL);
     return;
   }
   const Seq sq = seq_of(p, b);
@@ -298,12 +298,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 1) void window_dkv_kernel(WinPar
   __shared__ float s_lse[NT], s_dl[NT];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
   const int ktiles = max(1, (p.Lk + NT - 1) / NT), tiles = ktiles + p.nst * p.nch;
-  const Work work = work_of_block(p, tiles, 1);
+  const Work work = work_of_block(p, tiles, 1, false);
   if (work.none) return;
   const int b = work.b, kh = work.h, rep = p.H / p.G;
   if (b == p.B) {
-    zero_rest<T>((T*)p.dK, p.lddk, (int64_t)kh * p.d, p.d, p.k_off, p.B, p.Tk, work.tile, tiles);
-    zero_rest<T>((T*)p.dV, p.lddv, (int64_t)kh * p.d, p.d, p.k_off, p.B, p.Tk, work.tile, tiles);
+    zero_rest<T>((T*)p.dK, p.lddk, (int64_t)kh * p.d, p.d, p.k_off, p.B, p.Tk, work.tile, TAIL);
+    zero_rest<T>((T*)p.dV, p.lddv, (int64_t)kh * p.d, p.d, p.k_off, p.B, p.Tk, work.tile, TAIL);
     return;
   }
   const Seq sq = seq_of(p, b);

@@ -159,11 +159,11 @@ template <int D>
 __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void fwd_kernel(WinParams p, int qtiles) {
   __shared__ __attribute__((aligned(1024))) char lds[2][2 * tile_bytes<D>()];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, hf = lane >> 5;
-  const Work work = work_of_block(p, qtiles, p.H / p.G);
+  const Work work = work_of_block(p, qtiles, p.H / p.G, true);
   if (work.none) return;
   const int tile = work.tile, h = work.h, b = work.b, kh = h / (p.H / p.G);
   if (b == p.B) {
-    zero_rest<bf16_t>((bf16_t*)p.Oout, p.ldo, (int64_t)h * p.d, p.d, p.q_off, p.B, p.Tq, tile, qtiles);
+    zero_rest<bf16_t>((bf16_t*)p.Oout, p.ldo, (int64_t)h * p.d, p.d, p.q_off, p.B, p.Tq, tile, TAIL);
     return;
   }
   const Seq sq = seq_of(p, b);
@@ -288,11 +288,11 @@ template <int D>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dq_kernel(WinParams p, int qtiles) {
   __shared__ __attribute__((aligned(1024))) char lds[2][2 * tile_bytes<D>()];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, hf = lane >> 5;
-  const Work work = work_of_block(p, qtiles, p.H / p.G);
+  const Work work = work_of_block(p, qtiles, p.H / p.G, true);
   if (work.none) return;
   const int tile = work.tile, h = work.h, b = work.b, kh = h / (p.H / p.G);
   if (b == p.B) {
-    zero_rest<bf16_t>((bf16_t*)p.dQ, p.lddq, (int64_t)h * p.d, p.d, p.q_off, p.B, p.Tq, tile, qtiles);
+    zero_rest<bf16_t>((bf16_t*)p.dQ, p.lddq, (int64_t)h * p.d, p.d, p.q_off, p.B, p.Tq, tile, TAIL);
     return;
   }
   const Seq sq = seq_of(p, b);
@@ -419,12 +419,12 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(WinParams p, int ktiles) {
   __shared__ __attribute__((aligned(16))) float rowv[2][2][NT];   // log-sum-exp (log 2 units), delta
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, hf = lane >> 5;
   const int tiles = ktiles + p.nst * p.nch;
-  const Work item = work_of_block(p, tiles, 1);
+  const Work item = work_of_block(p, tiles, 1, false);
   if (item.none) return;
   const int work = item.tile, kh = item.h, b = item.b, rep = p.H / p.G;
   if (b == p.B) {
-    if (DK) zero_rest<bf16_t>((bf16_t*)p.dK, p.lddk, (int64_t)kh * p.d, p.d, p.k_off, p.B, p.Tk, work, tiles);
-    if (DV) zero_rest<bf16_t>((bf16_t*)p.dV, p.lddv, (int64_t)kh * p.d, p.d, p.k_off, p.B, p.Tk, work, tiles);
+    if (DK) zero_rest<bf16_t>((bf16_t*)p.dK, p.lddk, (int64_t)kh * p.d, p.d, p.k_off, p.B, p.Tk, work, TAIL);
+    if (DV) zero_rest<bf16_t>((bf16_t*)p.dV, p.lddv, (int64_t)kh * p.d, p.d, p.k_off, p.B, p.Tk, work, TAIL);
     return;
   }
   const Seq sq = seq_of(p, b);
@@ -537,7 +537,7 @@ bool sk_window_mfma_supported(const WinParams& p, int dtype) {
   for (const void* x : ptr)
     if (!aligned16(x)) return false;
   const int64_t tiles = (int64_t)(std::max(p.Lq, p.Lk) / OWN + 1) + (int64_t)p.nst * p.nch;
-  return tiles * p.H * (p.B + 1) < (1ll << 30);
+  return tiles * p.H * (p.B + 8) < (1ll << 30);
 }
 
 int sk_window_fwd_mfma(const WinParams& p, hipStream_t stream) {
