@@ -15,7 +15,7 @@ struct WinParams {
   const void *Q, *K, *V, *O, *dO;
   void *Oout, *dQ, *dK, *dV;
   float* LSE;               // [H][Tq]
-  float* delta;             // [H][Tq]; bf16 path: then the log-sum-exp in units of log 2, [H][Tq]
+  float* delta;             // [H][Tq]; bf16 path: -delta, then -log-sum-exp / scale, [H][Tq] each
   float* slabs;             // partial dK, dV of the tiles that hold sinks (see below)
   const uint8_t* key_pad;   // [B][Lk]; padded batches only
   const int32_t* q_off;     // packed batches: rows of sequence b are q_off[b] .. q_off[b+1]-1; NULL: (B, Lq) rows

@@ -277,7 +277,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void fwd_kernel(WinParams p, 
 }
 
 // ------------------------------------------------------------------------------ dQ, delta
-// Also leaves the rows' log-sum-exp in units of log 2 and delta = rowsum(dO O) for the dK / dV kernel.  dS is rounded to
+// Also leaves the rows' -log-sum-exp / scale and -delta, delta = rowsum(dO O), for the dK / dV kernel.  dS is rounded to
 // bf16 without the scale, which multiplies the fp32 sums at the end.
 // O carries two roundings to 2^-8 (the probabilities', its own), and delta inherits them: against the rounding of dS
 // itself that is 1 / sqrt(n) as much for a row that sees n keys alike.  Blocks with a row of at most FEW keys (the
@@ -400,9 +400,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dq_kernel(WinParams p, i
     __syncthreads();   // every wave is done with the tiles
   }
   sweep(std::false_type{});
-  if (i < sq.Lq && hf == 0) {
-    p.delta[si] = dl;
-    p.delta[(int64_t)p.H * p.Tq + si] = lse2;
+  if (i < sq.Lq && hf == 0) {   // what the dK / dV kernel's accumulators start from
+    p.delta[si] = -dl;
+    p.delta[(int64_t)p.H * p.Tq + si] = -p.LSE[si] / p.scale;
   }
   store_own<D>((bf16_t*)p.dQ + row * p.lddq + (int64_t)h * p.d, dq, p.scale, p.d, hf, i < sq.Lq);
 }
@@ -413,10 +413,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dq_kernel(WinParams p, i
 // are 192 registers, and with them only one wave fits a SIMD: dK and dV as launches of their own cost the scores twice
 // (10 instead of 8 products) but keep two (16384 tokens, causal, 16 heads: 3.73 ms together, 1.67 + 1.25 ms apart).
 template <int D, int WHAT>
-__global__ __launch_bounds__(256, 2) void dkv_kernel(WinParams p, int ktiles) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dkv_kernel(WinParams p, int ktiles) {
   constexpr bool DK = WHAT & 1, DV = WHAT & 2;
   __shared__ __attribute__((aligned(1024))) char lds[2][2 * tile_bytes<D>()];
-  __shared__ __attribute__((aligned(16))) float rowv[2][2][NT];   // log-sum-exp (log 2 units), delta
+  __shared__ __attribute__((aligned(16))) float rowv[2][2][NT];   // -log-sum-exp / scale, -delta
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, hf = lane >> 5;
   const int tiles = ktiles + p.nst * p.nch;
   const Work item = work_of_block(p, tiles, 1, false);
@@ -459,22 +459,23 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(WinParams p, int ktiles) {
     }
   };
   auto half_tile = [&](bool whole, const char* Qs, const char* Gs, const float (*rv)[NT], int k, uint32_t mk) {
-    f32x16_t sc = zero16(), dp = zero16();
+    // the sums start from the rows' -log-sum-exp / scale and -delta: no registers for them and no subtraction
+    f32x16_t sc, dp;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float4 ls = *(const float4*)&rv[0][32 * k + 8 * u + 4 * hf], de = *(const float4*)&rv[1][32 * k + 8 * u + 4 * hf];
+      sc[4 * u] = ls.x; sc[4 * u + 1] = ls.y; sc[4 * u + 2] = ls.z; sc[4 * u + 3] = ls.w;
+      dp[4 * u] = de.x; dp[4 * u + 1] = de.y; dp[4 * u + 2] = de.z; dp[4 * u + 3] = de.w;
+    }
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) {
       sc = mfma(x_rows<D>(Qs, 32 * k, s, lane), fk[s], sc);
       if (DK) dp = mfma(x_rows<D>(Gs, 32 * k, s, lane), fv[s], dp);
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const float4 ls = *(const float4*)&rv[0][32 * k + 8 * u + 4 * hf], de = *(const float4*)&rv[1][32 * k + 8 * u + 4 * hf];
-      const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, ev[4] = {de.x, de.y, de.z, de.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = 4 * u + e;
-        sc[r] = __builtin_amdgcn_exp2f(fmaf(sc[r], cs, -lv[e]));
-        dp[r] = sc[r] * (dp[r] - ev[e]);
-      }
+    for (int r = 0; r < 16; ++r) {
+      sc[r] = __builtin_amdgcn_exp2f(sc[r] * cs);
+      dp[r] *= sc[r];
     }
     if (!whole) {
       opaque(mk);
@@ -508,7 +509,7 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(WinParams p, int ktiles) {
     const bool whole = all_alive && r0 + NT <= i_hi && jl <= p0 + p.right && (jw >= p1 - p.left || jl < p.sinks);
     uint64_t see = 0;
     if (!whole && alive) see = queries_seeing(p, j, p0, i_hi - r0);
-#pragma unroll
+#pragma unroll(D == 64 ? 1 : 2)
     for (int k = 0; k < 2; ++k) half_tile(whole, Qs, Gs, rv, k, (uint32_t)(see >> (32 * k)) >> (4 * hf));
   }
   const bool sink = p.nst && j < p.sinks;   // (a sink's sum has further parts)
