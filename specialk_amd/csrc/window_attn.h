@@ -99,9 +99,10 @@ __device__ __forceinline__ void query_range(const WinParams& p, const Seq& sq, i
   }
 }
 
-// Slab of one (sequence, key head, sink tile, part): [2][tile rows][d] floats; part 0 is the window, 1 + c chunk c.
-__device__ __forceinline__ float* slab(const WinParams& p, int b, int g, int st, int part, int rows) {
-  return p.slabs + ((((int64_t)b * p.G + g) * p.nst + st) * (1 + p.nch) + part) * 2 * rows * p.d;
+// Slab of one (sequence, key head, sink tile, part): [2][sinks of a tile][d] floats; part 0 is the window, 1 + c chunk c.
+__host__ __device__ inline int slab_rows(const WinParams& p, int tile_rows) { return p.sinks < tile_rows ? p.sinks : tile_rows; }
+__device__ __forceinline__ float* slab(const WinParams& p, int b, int g, int st, int part, int tile_rows) {
+  return p.slabs + ((((int64_t)b * p.G + g) * p.nst + st) * (1 + p.nch) + part) * 2 * slab_rows(p, tile_rows) * p.d;
 }
 
 // The work of a block: tile `tile` of query head h (or key head, where `rep` is 1) of sequence b; the last blocks of a packed
@@ -113,7 +114,8 @@ __device__ __forceinline__ float* slab(const WinParams& p, int b, int g, int st,
 //  * Within an XCD the tile is the slowest index.  With the tiles of a sequence side by side, a batch where half of them
 //    are empty repeats "two full, two empty", and the dispatcher, which deals blocks to 4 shader engines in turn, leaves
 //    two engines without work (256 x 200 tokens given as at most 400: forward 81 instead of 55 us).
-//  * Late tiles first where they are the long ones (queries of a causal text), early ones first for keys.
+//  * Late tiles first where they are the long ones (queries of a causal text; the chunks of far queries behind the key
+//    tiles), else early ones first (keys of a causal text).
 struct Work { int tile, h, b; bool none; };
 constexpr int TAIL = 8;
 __host__ __device__ inline bool by_unit(int units) { return units % 8 == 0 || units >= 64; }

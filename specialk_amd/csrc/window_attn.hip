@@ -298,7 +298,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 1) void window_dkv_kernel(WinPar
   __shared__ float s_lse[NT], s_dl[NT];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
   const int ktiles = max(1, (p.Lk + NT - 1) / NT), tiles = ktiles + p.nst * p.nch;
-  const Work work = work_of_block(p, tiles, 1, false);
+  const Work work = work_of_block(p, tiles, 1, p.nst > 0);
   if (work.none) return;
   const int b = work.b, kh = work.h, rep = p.H / p.G;
   if (b == p.B) {
@@ -365,7 +365,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 1) void window_dkv_kernel(WinPar
   if (sink) {
     float* s = slab(p, b, kh, tile, 1 + chunk, NT) + (int64_t)(j - j0) * p.d;
     store_own<float, D>(s, dk, p.scale, p.d, g);
-    store_own<float, D>(s + (int64_t)NT * p.d, dv, 1.f, p.d, g);
+    store_own<float, D>(s + (int64_t)slab_rows(p, NT) * p.d, dv, 1.f, p.d, g);
   } else if (chunk < 0) {
     store_own<T, D>((T*)p.dK + (sq.kbase + j) * p.lddk + (int64_t)kh * p.d, dk, p.scale, p.d, g);
     store_own<T, D>((T*)p.dV + (sq.kbase + j) * p.lddv + (int64_t)kh * p.d, dv, 1.f, p.d, g);
@@ -384,12 +384,12 @@ __global__ __launch_bounds__(256) void window_join_kernel(WinParams p, int rows)
   query_range(p, sq, j0, min(j0 + rows, sq.Lk), 0, lo, hi);
   if (lo < hi) parts += (sq.Lq - lo + p.ch - 1) / p.ch;
   const float* x = slab(p, b, kh, tile, 0, rows) + (int64_t)(j - j0) * p.d + c;
-  const int64_t step = (int64_t)2 * rows * p.d;
+  const int64_t half = (int64_t)slab_rows(p, rows) * p.d, step = 2 * half;
   float a = 0.f, v = 0.f;
 #pragma unroll 8
   for (int s = 0; s < parts; ++s) {
     a += x[s * step];
-    v += x[s * step + (int64_t)rows * p.d];
+    v += x[s * step + half];
   }
   ((T*)p.dK)[(sq.kbase + j) * p.lddk + (int64_t)kh * p.d + c] = Cvt<T>::from_f32(a);
   ((T*)p.dV)[(sq.kbase + j) * p.lddv + (int64_t)kh * p.d + c] = Cvt<T>::from_f32(v);
@@ -425,17 +425,17 @@ void set_window(WinParams& p, int window, int causal) {
   p.sinks = std::min(p.sinks, p.Lk);
 }
 
-// Tiles that hold sinks and the chunks their far queries are cut into: as many rows per chunk as a key tile's own window
-// has, so that these blocks last no longer than the others.
+// Tiles that hold sinks and the chunks their far queries are cut into: about as many rows per chunk as a key tile's own
+// window has, so that these blocks last no longer than the others.
 void plan_sinks(WinParams& p, int rows) {
   const bool far = p.sinks > 0 && p.left < p.Lk;   // else every query's window reaches key 0
   p.nst = far ? (p.sinks + rows - 1) / rows : 0;
-  p.ch = std::max(512, (p.left + p.right + rows + 63) / 64 * 64);
+  p.ch = std::max(256, (p.left + p.right + rows + 63) / 64 * 64);
   p.nch = far ? (p.Lq + p.ch - 1) / p.ch : 0;
 }
 
 int64_t slab_floats(const WinParams& p, int rows) {
-  return (int64_t)p.B * p.G * p.nst * (1 + p.nch) * 2 * rows * p.d;
+  return (int64_t)p.B * p.G * p.nst * (1 + p.nch) * 2 * slab_rows(p, rows) * p.d;
 }
 
 template <typename T, int D>

@@ -419,7 +419,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dkv_kernel(WinParams p, 
   __shared__ __attribute__((aligned(16))) float rowv[2][2][NT];   // -log-sum-exp / scale, -delta
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, hf = lane >> 5;
   const int tiles = ktiles + p.nst * p.nch;
-  const Work item = work_of_block(p, tiles, 1, false);
+  const Work item = work_of_block(p, tiles, 1, p.nst > 0);
   if (item.none) return;
   const int work = item.tile, kh = item.h, b = item.b, rep = p.H / p.G;
   if (b == p.B) {
@@ -516,7 +516,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dkv_kernel(WinParams p, 
   if (sink && j < sq.Lk) {
     float* s = slab(p, b, kh, tile, 1 + chunk, OWN) + (int64_t)(j - j0) * p.d;
     if (DK) store_own_f32<D>(s, dk, p.scale, p.d, hf);
-    if (DV) store_own_f32<D>(s + (int64_t)OWN * p.d, dv, 1.f, p.d, hf);
+    if (DV) store_own_f32<D>(s + (int64_t)slab_rows(p, OWN) * p.d, dv, 1.f, p.d, hf);
   }
   if (chunk >= 0) return;
   if (DK) store_own<D>((bf16_t*)p.dK + (sq.kbase + jrow) * p.lddk + (int64_t)kh * p.d, dk, p.scale, p.d, hf, j < sq.Lk && !sink);

@@ -9,9 +9,8 @@
 // most CUs idle, so the visible positions are cut into splits, each block leaves the running maximum, sum and weighted
 // value of its part in the workspace, and a second small kernel joins them.
 //
-// bf16 heads of whole 16-byte pieces run on the matrix cores (v_mfma_f32_16x16x32_bf16): the query heads that share a key
-// head are the 16 columns of every product, so keys and values are read once for all of them.  Other rows and fp32 take
-// one block per query head on the vector ALU.
+// Heads of whole 16-byte pieces run on the matrix cores: the query heads that share a key head are the 16 columns of every
+// product, so keys and values are read once for all of them.  Other rows take one block per query head on the vector ALU.
 #include "window_attn.h"
 #include <algorithm>
 
@@ -100,9 +99,9 @@ __global__ __launch_bounds__(256) void step_kernel(StepParams p, int vec) {
     const int cnt = min(KT, u_end - u0);
 #pragma unroll 4
     for (int t = 0; t < cnt; ++t) {
-      const float w = __shfl(pr, t, 64);
-      const int64_t at = __shfl(row, t, 64);
-      const bool fr = __shfl((int)fresh, t, 64);
+      const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(pr), t));
+      const int64_t at = __builtin_amdgcn_readlane((int)row, t);   // (slots are below 2^30)
+      const bool fr = __builtin_amdgcn_readlane((int)fresh, t);
       const T* vr = fr ? vn : V + at * p.vp;
       if (lane < p.d) {
         const T x = vr[lane];
@@ -142,37 +141,95 @@ __global__ __launch_bounds__(256) void step_kernel(StepParams p, int vec) {
 typedef __attribute__((address_space(1))) void* gbl_ptr;
 typedef __attribute__((address_space(3))) void* lds_ptr;
 constexpr float LOG2E = 1.44269504088896340736f;
-constexpr int MT = 32;      // positions per pass of a wave
 constexpr int HEADS = 16;   // query heads per block
 
-__device__ __forceinline__ f32x4_t mfma16(bf16x8_t x, bf16x8_t y, f32x4_t acc) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, acc, 0, 0, 0);
-}
-// byte address of chunk `chunk` of row `row` of a tile of D columns: chunks exchanged with the row, so that the
-// transposing reads spread over the banks
-template <int D> __device__ __forceinline__ int at(int row, int chunk) { return row * (2 * D) + ((chunk ^ (row & 7)) << 4); }
+// byte address of 16-byte piece `piece` of row `row` of a tile whose rows are `bytes` long: pieces exchanged with the row,
+// so that reads by columns spread over the banks
+__device__ __forceinline__ int at(int bytes, int row, int piece) { return row * bytes + ((piece ^ (row & 7)) << 4); }
 
-// Products are D[rho][c] = sum_k X[rho][k] Y[c][k] with the query head on c = lane & 15: scores = keys (straight from
-// memory, a lane's 16 bytes of a row) x queries; output = values (transposed LDS read) x probabilities, which the score
-// accumulators are in the order 4 g + r, 16 + 4 g + r (g = lane / 16).  Every wave keeps two passes of 32 positions in
-// flight: the next pass's keys in registers and values in its own LDS buffer, by direct loads, while this one is
-// multiplied; nothing is shared between waves until the end.  Positions beyond the split read its first one again and
-// are masked, elements beyond the head its first piece against a zero query.
-template <int D>
+// A pass of a wave: MT positions.  Products are D[rho][c] = sum_k X[rho][k] Y[c][k] with the query head on c = lane & 15
+// and g = lane / 16; scores = keys x queries, piece t holding positions 16 t + 4 g + r in register r; output = values x
+// probabilities, for which the scores' registers are the Y operand as they stand.
+template <typename T, int D> struct Pass;
+
+template <int D> struct Pass<bf16_t, D> {   // v_mfma_f32_16x16x32_bf16
+  static constexpr int MT = 32, PIECES = 2, NK = D / 32;
+  typedef bf16x8_t frag;
+  static __device__ __forceinline__ int first(int s, int g) { return 32 * s + 8 * g; }
+  static __device__ __forceinline__ uint32_t sign() { return 0x80008000u; }
+  static __device__ __forceinline__ f32x4_t scores(const frag (&k)[NK], const frag (&q)[NK]) {
+    f32x4_t a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < NK; ++s) a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[s], q[s], a, 0, 0, 0);
+    return a;
+  }
+  // o[x] (columns 16 x + 4 g + r) = alpha o[x] + values x probabilities.  The probabilities are rounded to bf16: half a
+  // step of 2^-8 each, as the output's own rounding.
+  static __device__ __forceinline__ void add(f32x4_t (&o)[D / 16], float alpha, const f32x4_t (&p)[PIECES], const char* v, int c, int g) {
+    bf16x8_t y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { y[e] = (__bf16)p[0][e]; y[4 + e] = (__bf16)p[1][e]; }
+#pragma unroll
+    for (int x = 0; x < D / 16; ++x) {
+      typedef __attribute__((address_space(3))) s16x4_t* lds_v4;
+      const int row = 4 * g + (c >> 2), col = 16 * x + 4 * (c & 3);
+      s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)(v + at(2 * D, row, col >> 3) + (col & 7) * 2));
+      s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)(v + at(2 * D, row + 16, col >> 3) + (col & 7) * 2));
+      s16x8_t f = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      o[x] *= alpha;
+      o[x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, f), y, o[x], 0, 0, 0);
+    }
+  }
+};
+
+template <int D> struct Pass<float, D> {    // v_mfma_f32_16x16x4_f32
+  static constexpr int MT = 16, PIECES = 1, NK = D / 16;
+  typedef f32x4_t frag;
+  static __device__ __forceinline__ int first(int s, int g) { return 16 * s + 4 * g; }
+  static __device__ __forceinline__ uint32_t sign() { return 0x80000000u; }
+  static __device__ __forceinline__ f32x4_t scores(const frag (&k)[NK], const frag (&q)[NK]) {
+    f32x4_t a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < NK; ++s)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][j], q[s][j], a, 0, 0, 0);
+    return a;
+  }
+  static __device__ __forceinline__ void add(f32x4_t (&o)[D / 16], float alpha, const f32x4_t (&p)[PIECES], const char* v, int c, int g) {
+#pragma unroll
+    for (int x = 0; x < D / 16; ++x) o[x] *= alpha;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x) {
+        const float w = *(const float*)(v + at(4 * D, 4 * g + r, 4 * x + (c >> 2)) + (c & 3) * 4);
+        o[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, p[0][r], o[x], 0, 0, 0);
+      }
+  }
+};
+
+// Every wave keeps two passes in flight: the next pass's keys in registers and values in its own LDS buffer, by direct
+// loads, while this one is multiplied; nothing is shared between waves until the end.  Positions beyond the split read its
+// first one again and are masked, elements beyond the head its first piece against a zero query.
+template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void step_mfma_kernel(StepParams p, int chunks) {
-  constexpr int NS = D / 32, NV = D / 16, CH = D / 8, RPI = 64 / CH;   // k steps, value instructions, pieces per row, rows per instruction
-  constexpr int TILE = MT * 2 * D, LDO = D + 4;
-  __shared__ __attribute__((aligned(1024))) char lds[8 * TILE > 4 * HEADS * LDO * 4 ? 8 * TILE : 4 * HEADS * LDO * 4];
+  typedef Pass<T, D> P;
+  typedef typename P::frag frag;
+  constexpr int MT = P::MT, NK = P::NK, PE = 16 / sizeof(T);     // elements of a 16-byte piece
+  constexpr int CH = D / PE, RPI = 64 / CH, NV = MT / RPI;       // pieces per row, rows per instruction, instructions per tile
+  constexpr int ROWB = D * sizeof(T), TILE = MT * ROWB, LDO = D + 4;
+  constexpr int BYTES = 8 * TILE > 4 * HEADS * LDO * 4 ? 8 * TILE : 4 * HEADS * LDO * 4;
+  __shared__ __attribute__((aligned(1024))) char lds[BYTES];
   __shared__ float s_m[4][HEADS], s_l[4][HEADS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
   const int r = blockIdx.z, kh = blockIdx.y / chunks, hc = blockIdx.y - kh * chunks, split = blockIdx.x;
   const int rep = p.H / p.G, h0 = kh * rep + hc * HEADS, nh = min(HEADS, rep - hc * HEADS);
   const Visible vis(p, r);
   const int u_beg = split * p.per, u_end = min(vis.count, u_beg + p.per);
-  bf16_t* K = (bf16_t*)p.kc + r * p.ks + (int64_t)kh * p.d;
-  bf16_t* V = (bf16_t*)p.vc + r * p.vs + (int64_t)kh * p.d;
-  const bf16_t* kn = p.kn ? (const bf16_t*)p.kn + r * p.ldn + (int64_t)kh * p.d : nullptr;
-  const bf16_t* vn = p.vn ? (const bf16_t*)p.vn + r * p.ldn + (int64_t)kh * p.d : nullptr;
+  T* K = (T*)p.kc + r * p.ks + (int64_t)kh * p.d;
+  T* V = (T*)p.vc + r * p.vs + (int64_t)kh * p.d;
+  const T* kn = p.kn ? (const T*)p.kn + r * p.ldn + (int64_t)kh * p.d : nullptr;
+  const T* vn = p.vn ? (const T*)p.vn + r * p.ldn + (int64_t)kh * p.d : nullptr;
   // slots without a division per position: the window meets the ring's end at most once
   const int ring = p.cap - p.sinks, x0 = max(vis.lo, p.sinks), b0 = (x0 - p.sinks) % ring;
   auto slot = [&](int u) -> int64_t {
@@ -181,56 +238,54 @@ __global__ __launch_bounds__(256, 2) void step_mfma_kernel(StepParams p, int chu
     s -= s >= ring ? ring : 0;
     return j < p.sinks ? j : p.sinks + s;
   };
-  bf16x8_t q[NS];
+  frag q[NK];
 #pragma unroll
-  for (int s = 0; s < NS; ++s) {
+  for (int s = 0; s < NK; ++s) {
     uint4 v = make_uint4(0, 0, 0, 0);
-    const int e = 32 * s + 8 * g;
-    if (c < nh && e < p.d) v = *(const uint4*)((const bf16_t*)p.q + r * p.ldq + (int64_t)(h0 + c) * p.d + e);
-    if (p.scale < 0.f) { v.x ^= 0x80008000u; v.y ^= 0x80008000u; v.z ^= 0x80008000u; v.w ^= 0x80008000u; }
-    q[s] = __builtin_bit_cast(bf16x8_t, v);
+    const int e = P::first(s, g);
+    if (c < nh && e < p.d) v = *(const uint4*)((const T*)p.q + r * p.ldq + (int64_t)(h0 + c) * p.d + e);
+    if (p.scale < 0.f) { v.x ^= P::sign(); v.y ^= P::sign(); v.z ^= P::sign(); v.w ^= P::sign(); }   // (maxima are of unscaled scores)
+    q[s] = __builtin_bit_cast(frag, v);
   }
   const float cs = fabsf(p.scale) * LOG2E;
-  f32x4_t o[NV];
+  f32x4_t o[D / 16];
 #pragma unroll
-  for (int t = 0; t < NV; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < D / 16; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
 
-  bf16x8_t kc[2][NS], kx[2][NS];
+  frag ka[P::PIECES][NK], kb[P::PIECES][NK];
   char* mine = lds + wave * 2 * TILE;
-  auto fetch = [&](int u0, char* buf, bf16x8_t (&k)[2][NS]) {
+  auto fetch = [&](int u0, char* buf, frag (&k)[P::PIECES][NK]) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int row = j * RPI + lane / CH, piece = (lane % CH) ^ (row & 7);
       const int u = u0 + row < u_end ? u0 + row : u0;
       const bool fresh = vn && vis.pos(u) == vis.n - 1;
-      const bf16_t* src = (fresh ? vn : V + slot(u) * p.vp) + (piece * 8 < p.d ? piece * 8 : 0);
+      const T* src = (fresh ? vn : V + slot(u) * p.vp) + (piece * PE < p.d ? piece * PE : 0);
       __builtin_amdgcn_global_load_lds((gbl_ptr)src, (lds_ptr)(buf + j * 1024), 16, 0, 0);
     }
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < P::PIECES; ++t) {
       const int u = u0 + 16 * t + c < u_end ? u0 + 16 * t + c : u0;
       const bool fresh = kn && vis.pos(u) == vis.n - 1;
-      const bf16_t* src = fresh ? kn : K + slot(u) * p.kp;
+      const T* src = fresh ? kn : K + slot(u) * p.kp;
 #pragma unroll
-      for (int s = 0; s < NS; ++s) k[t][s] = *(const bf16x8_t*)(src + (32 * s + 8 * g < p.d ? 32 * s + 8 * g : 0));
+      for (int s = 0; s < NK; ++s) k[t][s] = *(const frag*)(src + (P::first(s, g) < p.d ? P::first(s, g) : 0));
     }
   };
   // one pass from registers `k` and buffer `vt`, while the next one is fetched into the others
-  auto pass = [&](int u0, bf16x8_t (&k)[2][NS], bf16x8_t (&next)[2][NS], char* vt, char* vnext) {
+  auto pass = [&](int u0, frag (&k)[P::PIECES][NK], frag (&next)[P::PIECES][NK], char* vt, char* vnext) {
     if (u0 + 4 * MT < u_end) {
       fetch(u0 + 4 * MT, vnext, next);
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NV + 2 * NS) : "memory");
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NV + P::PIECES * NK) : "memory");
     } else {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-    f32x4_t sc[2];
+    f32x4_t sc[P::PIECES];
     float mx = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      sc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < NS; ++s) sc[t] = mfma16(k[t][s], q[s], sc[t]);
+    for (int t = 0; t < P::PIECES; ++t) {
+      sc[t] = P::scores(k[t], q);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if (u0 + 16 * t + 4 * g + e >= u_end) sc[t][e] = -INFINITY;
@@ -244,32 +299,20 @@ __global__ __launch_bounds__(256, 2) void step_mfma_kernel(StepParams p, int chu
     m = mn;
     float sum = 0.f;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < P::PIECES; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         sc[t][e] = __builtin_amdgcn_exp2f(fmaf(sc[t][e], cs, -mc));
         sum += sc[t][e];
       }
     l = l * alpha + sum;      // (of this lane's positions; the four lanes of a head are added at the end)
-    bf16x8_t y;               // probabilities rounded to bf16: half a step of 2^-8 each, as the output's own rounding
-#pragma unroll
-    for (int e = 0; e < 4; ++e) { y[e] = (__bf16)sc[0][e]; y[4 + e] = (__bf16)sc[1][e]; }
-#pragma unroll
-    for (int x = 0; x < NV; ++x) {
-      typedef __attribute__((address_space(3))) s16x4_t* lds_v4;
-      const int row = 4 * g + (c >> 2), col = 16 * x + 4 * (c & 3);
-      s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)(vt + at<D>(row, col >> 3) + (col & 7) * 2));
-      s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)(vt + at<D>(row + 16, col >> 3) + (col & 7) * 2));
-      s16x8_t f = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      o[x] *= alpha;
-      o[x] = mfma16(__builtin_bit_cast(bf16x8_t, f), y, o[x]);
-    }
+    P::add(o, alpha, sc, vt, c, g);
   };
   const int first = u_beg + wave * MT;
-  if (first < u_end) fetch(first, mine, kc);
+  if (first < u_end) fetch(first, mine, ka);
   for (int u0 = first; u0 < u_end; u0 += 8 * MT) {   // (two passes a round: no register moves, which would wait for the loads)
-    pass(u0, kc, kx, mine, mine + TILE);
-    if (u0 + 4 * MT < u_end) pass(u0 + 4 * MT, kx, kc, mine + TILE, mine);
+    pass(u0, ka, kb, mine, mine + TILE);
+    if (u0 + 4 * MT < u_end) pass(u0 + 4 * MT, kb, ka, mine + TILE, mine);
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
@@ -277,9 +320,10 @@ __global__ __launch_bounds__(256, 2) void step_mfma_kernel(StepParams p, int chu
   // the newest key and value go into their slot (every reader took them from the new rows)
   if (kn && hc == 0 && vis.count > 0 && u_beg < vis.count && u_end == vis.count) {
     const int64_t at_slot = slot(vis.count - 1);
-    for (int e = threadIdx.x; e < p.d / 4; e += 256) {   // 8 bytes a thread: keys, then values
-      const bool isv = e >= p.d / 8;
-      const int x = 8 * (isv ? e - p.d / 8 : e);
+    const int n = p.d / PE;
+    for (int e = threadIdx.x; e < 2 * n; e += 256) {   // keys, then values
+      const bool isv = e >= n;
+      const int x = PE * (isv ? e - n : e);
       *(uint4*)((isv ? V + at_slot * p.vp : K + at_slot * p.kp) + x) = *(const uint4*)((isv ? vn : kn) + x);
     }
   }
@@ -288,7 +332,7 @@ __global__ __launch_bounds__(256, 2) void step_mfma_kernel(StepParams p, int chu
   float* so = (float*)lds;   // [4][HEADS][LDO]
   if (c < nh) {
 #pragma unroll
-    for (int x = 0; x < NV; ++x) *(float4*)&so[(wave * HEADS + c) * LDO + 16 * x + 4 * g] = make_float4(o[x][0], o[x][1], o[x][2], o[x][3]);
+    for (int x = 0; x < D / 16; ++x) *(float4*)&so[(wave * HEADS + c) * LDO + 16 * x + 4 * g] = make_float4(o[x][0], o[x][1], o[x][2], o[x][3]);
     if (g == 0) { s_m[wave][c] = m; s_l[wave][c] = l; }
   }
   __syncthreads();
@@ -296,59 +340,65 @@ __global__ __launch_bounds__(256, 2) void step_mfma_kernel(StepParams p, int chu
     const int hh = e / (D / 4), x = 4 * (e - hh * (D / 4));
     if (x >= p.d) continue;
     const float mm = fmaxf(fmaxf(s_m[0][hh], s_m[1][hh]), fmaxf(s_m[2][hh], s_m[3][hh]));
-    float ll = 0.f;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    float ll = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const float f = s_m[w][hh] == -INFINITY ? (s_l[w][hh] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f((s_m[w][hh] - mm) * cs);
       const float4 v = *(const float4*)&so[(w * HEADS + hh) * LDO + x];
       ll += f * s_l[w][hh];
-      a.x += f * v.x; a.y += f * v.y; a.z += f * v.z; a.w += f * v.w;
+      a[0] += f * v.x; a[1] += f * v.y; a[2] += f * v.z; a[3] += f * v.w;
     }
     if (p.splits == 1) {
       const float inv = ll == 0.f ? 0.f : 1.f / ll;
-      bf16_t* out = (bf16_t*)p.out + r * p.ldo + (int64_t)(h0 + hh) * p.d + x;
-      out[0] = f32_to_bf16(a.x * inv); out[1] = f32_to_bf16(a.y * inv); out[2] = f32_to_bf16(a.z * inv); out[3] = f32_to_bf16(a.w * inv);
+      T* out = (T*)p.out + r * p.ldo + (int64_t)(h0 + hh) * p.d + x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out[i] = Cvt<T>::from_f32(a[i] * inv);
     } else {
       float* part = p.part + (((int64_t)r * p.H + h0 + hh) * p.splits + split) * (p.d + 2);
-      part[x] = a.x; part[x + 1] = a.y; part[x + 2] = a.z; part[x + 3] = a.w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) part[x + i] = a[i];
       if (x == 0) { part[p.d] = mm * cs * (1.f / LOG2E); part[p.d + 1] = ll; }
     }
   }
 }
 
-// one block per (sequence, head): a thread adds one column over every second split
+// One block per (sequence, head), 512 threads: a thread adds one column over every fourth split.  The splits' maxima and
+// sums are loaded by all at once, the columns right behind them: two trips to memory.
 template <typename T>
-__global__ __launch_bounds__(256) void step_join_kernel(StepParams p) {
-  __shared__ float f[MAX_SPLITS], red[MAXD + 1];
+__global__ __launch_bounds__(512) void step_join_kernel(StepParams p) {
+  __shared__ float s_m[MAX_SPLITS], s_l[MAX_SPLITS], red[4][MAXD];
   const int64_t rh = blockIdx.x;
   const int r = (int)(rh / p.H), h = (int)(rh - (int64_t)r * p.H), lane = threadIdx.x & 63;
   const float* part = p.part + rh * p.splits * (p.d + 2);
-  float m = -INFINITY, l = 0.f;
-  for (int s = lane; s < p.splits; s += 64) m = fmaxf(m, part[(int64_t)s * (p.d + 2) + p.d]);
-  m = wave_max(m);
-  for (int s = threadIdx.x; s < p.splits; s += 256) {
-    const float ms = part[(int64_t)s * (p.d + 2) + p.d];
-    f[s] = ms == -INFINITY ? 0.f : expf(ms - m);
+  for (int s = threadIdx.x; s < p.splits; s += 512) {
+    s_m[s] = part[(int64_t)s * (p.d + 2) + p.d];
+    s_l[s] = part[(int64_t)s * (p.d + 2) + p.d + 1];
   }
   __syncthreads();
-  for (int s = lane; s < p.splits; s += 64) l += f[s] * part[(int64_t)s * (p.d + 2) + p.d + 1];
+  float m = -INFINITY, l = 0.f;   // every wave for itself
+  for (int s = lane; s < p.splits; s += 64) m = fmaxf(m, s_m[s]);
+  m = wave_max(m);
+  for (int s = lane; s < p.splits; s += 64) l += s_m[s] == -INFINITY ? 0.f : expf(s_m[s] - m) * s_l[s];
   l = wave_sum(l);
-  const int col = threadIdx.x & (MAXD - 1), half = threadIdx.x / MAXD;
+  const int col = threadIdx.x & (MAXD - 1), run = threadIdx.x / MAXD;
   float a = 0.f;
-  if (col < p.d)
-    for (int s = half; s < p.splits; s += 2) a += f[s] * part[(int64_t)s * (p.d + 2) + col];
-  if (half) red[col] = a;
+  if (col < p.d) {
+#pragma unroll 8
+    for (int s = run; s < p.splits; s += 4)
+      a += s_m[s] == -INFINITY ? 0.f : expf(s_m[s] - m) * part[(int64_t)s * (p.d + 2) + col];
+  }
+  red[run][col] = a;
   __syncthreads();
-  if (!half && col < p.d)
-    ((T*)p.out)[r * p.ldo + (int64_t)h * p.d + col] = Cvt<T>::from_f32(l == 0.f ? 0.f : (a + red[col]) / l);
+  if (run == 0 && col < p.d)
+    ((T*)p.out)[r * p.ldo + (int64_t)h * p.d + col] =
+        Cvt<T>::from_f32(l == 0.f ? 0.f : (red[0][col] + red[1][col] + red[2][col] + red[3][col]) / l);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // Splits: enough blocks to give every CU two, each with at least one pass of its four waves.
-void plan(StepParams& p, bool mfma) {
-  const int64_t most = std::min<int64_t>((int64_t)p.window + p.sinks, p.cap), pass = 4 * (mfma ? MT : KT);
+void plan(StepParams& p, bool mfma, int dtype) {
+  const int64_t most = std::min<int64_t>((int64_t)p.window + p.sinks, p.cap), pass = 4 * (!mfma ? KT : dtype == SK_BF16 ? 32 : 16);   // positions a block takes at a time
   const int64_t blocks = (int64_t)p.R * (mfma ? p.G * ((p.H / p.G + HEADS - 1) / HEADS) : p.H);
   const int64_t want = std::min<int64_t>(MAX_SPLITS, 2 * sk_num_cus() / std::max<int64_t>(1, blocks));
   const int64_t passes = (most + pass - 1) / pass, splits = std::max<int64_t>(1, std::min(want, passes));
@@ -365,11 +415,13 @@ extern "C" int64_t skhip_window_attn_step_ws_floats(int R, int n_head, int n_kv,
   StepParams p = {};
   p.R = R; p.H = n_head; p.G = n_kv; p.d = d; p.cap = cap; p.window = window; p.sinks = sinks;
   if (n_head % n_kv) return 0;
-  // the larger of the two paths' needs: which one a call takes depends on its pointers and strides
-  plan(p, false);
-  const int64_t plain = ws_floats(p);
-  plan(p, true);
-  return std::max(plain, ws_floats(p));
+  // the largest of the paths' needs: which one a call takes depends on its pointers and strides
+  plan(p, false, SK_F32);
+  int64_t n = ws_floats(p);
+  plan(p, true, SK_F32);
+  n = std::max(n, ws_floats(p));
+  plan(p, true, SK_BF16);
+  return std::max(n, ws_floats(p));
 }
 
 extern "C" int skhip_window_attn_step(const void* q, const void* k_new, const void* v_new, void* k_cache, void* v_cache,
@@ -399,22 +451,27 @@ extern "C" int skhip_window_attn_step(const void* q, const void* k_new, const vo
   const int per = dtype == SK_BF16 ? 8 : 4;
   const bool rows16 = d % per == 0 && strides % per == 0 && aligned16(q) && aligned16(k_cache) && aligned16(v_cache) &&
                       aligned16(k_new) && aligned16(v_new);
-  const bool mfma = dtype == SK_BF16 && rows16 && scale != 0.f && scale - scale == 0.f;
-  plan(p, mfma);
+  const bool mfma = rows16 && scale != 0.f && scale - scale == 0.f;
+  plan(p, mfma, dtype);
   if (ws_floats(p) > 0 && (!workspace || workspace_floats < ws_floats(p))) {
     sk_set_error("%s: workspace of %lld floats needed", who, (long long)ws_floats(p));
     return SK_ERR_WORKSPACE;
   }
   const int chunks = (n_head / n_kv + HEADS - 1) / HEADS;
   const dim3 grid(p.splits, mfma ? n_kv * chunks : n_head, R);
-  if (mfma && d <= 64) hipLaunchKernelGGL((step_mfma_kernel<64>), grid, dim3(256), 0, stream, p, chunks);
-  else if (mfma) hipLaunchKernelGGL((step_mfma_kernel<128>), grid, dim3(256), 0, stream, p, chunks);
-  else if (dtype == SK_BF16) hipLaunchKernelGGL((step_kernel<bf16_t>), grid, dim3(256), 0, stream, p, (int)rows16);
-  else hipLaunchKernelGGL((step_kernel<float>), grid, dim3(256), 0, stream, p, (int)rows16);
+  if (dtype == SK_BF16) {
+    if (mfma && d <= 64) hipLaunchKernelGGL((step_mfma_kernel<bf16_t, 64>), grid, dim3(256), 0, stream, p, chunks);
+    else if (mfma) hipLaunchKernelGGL((step_mfma_kernel<bf16_t, 128>), grid, dim3(256), 0, stream, p, chunks);
+    else hipLaunchKernelGGL((step_kernel<bf16_t>), grid, dim3(256), 0, stream, p, (int)rows16);
+  } else {
+    if (mfma && d <= 64) hipLaunchKernelGGL((step_mfma_kernel<float, 64>), grid, dim3(256), 0, stream, p, chunks);
+    else if (mfma) hipLaunchKernelGGL((step_mfma_kernel<float, 128>), grid, dim3(256), 0, stream, p, chunks);
+    else hipLaunchKernelGGL((step_kernel<float>), grid, dim3(256), 0, stream, p, (int)rows16);
+  }
   if (p.splits > 1) {
     const dim3 join((unsigned)(R * n_head));
-    if (dtype == SK_BF16) hipLaunchKernelGGL((step_join_kernel<bf16_t>), join, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((step_join_kernel<float>), join, dim3(256), 0, stream, p);
+    if (dtype == SK_BF16) hipLaunchKernelGGL((step_join_kernel<bf16_t>), join, dim3(512), 0, stream, p);
+    else hipLaunchKernelGGL((step_join_kernel<float>), join, dim3(512), 0, stream, p);
   }
   SK_CHECK_LAUNCH(who);
   return SK_OK;
