@@ -434,6 +434,13 @@ void plan_sinks(WinParams& p, int rows) {
   p.nch = far ? (p.Lq + p.ch - 1) / p.ch : 0;
 }
 
+// Grids of 256 threads a block whose threads are counted in 32 bits (tiles of 64 rows: the most that any kernel has).
+bool grids_fit(const WinParams& p) {
+  const int64_t tiles = std::max(p.Lq, p.Lk) / 64 + 1, units = (int64_t)p.B * p.G + 7;
+  return units * tiles * (p.H / p.G) + TAIL * p.H < (1 << 24) && units * (tiles + (int64_t)p.nst * p.nch) + TAIL * p.G < (1 << 24) &&
+         (p.nst == 0 || (int64_t)p.sinks * p.d < (1ll << 31));
+}
+
 int64_t slab_floats(const WinParams& p, int rows) {
   return (int64_t)p.B * p.G * p.nst * (1 + p.nch) * 2 * slab_rows(p, rows) * p.d;
 }
@@ -490,6 +497,7 @@ extern "C" int skhip_window_attn_fwd(const void* Q, const void* K, const void* V
   if (Tq == 0) return SK_OK;
   SK_CHECK_ARG(Q && O && LSE && (Tk == 0 || (K && V)), "%s: null pointer", who);
   set_window(p, window, causal);
+  SK_CHECK_ARG(grids_fit(p), "%s: more than 2^24 tiles of 64 rows", who);
   if (sk_window_mfma_supported(p, dtype)) return sk_window_fwd_mfma(p, stream);
   p.vec = whole_pieces(p, dtype);
   if (dtype == SK_BF16) {
@@ -526,6 +534,7 @@ extern "C" int skhip_window_attn_bwd(const void* Q, const void* K, const void* V
   plan_sinks(p, MFMA_ROWS);
   const bool mfma = sk_window_mfma_supported(p, dtype);
   if (!mfma) plan_sinks(p, NT);
+  SK_CHECK_ARG(grids_fit(p), "%s: more than 2^24 tiles of 64 rows", who);
   const int64_t head = (mfma ? 2 : 1) * (int64_t)n_head * Tq, need = (head + 3) / 4 * 4 + slab_floats(p, mfma ? MFMA_ROWS : NT);
   if (need > 0 && (!workspace || workspace_floats < need)) {
     sk_set_error("%s: workspace of %lld floats needed", who, (long long)need);

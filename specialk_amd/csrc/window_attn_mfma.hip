@@ -527,18 +527,17 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
 
-// Heads whose rows are whole 16-byte pieces; 32-bit offsets within a tile of 64 rows; a scale that the maximum of the
-// unscaled scores can stand for; item numbers that fit 31 bits.
+// Heads whose rows are whole 16-byte pieces; 32-bit offsets within a tile of 64 rows; a finite scale that is not zero or next
+// to it: the maximum of the unscaled scores stands for that of the scaled ones, and the backward pass divides by it.
 bool sk_window_mfma_supported(const WinParams& p, int dtype) {
-  if (dtype != SK_BF16 || p.d % 8 || p.d > 128 || p.scale == 0.f || !(p.scale - p.scale == 0.f)) return false;
+  if (dtype != SK_BF16 || p.d % 8 || p.d > 128 || !(fabsf(p.scale) >= 1e-30f) || !(p.scale - p.scale == 0.f)) return false;
   const int64_t lds[] = {p.ldq, p.ldk, p.ldv, p.ldo, p.lddo, p.lddq, p.lddk, p.lddv};
   for (int64_t ld : lds)
     if (ld % 8 || ld > (1 << 23)) return false;
   const void* ptr[] = {p.Q, p.K, p.V, p.O, p.dO, p.Oout, p.dQ, p.dK, p.dV};
   for (const void* x : ptr)
     if (!aligned16(x)) return false;
-  const int64_t tiles = (int64_t)(std::max(p.Lq, p.Lk) / OWN + 1) + (int64_t)p.nst * p.nch;
-  return tiles * p.H * (p.B + 8) < (1ll << 30);
+  return true;
 }
 
 int sk_window_fwd_mfma(const WinParams& p, hipStream_t stream) {

@@ -123,7 +123,7 @@ __global__ __launch_bounds__(256) void step_kernel(StepParams p, int vec) {
   float f[4], ll = 0.f;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    f[w] = s_m[w] == -INFINITY ? 0.f : expf(s_m[w] - mm);
+    f[w] = s_m[w] == -INFINITY ? (s_l[w] == 0.f ? 0.f : 1.f) : expf(s_m[w] - mm);   // (a sum of NaN scores has no maximum)
     ll += f[w] * s_l[w];
   }
   float* part = p.part + (((int64_t)r * p.H + h) * p.splits + split) * (p.d + 2);
@@ -378,7 +378,7 @@ __global__ __launch_bounds__(512) void step_join_kernel(StepParams p) {
   float m = -INFINITY, l = 0.f;   // every wave for itself
   for (int s = lane; s < p.splits; s += 64) m = fmaxf(m, s_m[s]);
   m = wave_max(m);
-  for (int s = lane; s < p.splits; s += 64) l += s_m[s] == -INFINITY ? 0.f : expf(s_m[s] - m) * s_l[s];
+  for (int s = lane; s < p.splits; s += 64) l += s_m[s] == -INFINITY ? s_l[s] : expf(s_m[s] - m) * s_l[s];   // (0 or NaN)
   l = wave_sum(l);
   const int col = threadIdx.x & (MAXD - 1), run = threadIdx.x / MAXD;
   float a = 0.f;
@@ -451,7 +451,8 @@ extern "C" int skhip_window_attn_step(const void* q, const void* k_new, const vo
   const int per = dtype == SK_BF16 ? 8 : 4;
   const bool rows16 = d % per == 0 && strides % per == 0 && aligned16(q) && aligned16(k_cache) && aligned16(v_cache) &&
                       aligned16(k_new) && aligned16(v_new);
-  const bool mfma = rows16 && scale != 0.f && scale - scale == 0.f;
+  // (the matrix cores take maxima of unscaled scores, which a scale of 0 or inf cannot stand for)
+  const bool mfma = rows16 && fabsf(scale) >= 1e-30f && scale - scale == 0.f;
   plan(p, mfma, dtype);
   if (ws_floats(p) > 0 && (!workspace || workspace_floats < ws_floats(p))) {
     sk_set_error("%s: workspace of %lld floats needed", who, (long long)ws_floats(p));

@@ -987,8 +987,8 @@ class RotaryFrequencies:
             raise ValueError(f"base and factor must be positive, got {base} and {factor}")
         if scaling == "ntk" and rot_dim <= 2:
             raise ValueError('"ntk" needs more than one pair')
-        if scaling == "yarn" and trained_len <= 0:
-            raise ValueError('"yarn" needs trained_len')
+        if scaling == "yarn" and (trained_len <= 0 or factor < 1):
+            raise ValueError('"yarn" needs trained_len and a factor of at least 1')
         if scaling == "ntk":
             base = base * factor ** (rot_dim / (rot_dim - 2))
         radians = [base ** (-2.0 * i / rot_dim) for i in range(rot_dim // 2)]
@@ -1145,20 +1145,21 @@ class WindowAttnFn(torch.autograd.Function):
     """softmax(scale q k^T on the visible pairs) v over packed or padded rows with shared key heads."""
 
     @staticmethod
-    def forward(ctx, q, k, v, cfg):
+    def forward(ctx, q, k, v, key_pad, q_off, k_off, cfg):
         with L.on_device(q):
-            o, lse = L.window_attn_fwd(q, k, v, **cfg)
-        ctx.save_for_backward(q, k, v, o, lse)
+            o, lse = L.window_attn_fwd(q, k, v, key_pad=key_pad, q_off=q_off, k_off=k_off, **cfg)
+        ctx.save_for_backward(q, k, v, key_pad, q_off, k_off, o, lse)
         ctx.cfg = cfg
         return o
 
     @staticmethod
     def backward(ctx, do):
         _once()
-        q, k, v, o, lse = ctx.saved_tensors
+        q, k, v, key_pad, q_off, k_off, o, lse = ctx.saved_tensors
         with L.on_device(q):
-            dq, dk, dv = L.window_attn_bwd(q, k, v, o, _rows(do, o.shape[1], "do"), lse, **ctx.cfg)
-        return dq, dk, dv, None
+            dq, dk, dv = L.window_attn_bwd(q, k, v, o, _rows(do, o.shape[1], "do"), lse, key_pad=key_pad, q_off=q_off,
+                                           k_off=k_off, **ctx.cfg)
+        return dq, dk, dv, None, None, None, None
 
 
 def _window(window):
@@ -1196,6 +1197,7 @@ def window_attention(q, k, v, B, Lq, Lk, n_head, n_kv_head=None, window=None, si
         for o in (q_off, k_off):
             if o.dtype != torch.int32 or o.shape != (B + 1,) or not o.is_contiguous():
                 raise ValueError(f"row offsets must be contiguous int32 ({B + 1},), got {o.dtype} {tuple(o.shape)}")
+        Lq, Lk = min(Lq, q.shape[0]), min(Lk, k.shape[0])
     elif q.shape[0] != B * Lq or k.shape[0] != B * Lk:
         raise ValueError(f"{q.shape[0]} query and {k.shape[0]} key rows are not {B} x {Lq} and {B} x {Lk}")
     if key_pad is not None:
@@ -1204,9 +1206,8 @@ def window_attention(q, k, v, B, Lq, Lk, n_head, n_kv_head=None, window=None, si
         key_pad = key_pad.contiguous().view(torch.uint8)
     _same(q, k, v, key_pad, q_off, k_off)
     cfg = dict(B=B, Lq=Lq, Lk=Lk, n_head=n_head, n_kv=n_kv, d=d, scale=d ** -0.5 if scale is None else float(scale),
-               window=_window(window), sinks=min(int(sinks), NO_WINDOW), causal=bool(causal), key_pad=key_pad, q_off=q_off,
-               k_off=k_off)
-    return _run(WindowAttnFn, q, k, v, cfg)
+               window=_window(window), sinks=min(int(sinks), NO_WINDOW), causal=bool(causal))
+    return _run(WindowAttnFn, q, k, v, key_pad, q_off, k_off, cfg)
 
 
 def window_attention_step(q, k_new, v_new, k_cache, v_cache, kv_len, n_head, n_kv_head=None, window=None, sinks=0,
@@ -1246,6 +1247,8 @@ def window_attention_step(q, k_new, v_new, k_cache, v_cache, kv_len, n_head, n_k
         raise ValueError(f"q is {q.dtype}, the caches {k_cache.dtype} and {v_cache.dtype}")
     if kv_len.dtype != torch.int32 or kv_len.shape != (R,) or not kv_len.is_contiguous():
         raise ValueError(f"kv_len must be contiguous int32 ({R},), got {kv_len.dtype} {tuple(kv_len.shape)}")
+    if cap > 1 << 30:
+        raise ValueError(f"a cache of {cap} slots is longer than 2^30")
     window = cap - sinks if window is None else _window(window)
     if sinks < 0 or window < 1 or cap - sinks < window:
         raise ValueError(f"a cache of {cap} slots cannot hold {sinks} sinks and a window of {window}")

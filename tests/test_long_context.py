@@ -39,7 +39,8 @@ def test_scaling_keeps_and_stretches_the_right_ends(scaling):
 
 @pytest.mark.parametrize("kw", [dict(rot_dim=3), dict(rot_dim=-2), dict(rot_dim=8, base=0.0), dict(rot_dim=8, factor=-1.0),
                                 dict(rot_dim=8, base=float("nan")), dict(rot_dim=8, scaling="other"),
-                                dict(rot_dim=2, scaling="ntk", factor=2.0), dict(rot_dim=8, scaling="yarn", factor=2.0)])
+                                dict(rot_dim=2, scaling="ntk", factor=2.0), dict(rot_dim=8, scaling="yarn", factor=2.0),
+                                dict(rot_dim=8, scaling="yarn", factor=0.5, trained_len=64)])
 def test_frequency_refusals(kw):
     with pytest.raises(ValueError):
         ops.RotaryFrequencies(device="cpu", **kw)
@@ -164,7 +165,8 @@ def test_entry_points_refuse_before_any_launch():
                                          sinks, 1, 0, None)
 
     for kw in (dict(G=3), dict(d=129, ldq=1000, ldk=1000), dict(window=0), dict(sinks=-1), dict(ldq=63), dict(ldk=31), dict(Tq=11),
-               dict(qo=p), dict(qo=p, ko=p, pad=p), dict(lse=None), dict(B=65535, Lq=0, Tq=0)):
+               dict(qo=p), dict(qo=p, ko=p, pad=p), dict(lse=None), dict(B=65535, Lq=0, Tq=0),
+               dict(qo=p, ko=p, B=65000, Lq=1 << 20)):
         assert fwd(**kw) == -1, kw
         assert b"skhip_window_attn_fwd" in lib.skhip_last_error()
 

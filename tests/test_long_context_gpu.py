@@ -223,13 +223,13 @@ def attention64(q, k, v, do, vis, scale, dtype):
     dq, dk, dv = ds @ k, ds.t() @ q, p.t() @ do
     ub = unit(dtype) if dtype == BF else 0.0                   # operands of the matrix products
     u = unit(dtype)
-    smax = (q.abs() @ k.abs().t() * scale * vis).max()
+    smax = (q.abs() @ k.abs().t() * abs(scale) * vis).max()
     rel = (2 * (d + 6) * smax + 2 * n + 16) * E                # of a probability: score, exponential, row sum
     a = p @ v.abs()
     eo = u * o.abs() + a * (ub + rel)
     edelta = (do.abs() * eo).sum(1, keepdim=True) + (d + 2) * E * (do.abs() * o.abs()).sum(1, keepdim=True)
     edp = (d + 2) * E * (do.abs() @ v.abs().t())
-    eds = ds.abs() * (ub + rel + 4 * E) + p * scale * (edelta + edp)
+    eds = ds.abs() * (ub + rel + 4 * E) + p * abs(scale) * (edelta + edp)
     acc = (max(vis.shape) + 8) * E
     return ((o, eo), (dq, u * dq.abs() + eds @ k.abs() + acc * ds.abs() @ k.abs()),
             (dk, u * dk.abs() + eds.t() @ q.abs() + acc * ds.abs().t() @ q.abs()),
@@ -520,8 +520,6 @@ def test_step_offsets_beyond_32_bits():
         pytest.skip("needs 48 GiB of free memory")
     g = torch.Generator().manual_seed(9)
     cache = torch.zeros((R, cap, G * d), dtype=BF, device=DEV)
-    v_small = torch.zeros((R, cap, 1), dtype=BF, device=DEV)
-    del v_small
     n = torch.tensor([cap, 1, cap - 5], dtype=torch.int32, device=DEV)
     rowk = rnd((300, G * d), BF, g).to(DEV)
     cache[2, cap - 5 - 300:cap - 5] = rowk
@@ -633,3 +631,128 @@ def test_other_stream_and_captured_graph():
         want = work()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), seed
+
+
+def test_two_graphs_share_a_pool():
+    """Two graphs whose workspaces are the same memory, replayed in turn on new inputs: nothing is carried between calls."""
+    g = torch.Generator().manual_seed(15)
+    H, G, d, sinks, cap = 4, 2, 64, 3, 5000
+    do = rnd((400, H * d), BF, g).to(DEV)
+    x = rnd((400, (H + 2 * G) * d), BF, g).to(DEV)
+    kc, vc = rnd((1, cap, G * d), BF, g).to(DEV), rnd((1, cap, G * d), BF, g).to(DEV)
+    length = torch.tensor([4500], dtype=torch.int32, device=DEV)
+
+    def work(n, window):
+        leaf = x[:n].detach().requires_grad_()
+        q, k, v = leaf[:, :H * d], leaf[:, H * d:(H + G) * d], leaf[:, (H + G) * d:]
+        o = ops.window_attention(q, k, v, 1, n, n, H, G, window, sinks)
+        grad, = torch.autograd.grad(o, leaf, do[:n])
+        return o.detach(), grad, ops.window_attention_step(x[:1, :H * d], None, None, kc, vc, length, H, G, 100 * window, sinks)
+
+    cases, graphs = ((400, 30), (150, 40)), []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for c in cases:
+            work(*c)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    pool = torch.cuda.graph_pool_handle()
+    for c in cases:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            out = work(*c)
+        graphs.append((graph, out))
+    for seed in range(3):
+        x.copy_(rnd(x.shape, BF, torch.Generator().manual_seed(200 + seed)))
+        for (graph, out), c in zip(graphs, cases):
+            graph.replay()
+            torch.cuda.synchronize()
+            got = [t.clone() for t in out]
+            want = work(*c)
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), (seed, c)
+
+
+# ------------------------------------------------------------------------------ odd calls
+def test_no_second_derivative():
+    f = ops.RotaryFrequencies(8, device=DEV)
+    x = torch.randn(6, 32, device=DEV, requires_grad=True)
+    gamma = torch.ones(16, device=DEV)
+    pos = torch.arange(6, device=DEV)
+    for y in (ops.rotary(x, None, pos, f, 2)[0], ops.qk_norm_rotary(x, None, gamma, None, pos, f, 2)[0],
+              ops.window_attention(x, x, x, 1, 6, 6, 2)):
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+def test_masks_may_not_change_before_the_backward_pass():
+    x = torch.randn(6, 32, device=DEV, requires_grad=True)
+    pad = torch.zeros((1, 6), dtype=torch.uint8, device=DEV)
+    off = torch.tensor([0, 6], dtype=torch.int32, device=DEV)
+    for y, t in ((ops.window_attention(x, x, x, 1, 6, 6, 2, key_pad=pad), pad),
+                 (ops.window_attention(x, x, x, 1, 6, 6, 2, q_off=off, k_off=off.clone()), off)):
+        t.add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y.sum(), x)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("d", [64, 37])
+def test_window_lengths_given_as_any_upper_bound(d, dtype):
+    """Packed rows: longest lengths far beyond the rows (and 32 bits) change nothing."""
+    g = torch.Generator().manual_seed(16)
+    q, k, v, do = (rnd((90, 2 * d), dtype, g).to(DEV) for _ in range(4))
+    off = torch.tensor([0, 70, 70, 85], dtype=torch.int32, device=DEV)
+    res = []
+    for L in (70, 1 << 33):
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        o = ops.window_attention(*leaves, 3, L, L, 2, None, 20, 2, q_off=off, k_off=off)
+        res.append((o,) + torch.autograd.grad(o, leaves, do))
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("d", [64, 37])
+def test_nan_query_stays_in_its_row(d, dtype):
+    """A query with a NaN gives a row of NaN, and every other row what it gives without it."""
+    g = torch.Generator().manual_seed(17)
+    n, H = 200, 2
+    q, k, v = (rnd((n, H * d), dtype, g).to(DEV) for _ in range(3))
+    want = ops.window_attention(q, k, v, 1, n, n, H, None, 40, 2)
+    bad = q.clone()
+    bad[77, d + 3] = float("nan")
+    got = ops.window_attention(bad, k, v, 1, n, n, H, None, 40, 2)
+    assert got[77, d:].isnan().all()
+    got[77, d:] = want[77, d:]
+    assert torch.equal(got, want)
+    # one step, one split and several, with positions in one split only and in all
+    for cap, lens in ((64, [1, 60, 64]), (6000, [1, 50, 5000])):
+        kc, vc = rnd((3, cap, H * d), dtype, g).to(DEV), rnd((3, cap, H * d), dtype, g).to(DEV)
+        for r in range(3):
+            length = torch.tensor(lens, dtype=torch.int32, device=DEV)
+            want = ops.window_attention_step(q[:3], None, None, kc, vc, length, H)
+            bad = q[:3].clone()
+            bad[r, 5] = float("nan")
+            got = ops.window_attention_step(bad, None, None, kc, vc, length, H)
+            assert got[r, :d].isnan().all(), (cap, r)
+            got[r, :d] = want[r, :d]
+            assert torch.equal(got, want), (cap, r)
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-35, -0.2])
+def test_window_scales(scale):
+    """A scale of nothing and next to it (every visible key counts alike), and a negative one."""
+    run_window([90], [90], 2, 1, 64, 20, 2, True, BF, "dense", scale=scale)
+
+
+def test_step_scale_of_nothing():
+    g = torch.Generator().manual_seed(18)
+    kc, vc = rnd((1, 600, 64), BF, g).to(DEV), rnd((1, 600, 64), BF, g).to(DEV)
+    length = torch.tensor([600], dtype=torch.int32, device=DEV)
+    for scale in (0.0, 1e-35):
+        o = ops.window_attention_step(kc[0, :1] * 3, None, None, kc, vc, length, 1, scale=scale)
+        want = vc[0].double().mean(0)
+        # the mean of 600 values in fp32 (n E of their mean size), rounded once
+        bound = want.abs() * unit(BF) + 700 * E * vc[0].double().abs().mean(0)
+        check(o[0], want, bound, scale)
