@@ -408,14 +408,14 @@ def _step_ws(*sizes):
 def window_attn_step(q, k_new, v_new, k_cache, v_cache, kv_len, n_head, n_kv, d, scale, window, sinks):
     """o (R, n_head * d); k_new / v_new (R, n_kv * d; one row stride) or None; caches (R, cap, n_kv * d), written in place."""
     lib = load()
-    R, cap = k_cache.shape[:2]
+    R, cap, _ = k_cache.shape
     o = q.new_empty((R, n_head * d))
     n = _step_ws(R, n_head, n_kv, d, cap, window, sinks)
     ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
     rc = lib.skhip_window_attn_step(_ptr(q), _ptr(k_new), _ptr(v_new), _ptr(k_cache), _ptr(v_cache), _ptr(o), _ptr(kv_len), R,
                                     n_head, n_kv, d, cap, q.stride(0), 0 if k_new is None else k_new.stride(0), n_head * d,
-                                    k_cache.stride(0), k_cache.stride(1), v_cache.stride(0), v_cache.stride(1), float(scale),
-                                    window, sinks, _ptr(ws), n, dcode(q.dtype), _stream())
+                                    *k_cache.stride()[:2], *v_cache.stride()[:2], float(scale), window, sinks, _ptr(ws), n,
+                                    dcode(q.dtype), _stream())
     _check(rc, "skhip_window_attn_step")
     return o
 

@@ -1006,17 +1006,20 @@ class RotaryFrequencies:
 
 def _rows(x, width, what):
     """x as rows (T, width) that kernels can address: unit inner stride, no overlapping rows."""
-    if x.dim() != 2 or x.shape[1] != width:
-        raise ValueError(f"{what} must be (rows, {width}), got {tuple(x.shape)}")
-    return x if x.stride(1) == 1 and x.stride(0) >= width else x.contiguous()
+    shape = x.shape
+    if len(shape) != 2 or shape[1] != width:
+        raise ValueError(f"{what} must be (rows, {width}), got {tuple(shape)}")
+    row, col = x.stride()
+    return x if col == 1 and row >= width else x.contiguous()
 
 
 def _heads(x, n_head, n_kv_head, most):
     if n_head <= 0 or n_kv_head <= 0 or n_head % n_kv_head:
         raise ValueError(f"{n_head} query heads cannot share {n_kv_head} key heads evenly")
-    if x.dim() != 2 or x.shape[1] % n_head or not 0 < x.shape[1] // n_head <= most:
-        raise ValueError(f"q must be (rows, {n_head} heads of 1..{most} elements), got {tuple(x.shape)}")
-    return x.shape[1] // n_head
+    shape = x.shape
+    if len(shape) != 2 or shape[1] % n_head or not 0 < shape[1] // n_head <= most:
+        raise ValueError(f"q must be (rows, {n_head} heads of 1..{most} elements), got {tuple(shape)}")
+    return shape[1] // n_head
 
 
 def _same(first, *tensors):
@@ -1026,13 +1029,13 @@ def _same(first, *tensors):
             raise ValueError(f"tensors on {dev} and {t.device}")
 
 
-def _run(fn, *args):
-    """call(fn, *args), without the tape where no tensor among the arguments asks for it."""
+def _run(fn, leaves, *rest):
+    """fn of the tensors `leaves` that may want gradients and of the rest, without the tape where none does."""
     if torch.is_grad_enabled():
-        for a in args:
-            if isinstance(a, torch.Tensor) and a.requires_grad:
-                return fn.apply(*args)
-    return fn.forward(_InferCtx(), *args)
+        for a in leaves:
+            if a is not None and a.requires_grad:
+                return fn.apply(*leaves, *rest)
+    return fn.forward(_InferCtx(), *leaves, *rest)
 
 
 def _once():
@@ -1094,17 +1097,17 @@ def _rotary_args(q, k, pos, freqs, n_head, n_kv_head):
     q = _rows(q, n_head * d, "q")
     if k is not None:
         k = _rows(k, n_kv * d, "k")
-        if k.shape[0] != q.shape[0] or k.dtype != q.dtype:
+        if k.shape[0] != q.shape[0] or k.dtype is not q.dtype:
             raise ValueError(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} do not go together")
     L.dcode(q.dtype)
     if freqs is None:
         return q, k, None, n_kv
     if freqs.rot_dim > d:
         raise ValueError(f"{freqs.rot_dim} rotated elements in a head of {d}")
-    if pos is None or pos.dtype != torch.int64 or pos.numel() != q.shape[0]:
+    if pos is None or pos.dtype is not torch.int64 or pos.numel() != q.shape[0]:
         raise ValueError(f"pos must hold one int64 position for each of the {q.shape[0]} rows")
     _same(q, k, pos, freqs.turns)
-    return q, k, pos.reshape(-1).contiguous(), n_kv
+    return q, k, pos if pos.dim() == 1 and pos.is_contiguous() else pos.reshape(-1).contiguous(), n_kv
 
 
 def rotary(q, k, pos, freqs, n_head, n_kv_head=None, interleaved=False):
@@ -1116,7 +1119,7 @@ def rotary(q, k, pos, freqs, n_head, n_kv_head=None, interleaved=False):
     if freqs is None:
         raise ValueError("rotary needs a RotaryFrequencies")
     q, k, pos, n_kv = _rotary_args(q, k, pos, freqs, n_head, n_kv_head)
-    return _run(QKRotaryFn, q, k, pos, freqs, n_head, n_kv, bool(interleaved))
+    return _run(QKRotaryFn, (q, k), pos, freqs, n_head, n_kv, bool(interleaved))
 
 
 def qk_norm_rotary(q, k, gamma_q, gamma_k, pos, freqs, n_head, n_kv_head=None, eps=1e-6, interleaved=False):
@@ -1129,12 +1132,12 @@ def qk_norm_rotary(q, k, gamma_q, gamma_k, pos, freqs, n_head, n_kv_head=None, e
     if (k is None) != (gamma_k is None):
         raise ValueError("k and gamma_k go together")
     for g in (gamma_q, gamma_k):
-        if g is not None and (g.dtype != torch.float32 or g.shape != (d,) or not g.is_contiguous()):
+        if g is not None and (g.dtype is not torch.float32 or g.shape != (d,) or not g.is_contiguous()):
             raise ValueError(f"a norm weight must be a contiguous fp32 vector of {d}, got {g.dtype} {tuple(g.shape)}")
     if not eps >= 0:
         raise ValueError(f"eps {eps} is negative")
     _same(q, k, gamma_q, gamma_k)
-    return _run(QKNormRotaryFn, q, k, gamma_q, gamma_k, pos, freqs, n_head, n_kv, float(eps), bool(interleaved))
+    return _run(QKNormRotaryFn, (q, k, gamma_q, gamma_k), pos, freqs, n_head, n_kv, float(eps), bool(interleaved))
 
 
 # ----------------------------------------------------------------------------- attention within a window
@@ -1207,7 +1210,7 @@ def window_attention(q, k, v, B, Lq, Lk, n_head, n_kv_head=None, window=None, si
     _same(q, k, v, key_pad, q_off, k_off)
     cfg = dict(B=B, Lq=Lq, Lk=Lk, n_head=n_head, n_kv=n_kv, d=d, scale=d ** -0.5 if scale is None else float(scale),
                window=_window(window), sinks=min(int(sinks), NO_WINDOW), causal=bool(causal))
-    return _run(WindowAttnFn, q, k, v, key_pad, q_off, k_off, cfg)
+    return _run(WindowAttnFn, (q, k, v), key_pad, q_off, k_off, cfg)
 
 
 def window_attention_step(q, k_new, v_new, k_cache, v_cache, kv_len, n_head, n_kv_head=None, window=None, sinks=0,
@@ -1224,13 +1227,14 @@ def window_attention_step(q, k_new, v_new, k_cache, v_cache, kv_len, n_head, n_k
     n_kv = n_head if n_kv_head is None else n_kv_head
     d = _heads(q, n_head, n_kv, 128)
     q = _rows(q, n_head * d, "q")
-    R, w = q.shape[0], n_kv * d
-    L.dcode(q.dtype)
+    R, w, dt = q.shape[0], n_kv * d, q.dtype
+    L.dcode(dt)
     if (k_new is None) != (v_new is None):
         raise ValueError("k_new and v_new go together")
-    if k_cache.dim() != 3 or k_cache.shape[0] != R or k_cache.shape[2] != w or v_cache.shape != k_cache.shape:
-        raise ValueError(f"caches must be ({R}, cap, {w}), got {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
-    cap = k_cache.shape[1]
+    shape = k_cache.shape
+    if len(shape) != 3 or shape[0] != R or shape[2] != w or v_cache.shape != shape:
+        raise ValueError(f"caches must be ({R}, cap, {w}), got {tuple(shape)} and {tuple(v_cache.shape)}")
+    cap = shape[1]
     for c in (k_cache, v_cache):
         s0, s1, s2 = c.stride()   # sequence by sequence, or position by position
         if s2 != 1 or s1 < w or s0 < 0 or (R > 1 and s0 < (cap - 1) * s1 + w and (s0 < w or s1 < (R - 1) * s0 + w)):
@@ -1241,11 +1245,11 @@ def window_attention_step(q, k_new, v_new, k_cache, v_cache, kv_len, n_head, n_k
             k_new, v_new = k_new.contiguous(), v_new.contiguous()
         if k_new.shape[0] != R or v_new.shape[0] != R:
             raise ValueError(f"k_new and v_new must have {R} rows")
-        if k_new.dtype != q.dtype or v_new.dtype != q.dtype:
-            raise ValueError(f"q is {q.dtype}, k_new and v_new {k_new.dtype} and {v_new.dtype}")
-    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
-        raise ValueError(f"q is {q.dtype}, the caches {k_cache.dtype} and {v_cache.dtype}")
-    if kv_len.dtype != torch.int32 or kv_len.shape != (R,) or not kv_len.is_contiguous():
+        if k_new.dtype is not dt or v_new.dtype is not dt:
+            raise ValueError(f"q is {dt}, k_new and v_new {k_new.dtype} and {v_new.dtype}")
+    if k_cache.dtype is not dt or v_cache.dtype is not dt:
+        raise ValueError(f"q is {dt}, the caches {k_cache.dtype} and {v_cache.dtype}")
+    if kv_len.dtype is not torch.int32 or kv_len.shape != (R,) or not kv_len.is_contiguous():
         raise ValueError(f"kv_len must be contiguous int32 ({R},), got {kv_len.dtype} {tuple(kv_len.shape)}")
     if cap > 1 << 30:
         raise ValueError(f"a cache of {cap} slots is longer than 2^30")
