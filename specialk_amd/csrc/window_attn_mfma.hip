@@ -40,8 +40,13 @@ __device__ __forceinline__ f32x16_t zero16() {
   return z;
 }
 
-// byte address of 16-byte chunk `chunk` of row `row` within a tile of D columns
-template <int D> __device__ __forceinline__ int at(int row, int chunk) { return row * (2 * D) + ((chunk ^ (row & 7)) << 4); }
+// Byte address of 16-byte chunk `chunk` of row `row` within a tile of D columns.  The banks' 256 bytes hold one row of 128
+// columns or two of 64; the exchange sends the same chunk of 16 rows (reads by rows) to 16 different places, and four
+// neighbouring chunks of 4 rows (reads by columns) too.
+template <int D> __device__ __forceinline__ int mix(int row) {
+  return D == 64 ? ((row & 2) << 1) | ((row & 4) >> 1) | ((row & 8) >> 3) : ((row & 3) << 2) | ((row & 12) >> 2);
+}
+template <int D> __device__ __forceinline__ int at(int row, int chunk) { return row * (2 * D) + ((chunk ^ mix<D>(row)) << 4); }
 template <int D> constexpr int tile_bytes() { return NT * 2 * D; }
 
 // rows row0 .. row0+31 as the X operand, columns 16 s + 8 h ..
@@ -66,7 +71,7 @@ __device__ __forceinline__ void load_tile(char* t, const bf16_t* base, int64_t l
   const uint32_t ldb = (uint32_t)ld * 2;
 #pragma unroll
   for (int j = 0; j < NT / ROWS / 4; ++j) {
-    const int idx = wave * (NT / ROWS / 4) + j, row = idx * ROWS + lane / CH, chunk = (lane % CH) ^ (row & 7);
+    const int idx = wave * (NT / ROWS / 4) + j, row = idx * ROWS + lane / CH, chunk = (lane % CH) ^ mix<D>(row);
     const bool use = ((ok >> row) & 1) && chunk * 8 < d;
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(t + idx * 1024), 16, use ? row * ldb + chunk * 16 : NOWHERE, 0, 0, 0);
   }
