@@ -362,14 +362,22 @@ __global__ __launch_bounds__(256, 2) void step_mfma_kernel(StepParams p, int chu
   }
 }
 
-// One block per (sequence, head), 512 threads: a thread adds one column over every fourth split.  The splits' maxima and
-// sums are loaded by all at once, the columns right behind them: two trips to memory.
+// One block per (sequence, head), 512 threads: a thread adds one column over every fourth split.  The columns of the first
+// 64 splits are on their way with the splits' maxima and sums: one trip to memory for most launches.
 template <typename T>
 __global__ __launch_bounds__(512) void step_join_kernel(StepParams p) {
   __shared__ float s_m[MAX_SPLITS], s_l[MAX_SPLITS], red[4][MAXD];
   const int64_t rh = blockIdx.x;
   const int r = (int)(rh / p.H), h = (int)(rh - (int64_t)r * p.H), lane = threadIdx.x & 63;
   const float* part = p.part + rh * p.splits * (p.d + 2);
+  const int col = threadIdx.x & (MAXD - 1), run = threadIdx.x / MAXD;
+  constexpr int FIRST = 16;
+  float v[FIRST];
+#pragma unroll
+  for (int i = 0; i < FIRST; ++i) {
+    const int s = run + 4 * i;
+    v[i] = col < p.d && s < p.splits ? part[(int64_t)s * (p.d + 2) + col] : 0.f;
+  }
   for (int s = threadIdx.x; s < p.splits; s += 512) {
     s_m[s] = part[(int64_t)s * (p.d + 2) + p.d];
     s_l[s] = part[(int64_t)s * (p.d + 2) + p.d + 1];
@@ -380,11 +388,15 @@ __global__ __launch_bounds__(512) void step_join_kernel(StepParams p) {
   m = wave_max(m);
   for (int s = lane; s < p.splits; s += 64) l += s_m[s] == -INFINITY ? s_l[s] : expf(s_m[s] - m) * s_l[s];   // (0 or NaN)
   l = wave_sum(l);
-  const int col = threadIdx.x & (MAXD - 1), run = threadIdx.x / MAXD;
   float a = 0.f;
+#pragma unroll
+  for (int i = 0; i < FIRST; ++i) {
+    const int s = run + 4 * i;
+    if (s < p.splits && s_m[s] != -INFINITY) a += expf(s_m[s] - m) * v[i];
+  }
   if (col < p.d) {
 #pragma unroll 8
-    for (int s = run; s < p.splits; s += 4)
+    for (int s = run + 4 * FIRST; s < p.splits; s += 4)
       a += s_m[s] == -INFINITY ? 0.f : expf(s_m[s] - m) * part[(int64_t)s * (p.d + 2) + col];
   }
   red[run][col] = a;
