@@ -30,6 +30,10 @@ struct WinParams {
   // sinks would sweep the whole sequence alone.  Their far queries are cut into nch chunks of ch rows, one block each;
   // window part and chunks leave fp32 partial sums in slabs, which a small kernel adds in a fixed order.
   int nst, nch, ch;
+  // Few (sequence, key head, key tile)s, as where many query heads share a key head: what a block sweeps is cut into `parts`
+  // blocks, each of which leaves fp32 sums in split, [parts][dK, dV][B * Lk][G * d], added in a fixed order as well.
+  int parts;
+  float* split;
 };
 
 struct Seq { int64_t qbase, kbase; int Lq, Lk, off; };
@@ -104,6 +108,20 @@ __host__ __device__ inline int slab_rows(const WinParams& p, int tile_rows) { re
 __device__ __forceinline__ float* slab(const WinParams& p, int b, int g, int st, int part, int tile_rows) {
   return p.slabs + ((((int64_t)b * p.G + g) * p.nst + st) * (1 + p.nch) + part) * 2 * slab_rows(p, tile_rows) * p.d;
 }
+
+// row j of sequence b, key head g in the partial sums of a part (which: 0 dK, 1 dV)
+__device__ __forceinline__ float* split_row(const WinParams& p, int part, int which, int b, int j, int g) {
+  return p.split + ((((int64_t)part * 2 + which) * p.B + b) * p.Lk + j) * ((int64_t)p.G * p.d) + (int64_t)g * p.d;
+}
+
+// The work of a block of the dK / dV kernels: a part of a key tile's window, or a chunk of a sink tile's far queries.
+struct KeyWork { int tile, part, chunk; };
+__device__ __forceinline__ KeyWork key_work(const WinParams& p, int ktiles, int work) {
+  const int extra = work - ktiles * p.parts;
+  if (extra < 0) return {work / p.parts, work % p.parts, -1};
+  return {extra / p.nch, 0, extra % p.nch};
+}
+__host__ __device__ inline int key_tiles_of_grid(const WinParams& p, int ktiles) { return ktiles * p.parts + p.nst * p.nch; }
 
 // The work of a block: tile `tile` of query head h (or key head, where `rep` is 1) of sequence b; the last blocks of a packed
 // batch's grid (b == B) zero rows of no sequence, TAIL parts a head.

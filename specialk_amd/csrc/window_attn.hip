@@ -297,8 +297,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 1) void window_dkv_kernel(WinPar
   __shared__ __attribute__((aligned(16))) Tile<D> Ds;
   __shared__ float s_lse[NT], s_dl[NT];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-  const int ktiles = max(1, (p.Lk + NT - 1) / NT), tiles = ktiles + p.nst * p.nch;
-  const Work work = work_of_block(p, tiles, 1, p.nst > 0);
+  const int ktiles = max(1, (p.Lk + NT - 1) / NT);
+  const Work work = work_of_block(p, key_tiles_of_grid(p, ktiles), 1, p.nst > 0);
   if (work.none) return;
   const int b = work.b, kh = work.h, rep = p.H / p.G;
   if (b == p.B) {
@@ -307,8 +307,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 1) void window_dkv_kernel(WinPar
     return;
   }
   const Seq sq = seq_of(p, b);
-  const int extra = work.tile - ktiles;                            // >= 0: a chunk of far queries of a sink tile
-  const int tile = extra < 0 ? work.tile : extra / p.nch, chunk = extra < 0 ? -1 : extra % p.nch;
+  const KeyWork kw = key_work(p, ktiles, work.tile);
+  const int tile = kw.tile, chunk = kw.chunk;
   const int j0 = tile * NT, j1 = min(j0 + NT, sq.Lk);
   if (j0 >= sq.Lk) return;
   int i_lo, i_hi;
@@ -334,8 +334,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 1) void window_dkv_kernel(WinPar
     row_lse = p.LSE[si];
     row_dl = p.delta[si];
   };
-  if (n > 0) load(0);
-  for (int t = 0; t < n; ++t) {
+  const int t_beg = chunk < 0 ? (int)((int64_t)n * kw.part / p.parts) : 0, t_end = chunk < 0 ? (int)((int64_t)n * (kw.part + 1) / p.parts) : n;
+  if (t_beg < t_end) load(t_beg);
+  for (int t = t_beg; t < t_end; ++t) {
     const int r0 = i_lo + (t % per) * NT;
     const uint64_t ok = bits(0, i_hi - r0);
     __syncthreads();
@@ -343,7 +344,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 1) void window_dkv_kernel(WinPar
     stage_d.store(Ds, ok, p.d);
     if (threadIdx.x < NT) { s_lse[threadIdx.x] = row_lse * LOG2E; s_dl[threadIdx.x] = row_dl; }
     __syncthreads();
-    if (t + 1 < n) load(t + 1);
+    if (t + 1 < t_end) load(t + 1);
     const uint64_t see = alive ? queries_seeing(p, j, r0 + sq.off, i_hi - r0) : 0;
     const uint64_t mk = see >> (4 * g);
 #pragma unroll
@@ -362,7 +363,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 1) void window_dkv_kernel(WinPar
     }
   }
   if (j >= sq.Lk) return;
-  if (sink) {
+  if (p.parts > 1 && chunk < 0) {
+    store_own<float, D>(split_row(p, kw.part, 0, b, j, kh), dk, p.scale, p.d, g);
+    store_own<float, D>(split_row(p, kw.part, 1, b, j, kh), dv, 1.f, p.d, g);
+  } else if (sink) {
     float* s = slab(p, b, kh, tile, 1 + chunk, NT) + (int64_t)(j - j0) * p.d;
     store_own<float, D>(s, dk, p.scale, p.d, g);
     store_own<float, D>(s + (int64_t)slab_rows(p, NT) * p.d, dv, 1.f, p.d, g);
@@ -395,6 +399,37 @@ __global__ __launch_bounds__(256) void window_join_kernel(WinParams p, int rows)
   ((T*)p.dV)[(sq.kbase + j) * p.lddv + (int64_t)kh * p.d + c] = Cvt<T>::from_f32(v);
 }
 
+// dK, dV of all keys where windows are cut into parts: the parts, then a sink's chunks.
+template <typename T>
+__global__ __launch_bounds__(256) void window_split_join_kernel(WinParams p, int rows) {
+  const int b = blockIdx.y;
+  const Seq sq = seq_of(p, b);
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int width = p.G * p.d, j = (int)(e / width), col = (int)(e - (int64_t)j * width), kh = col / p.d, c = col - kh * p.d;
+  if (j >= sq.Lk) return;
+  const float* x = split_row(p, 0, 0, b, j, kh) + c;
+  const int64_t half = (int64_t)p.B * p.Lk * width;
+  float a = 0.f, v = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < p.parts; ++s) {
+    a += x[2 * s * half];
+    v += x[(2 * s + 1) * half];
+  }
+  if (p.nst && j < p.sinks) {
+    const int tile = j / rows, j0 = tile * rows;
+    int lo, hi;
+    query_range(p, sq, j0, min(j0 + rows, sq.Lk), 0, lo, hi);
+    const int chunks = lo < hi ? (sq.Lq - lo + p.ch - 1) / p.ch : 0;
+    for (int s = 1; s <= chunks; ++s) {
+      const float* y = slab(p, b, kh, tile, s, rows) + (int64_t)(j - j0) * p.d + c;
+      a += y[0];
+      v += y[(int64_t)slab_rows(p, rows) * p.d];
+    }
+  }
+  ((T*)p.dK)[(sq.kbase + j) * p.lddk + col] = Cvt<T>::from_f32(a);
+  ((T*)p.dV)[(sq.kbase + j) * p.lddv + col] = Cvt<T>::from_f32(v);
+}
+
 // whether every row of the operands that go through LDS is made of whole 4-element pieces
 bool whole_pieces(const WinParams& p, int dtype) {
   const int64_t size = dtype == SK_BF16 ? 2 : 4;
@@ -425,25 +460,35 @@ void set_window(WinParams& p, int window, int causal) {
   p.sinks = std::min(p.sinks, p.Lk);
 }
 
-// Tiles that hold sinks and the chunks their far queries are cut into: about as many rows per chunk as a key tile's own
-// window has, so that these blocks last no longer than the others.
-void plan_sinks(WinParams& p, int rows) {
+// Parts of a key tile's window: two blocks for every CU, each with at least four tiles of queries (bf16, 2 x 4096 tokens, 8
+// heads of 128 over 2 key heads, window 512: 128 blocks alone 178 us, cut in four 80 and 15 for the join; fp32, 3 x 2000
+// tokens, 4 heads of 96 over one, window 1024, 30 sinks: 945 and 440.  Where one block fills a CU, fp32 at width 128, and
+// every CU has one, the cut gains nothing: the first case in fp32 530 and 550).
+// Tiles that hold sinks and the chunks their far queries are cut into: about as many rows per chunk as a part of a key
+// tile's own window has, so that these blocks last no longer than the others.
+void plan_keys(WinParams& p, int rows) {
+  const int64_t cus = sk_num_cus(), units = (int64_t)p.B * p.G, blocks = std::max<int64_t>(1, units * ((p.Lk + rows - 1) / rows));
+  const int64_t span = (int64_t)p.left + p.right + rows, tiles = (std::min<int64_t>(p.Lq, span) + 63) / 64 * (p.H / p.G);
+  p.parts = (int)std::max<int64_t>(1, std::min(2 * cus / blocks, tiles / 4));
   const bool far = p.sinks > 0 && p.left < p.Lk;   // else every query's window reaches key 0
   p.nst = far ? (p.sinks + rows - 1) / rows : 0;
-  p.ch = std::max(256, (p.left + p.right + rows + 63) / 64 * 64);
+  p.ch = (int)std::max<int64_t>(256, (span + 63) / 64 * 64);
+  const int64_t less = std::max<int64_t>(64, (span / p.parts + 63) / 64 * 64);
+  if (units * p.nst * (p.Lq / less + 1) <= 4 * cus) p.ch = (int)std::min<int64_t>(p.ch, p.parts > 1 ? less : p.ch);
   p.nch = far ? (p.Lq + p.ch - 1) / p.ch : 0;
 }
 
 // Grids of 256 threads a block whose threads are counted in 32 bits (tiles of 64 rows: the most that any kernel has).
 bool grids_fit(const WinParams& p) {
   const int64_t tiles = std::max(p.Lq, p.Lk) / 64 + 1, units = (int64_t)p.B * p.G + 7;
-  return units * tiles * (p.H / p.G) + TAIL * p.H < (1 << 24) && units * (tiles + (int64_t)p.nst * p.nch) + TAIL * p.G < (1 << 24) &&
+  return units * tiles * (p.H / p.G) + TAIL * p.H < (1 << 24) && units * (tiles * p.parts + (int64_t)p.nst * p.nch) + TAIL * p.G < (1 << 24) &&
          (p.nst == 0 || (int64_t)p.sinks * p.d < (1ll << 31));
 }
 
 int64_t slab_floats(const WinParams& p, int rows) {
-  return (int64_t)p.B * p.G * p.nst * (1 + p.nch) * 2 * slab_rows(p, rows) * p.d;
+  return ((int64_t)p.B * p.G * p.nst * (1 + p.nch) * 2 * slab_rows(p, rows) * p.d + 3) / 4 * 4;   // (16-byte stores behind)
 }
+int64_t split_floats(const WinParams& p) { return p.parts > 1 ? 2ll * p.parts * p.B * p.Lk * p.G * p.d : 0; }
 
 template <typename T, int D>
 void launch_fwd(const WinParams& p, hipStream_t stream) {
@@ -453,7 +498,7 @@ void launch_fwd(const WinParams& p, hipStream_t stream) {
 template <typename T, int D>
 void launch_bwd(const WinParams& p, hipStream_t stream) {
   const dim3 gq(work_blocks(p, std::max(1, (p.Lq + 63) / 64), p.H / p.G));
-  const dim3 gk(work_blocks(p, std::max(1, (p.Lk + NT - 1) / NT) + p.nst * p.nch, 1));
+  const dim3 gk(work_blocks(p, key_tiles_of_grid(p, std::max(1, (p.Lk + NT - 1) / NT)), 1));
   if (p.Tq) hipLaunchKernelGGL((window_dq_kernel<T, D>), gq, dim3(256), 0, stream, p);
   if (p.Tk) hipLaunchKernelGGL((window_dkv_kernel<T, D>), gk, dim3(256), 0, stream, p);
 }
@@ -461,7 +506,14 @@ void launch_bwd(const WinParams& p, hipStream_t stream) {
 }  // namespace
 
 int sk_window_join(const WinParams& p, int rows, int dtype, hipStream_t stream) {
-  if (!p.nst || !p.Tk) return SK_OK;
+  if ((!p.nst && p.parts == 1) || !p.Tk) return SK_OK;
+  if (p.parts > 1) {
+    const dim3 all((unsigned)(((int64_t)p.Lk * p.G * p.d + 255) / 256), p.B);
+    if (dtype == SK_BF16) hipLaunchKernelGGL((window_split_join_kernel<bf16_t>), all, dim3(256), 0, stream, p, rows);
+    else hipLaunchKernelGGL((window_split_join_kernel<float>), all, dim3(256), 0, stream, p, rows);
+    SK_CHECK_LAUNCH("skhip_window_attn_bwd(join)");
+    return SK_OK;
+  }
   dim3 grid((unsigned)(((int64_t)p.sinks * p.d + 255) / 256), p.G, p.B);
   if (dtype == SK_BF16) hipLaunchKernelGGL((window_join_kernel<bf16_t>), grid, dim3(256), 0, stream, p, rows);
   else hipLaunchKernelGGL((window_join_kernel<float>), grid, dim3(256), 0, stream, p, rows);
@@ -476,10 +528,10 @@ extern "C" int64_t skhip_window_attn_bwd_ws_floats(int B, int n_head, int n_kv, 
   p.B = B; p.H = n_head; p.G = n_kv; p.Lq = Lq; p.Lk = Lk; p.d = d; p.sinks = sinks;
   set_window(p, window, causal);
   // the larger of the two paths' needs: which one a call takes depends on its pointers and strides
-  plan_sinks(p, NT);
-  const int64_t plain = ((int64_t)n_head * Tq + 3) / 4 * 4 + slab_floats(p, NT);
-  plan_sinks(p, MFMA_ROWS);
-  return std::max(plain, (2 * (int64_t)n_head * Tq + 3) / 4 * 4 + slab_floats(p, MFMA_ROWS));
+  plan_keys(p, NT);
+  const int64_t plain = ((int64_t)n_head * Tq + 3) / 4 * 4 + slab_floats(p, NT) + split_floats(p);
+  plan_keys(p, MFMA_ROWS);
+  return std::max(plain, (2 * (int64_t)n_head * Tq + 3) / 4 * 4 + slab_floats(p, MFMA_ROWS) + split_floats(p));
 }
 
 extern "C" int skhip_window_attn_fwd(const void* Q, const void* K, const void* V, void* O, float* LSE, const uint8_t* key_pad,
@@ -531,21 +583,22 @@ extern "C" int skhip_window_attn_bwd(const void* Q, const void* K, const void* V
   if (Tq == 0 && Tk == 0) return SK_OK;
   SK_CHECK_ARG((Tq == 0 || (Q && O && dO && LSE && dQ)) && (Tk == 0 || (K && V && dK && dV)), "%s: null pointer", who);
   set_window(p, window, causal);
-  plan_sinks(p, MFMA_ROWS);
   const bool mfma = sk_window_mfma_supported(p, dtype);
-  if (!mfma) plan_sinks(p, NT);
+  const int rows = mfma ? MFMA_ROWS : NT;
+  plan_keys(p, rows);
   SK_CHECK_ARG(grids_fit(p), "%s: more than 2^24 tiles of 64 rows", who);
-  const int64_t head = (mfma ? 2 : 1) * (int64_t)n_head * Tq, need = (head + 3) / 4 * 4 + slab_floats(p, mfma ? MFMA_ROWS : NT);
+  const int64_t head = (mfma ? 2 : 1) * (int64_t)n_head * Tq, need = (head + 3) / 4 * 4 + slab_floats(p, rows) + split_floats(p);
   if (need > 0 && (!workspace || workspace_floats < need)) {
     sk_set_error("%s: workspace of %lld floats needed", who, (long long)need);
     return SK_ERR_WORKSPACE;
   }
   p.delta = workspace;
   p.slabs = workspace + (head + 3) / 4 * 4;   // (16-byte stores)
+  p.split = p.slabs + slab_floats(p, rows);
   p.vec = whole_pieces(p, dtype);
   if (mfma) {
     rc = sk_window_bwd_mfma(p, stream);
-    return rc ? rc : sk_window_join(p, MFMA_ROWS, dtype, stream);
+    return rc ? rc : sk_window_join(p, rows, dtype, stream);
   }
   if (dtype == SK_BF16) {
     if (d <= 64) launch_bwd<bf16_t, 64>(p, stream); else launch_bwd<bf16_t, 128>(p, stream);
@@ -553,5 +606,5 @@ extern "C" int skhip_window_attn_bwd(const void* Q, const void* K, const void* V
     if (d <= 64) launch_bwd<float, 64>(p, stream); else launch_bwd<float, 128>(p, stream);
   }
   SK_CHECK_LAUNCH(who);
-  return sk_window_join(p, NT, dtype, stream);
+  return sk_window_join(p, rows, dtype, stream);
 }

@@ -423,8 +423,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dkv_kernel(WinParams p, 
   __shared__ __attribute__((aligned(1024))) char lds[2][2 * tile_bytes<D>()];
   __shared__ __attribute__((aligned(16))) float rowv[2][2][NT];   // -log-sum-exp / scale, -delta
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, hf = lane >> 5;
-  const int tiles = ktiles + p.nst * p.nch;
-  const Work item = work_of_block(p, tiles, 1, p.nst > 0);
+  const Work item = work_of_block(p, key_tiles_of_grid(p, ktiles), 1, p.nst > 0);
   if (item.none) return;
   const int work = item.tile, kh = item.h, b = item.b, rep = p.H / p.G;
   if (b == p.B) {
@@ -433,7 +432,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dkv_kernel(WinParams p, 
     return;
   }
   const Seq sq = seq_of(p, b);
-  const int extra = work - ktiles, tile = extra < 0 ? work : extra / p.nch, chunk = extra < 0 ? -1 : extra % p.nch;
+  const KeyWork kw = key_work(p, ktiles, work);
+  const int tile = kw.tile, chunk = kw.chunk;
   const int j0 = tile * OWN, j1 = min(j0 + OWN, sq.Lk);
   if (j0 >= sq.Lk) return;
   int i_lo, i_hi;
@@ -501,11 +501,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dkv_kernel(WinParams p, 
       }
     }
   };
-  if (n > 0) fetch(0);
-  for (int t = 0; t < n; ++t) {
+  const int t_beg = chunk < 0 ? (int)((int64_t)n * kw.part / p.parts) : 0, t_end = chunk < 0 ? (int)((int64_t)n * (kw.part + 1) / p.parts) : n;
+  if (t_beg < t_end) fetch(t_beg);
+  for (int t = t_beg; t < t_end; ++t) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (t + 1 < n) fetch(t + 1);
+    if (t + 1 < t_end) fetch(t + 1);
     const int r0 = i_lo + (t % per) * NT, p0 = r0 + sq.off, p1 = min(r0 + NT, i_hi) - 1 + sq.off;
     if (!busy || p1 < jw - p.right || (p0 > jl + p.left && jw >= p.sinks)) continue;
     const char* Qs = lds[t & 1];
@@ -516,6 +517,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dkv_kernel(WinParams p, 
     if (!whole && alive) see = queries_seeing(p, j, p0, i_hi - r0);
 #pragma unroll(D == 64 ? 1 : 2)
     for (int k = 0; k < 2; ++k) half_tile(whole, Qs, Gs, rv, k, (uint32_t)(see >> (32 * k)) >> (4 * hf));
+  }
+  if (p.parts > 1 && chunk < 0) {
+    if (j >= sq.Lk) return;
+    if (DK) store_own_f32<D>(split_row(p, kw.part, 0, b, j, kh), dk, p.scale, p.d, hf);
+    if (DV) store_own_f32<D>(split_row(p, kw.part, 1, b, j, kh), dv, 1.f, p.d, hf);
+    return;
   }
   const bool sink = p.nst && j < p.sinks;   // (a sink's sum has further parts)
   if (sink && j < sq.Lk) {
@@ -556,7 +563,7 @@ int sk_window_fwd_mfma(const WinParams& p, hipStream_t stream) {
 
 int sk_window_bwd_mfma(const WinParams& p, hipStream_t stream) {
   const int qtiles = std::max(1, (p.Lq + OWN - 1) / OWN), ktiles = std::max(1, (p.Lk + OWN - 1) / OWN);
-  const dim3 gq(work_blocks(p, qtiles, p.H / p.G)), gk(work_blocks(p, ktiles + p.nst * p.nch, 1));
+  const dim3 gq(work_blocks(p, qtiles, p.H / p.G)), gk(work_blocks(p, key_tiles_of_grid(p, ktiles), 1));
   if (p.d <= 64) {
     if (p.Tq) hipLaunchKernelGGL((dq_kernel<64>), gq, dim3(256), 0, stream, p, qtiles);
     if (p.Tk) hipLaunchKernelGGL((dkv_kernel<64, 3>), gk, dim3(256), 0, stream, p, ktiles);

@@ -432,6 +432,24 @@ def test_window_results_repeat_bit_for_bit():
         assert all(torch.equal(a, b) for a, b in zip(res, first))
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("case", [  # few key heads: the dK / dV sums of a key tile come from several blocks
+    ([400], [400], 8, 1, 64, 100, 3, True), ([700], [700], 4, 1, 128, 60, 140, True), ([520], [520], 2, 1, 64, None, 0, True),
+    ([300], [410], 8, 2, 96, 200, 5, False), ([333], [333], 6, 1, 37, 150, 70, True), ([260], [130], 8, 1, 64, 90, 2, True)])
+def test_window_keys_in_parts(case, dtype):
+    lens_q, lens_k, H, G, d, window, sinks, causal = case
+    run_window(lens_q, lens_k, H, G, d, window, sinks, causal, dtype, "dense", seed=3)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_window_keys_in_parts_of_ragged_batches(dtype):
+    lens = [300, 1, 0, 170, 64]
+    run_window(lens, lens, 8, 1, 64, 120, 4, True, dtype, "packed", seed=4)
+    pads = torch.zeros((3, 290), dtype=torch.uint8)
+    pads[0, 200:], pads[1, :40], pads[2, :] = 1, 1, 1
+    run_window([290] * 3, [290] * 3, 8, 2, 80, 150, 2, True, dtype, "padded", seed=5, pads=pads)
+
+
 # ------------------------------------------------------------------------------ one step over a cache
 def slot_of(j, cap, sinks):
     return j if j < sinks else sinks + (j - sinks) % (cap - sinks)
