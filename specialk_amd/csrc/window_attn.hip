@@ -20,6 +20,9 @@ using namespace skwin;
 namespace {
 
 constexpr int NT = 64;     // rows per LDS tile
+// Blocks per CU.  At width 128 the dK / dV kernel spills 23 registers for its second block and is faster for it (2 x 4096
+// tokens, 8 heads, 2 key heads, window 512: 530 us alone, 428 by two; dQ 448 and 327).
+constexpr int BLOCKS(int D) { return D <= 64 ? 3 : 2; }
 constexpr int MAXD = 128;
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr int MFMA_ROWS = 128;   // key rows of a block of the bf16 path
@@ -176,7 +179,7 @@ __device__ __forceinline__ bool piece(uint64_t see, int k) { return __any(((see 
 
 // ------------------------------------------------------------------------------ forward
 template <typename T, int D>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 1) void window_fwd_kernel(WinParams p) {
+__global__ __launch_bounds__(256, BLOCKS(D)) void window_fwd_kernel(WinParams p) {
   __shared__ __attribute__((aligned(16))) Tile<D> Ks;
   __shared__ __attribute__((aligned(16))) Tile<D> Vs;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
@@ -241,7 +244,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 1) void window_fwd_kernel(WinPar
 
 // ------------------------------------------------------------------------------ dQ, delta
 template <typename T, int D>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 1) void window_dq_kernel(WinParams p) {
+__global__ __launch_bounds__(256, BLOCKS(D)) void window_dq_kernel(WinParams p) {
   __shared__ __attribute__((aligned(16))) Tile<D> Ks;
   __shared__ __attribute__((aligned(16))) Tile<D> Vs;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
@@ -292,7 +295,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 1) void window_dq_kernel(WinPara
 
 // ------------------------------------------------------------------------------ dK, dV
 template <typename T, int D>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 1) void window_dkv_kernel(WinParams p) {
+__global__ __launch_bounds__(256, BLOCKS(D)) void window_dkv_kernel(WinParams p) {
   __shared__ __attribute__((aligned(16))) Tile<D> Qs;
   __shared__ __attribute__((aligned(16))) Tile<D> Ds;
   __shared__ float s_lse[NT], s_dl[NT];
@@ -462,8 +465,7 @@ void set_window(WinParams& p, int window, int causal) {
 
 // Parts of a key tile's window: two blocks for every CU, each with at least four tiles of queries (bf16, 2 x 4096 tokens, 8
 // heads of 128 over 2 key heads, window 512: 128 blocks alone 178 us, cut in four 80 and 15 for the join; fp32, 3 x 2000
-// tokens, 4 heads of 96 over one, window 1024, 30 sinks: 945 and 440.  Where one block fills a CU, fp32 at width 128, and
-// every CU has one, the cut gains nothing: the first case in fp32 530 and 550).
+// tokens, 4 heads of 96 over one, window 1024, 30 sinks: 945 and 440).
 // Tiles that hold sinks and the chunks their far queries are cut into: about as many rows per chunk as a part of a key
 // tile's own window has, so that these blocks last no longer than the others.
 void plan_keys(WinParams& p, int rows) {
@@ -491,16 +493,32 @@ int64_t slab_floats(const WinParams& p, int rows) {
 int64_t split_floats(const WinParams& p) { return p.parts > 1 ? 2ll * p.parts * p.B * p.Lk * p.G * p.d : 0; }
 
 template <typename T, int D>
-void launch_fwd(const WinParams& p, hipStream_t stream) {
+void launch_fwd_at(const WinParams& p, hipStream_t stream) {
   const dim3 grid(work_blocks(p, std::max(1, (p.Lq + 63) / 64), p.H / p.G));
   hipLaunchKernelGGL((window_fwd_kernel<T, D>), grid, dim3(256), 0, stream, p);
 }
 template <typename T, int D>
-void launch_bwd(const WinParams& p, hipStream_t stream) {
+void launch_bwd_at(const WinParams& p, hipStream_t stream) {
   const dim3 gq(work_blocks(p, std::max(1, (p.Lq + 63) / 64), p.H / p.G));
   const dim3 gk(work_blocks(p, key_tiles_of_grid(p, std::max(1, (p.Lk + NT - 1) / NT)), 1));
   if (p.Tq) hipLaunchKernelGGL((window_dq_kernel<T, D>), gq, dim3(256), 0, stream, p);
   if (p.Tk) hipLaunchKernelGGL((window_dkv_kernel<T, D>), gk, dim3(256), 0, stream, p);
+}
+// Heads are computed at the next multiple of 32 elements (4 x 4096 tokens, 8 heads, window 512, forward and backward: 32 of
+// 64 columns 862 us, of 32 466; 80 of 128 2540, of 96 1570).
+template <typename T>
+void launch_fwd(const WinParams& p, hipStream_t stream) {
+  if (p.d <= 32) launch_fwd_at<T, 32>(p, stream);
+  else if (p.d <= 64) launch_fwd_at<T, 64>(p, stream);
+  else if (p.d <= 96) launch_fwd_at<T, 96>(p, stream);
+  else launch_fwd_at<T, 128>(p, stream);
+}
+template <typename T>
+void launch_bwd(const WinParams& p, hipStream_t stream) {
+  if (p.d <= 32) launch_bwd_at<T, 32>(p, stream);
+  else if (p.d <= 64) launch_bwd_at<T, 64>(p, stream);
+  else if (p.d <= 96) launch_bwd_at<T, 96>(p, stream);
+  else launch_bwd_at<T, 128>(p, stream);
 }
 
 }  // namespace
@@ -553,9 +571,9 @@ extern "C" int skhip_window_attn_fwd(const void* Q, const void* K, const void* V
   if (sk_window_mfma_supported(p, dtype)) return sk_window_fwd_mfma(p, stream);
   p.vec = whole_pieces(p, dtype);
   if (dtype == SK_BF16) {
-    if (d <= 64) launch_fwd<bf16_t, 64>(p, stream); else launch_fwd<bf16_t, 128>(p, stream);
+    launch_fwd<bf16_t>(p, stream);
   } else {
-    if (d <= 64) launch_fwd<float, 64>(p, stream); else launch_fwd<float, 128>(p, stream);
+    launch_fwd<float>(p, stream);
   }
   SK_CHECK_LAUNCH(who);
   return SK_OK;
@@ -601,9 +619,9 @@ extern "C" int skhip_window_attn_bwd(const void* Q, const void* K, const void* V
     return rc ? rc : sk_window_join(p, rows, dtype, stream);
   }
   if (dtype == SK_BF16) {
-    if (d <= 64) launch_bwd<bf16_t, 64>(p, stream); else launch_bwd<bf16_t, 128>(p, stream);
+    launch_bwd<bf16_t>(p, stream);
   } else {
-    if (d <= 64) launch_bwd<float, 64>(p, stream); else launch_bwd<float, 128>(p, stream);
+    launch_bwd<float>(p, stream);
   }
   SK_CHECK_LAUNCH(who);
   return sk_window_join(p, rows, dtype, stream);

@@ -1,6 +1,6 @@
 // Attention within a sliding window, forward and backward, for bf16 heads on the matrix cores (v_mfma_f32_32x32x16_bf16).
-// The mathematics stands in window_attn.hip; this is the path for 16-byte aligned heads of a multiple of 8 elements, run
-// at a width of 64 or 128 (elements beyond the head read as zero).
+// The mathematics stands in window_attn.hip; this is the path for 16-byte aligned heads of a multiple of 8 elements.  LDS
+// rows are 64 or 128 columns (D), the arithmetic is done on the next multiple of 32 (W; elements beyond the head are zero).
 //
 // A wave owns 32 rows (queries; keys in the dK / dV kernel), a block 128, and sweeps the other side in tiles of 64 rows.
 // All products are D[rho][c] = sum_k X[rho][k] Y[c][k] with X from LDS and the own rows Y in registers: lane c = lane & 31
@@ -27,6 +27,7 @@ typedef __attribute__((address_space(3))) void* lds_ptr;
 
 constexpr int NT = 64;         // rows per LDS tile
 constexpr int OWN = 128;       // own rows per block
+constexpr int TOGETHER = 96;   // widest heads whose dK and dV come from one launch (see there)
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr uint32_t NOWHERE = 0x80000000u;   // offset beyond every buffer
 
@@ -78,10 +79,10 @@ __device__ __forceinline__ void load_tile(char* t, const bf16_t* base, int64_t l
 }
 
 // own row: y[s] = elements 16 s + 8 h .. + 7
-template <int D>
-__device__ __forceinline__ void load_own(bf16x8_t (&y)[D / 16], const bf16_t* row, int d, int h, bool ok) {
+template <int W>
+__device__ __forceinline__ void load_own(bf16x8_t (&y)[W / 16], const bf16_t* row, int d, int h, bool ok) {
 #pragma unroll
-  for (int s = 0; s < D / 16; ++s) {
+  for (int s = 0; s < W / 16; ++s) {
     const int c = 16 * s + 8 * h;
     uint4 v = make_uint4(0, 0, 0, 0);
     if (ok && c < d) v = *(const uint4*)(row + c);
@@ -119,10 +120,10 @@ __device__ __forceinline__ bf16x8_t pack_y(const f32x16_t& a, int s) {
 
 // Own row's output, columns 32 t + 8 (r / 4) + 4 h + r % 4: the halves exchange their 8-byte pieces so that each lane
 // stores 16 bytes.
-template <int D>
-__device__ __forceinline__ void store_own(bf16_t* row, const f32x16_t (&o)[D / 32], float mul, int d, int h, bool ok) {
+template <int W>
+__device__ __forceinline__ void store_own(bf16_t* row, const f32x16_t (&o)[W / 32], float mul, int d, int h, bool ok) {
 #pragma unroll
-  for (int t = 0; t < D / 32; ++t)
+  for (int t = 0; t < W / 32; ++t)
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       uint32_t a0 = pack2(o[t][8 * u] * mul, o[t][8 * u + 1] * mul), a1 = pack2(o[t][8 * u + 2] * mul, o[t][8 * u + 3] * mul);
@@ -135,10 +136,10 @@ __device__ __forceinline__ void store_own(bf16_t* row, const f32x16_t (&o)[D / 3
 }
 
 // the same in fp32, for partial sums
-template <int D>
-__device__ __forceinline__ void store_own_f32(float* row, const f32x16_t (&o)[D / 32], float mul, int d, int h) {
+template <int W>
+__device__ __forceinline__ void store_own_f32(float* row, const f32x16_t (&o)[W / 32], float mul, int d, int h) {
 #pragma unroll
-  for (int t = 0; t < D / 32; ++t)
+  for (int t = 0; t < W / 32; ++t)
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int c = 32 * t + 8 * u + 4 * h;
@@ -160,7 +161,7 @@ __device__ __forceinline__ float keep_or(float v, uint32_t m, uint32_t other) {
 // exponentials of 16 cycles plus some five full-rate instructions per register.  The scale goes into the exponent's
 // multiply-add, and the accumulators are rescaled only when a row's maximum has grown by more than 2^8 since the last
 // time: until then probabilities stay below 256, which bf16 holds as precisely as values below one.
-template <int D>
+template <int D, int W>
 __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void fwd_kernel(WinParams p, int qtiles) {
   __shared__ __attribute__((aligned(1024))) char lds[2][2 * tile_bytes<D>()];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, hf = lane >> 5;
@@ -181,19 +182,19 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void fwd_kernel(WinParams p, 
   const bf16_t* V = (const bf16_t*)p.V + sq.kbase * p.ldv + (int64_t)kh * p.d;
   const uint8_t* pad = p.key_pad ? p.key_pad + (int64_t)b * p.Lk : nullptr;
   const float cs = fabsf(p.scale) * LOG2E;
-  bf16x8_t q[D / 16];
-  load_own<D>(q, (const bf16_t*)p.Q + (sq.qbase + min(i, sq.Lq - 1)) * p.ldq + (int64_t)h * p.d, p.d, hf, i < sq.Lq);
+  bf16x8_t q[W / 16];
+  load_own<W>(q, (const bf16_t*)p.Q + (sq.qbase + min(i, sq.Lq - 1)) * p.ldq + (int64_t)h * p.d, p.d, hf, i < sq.Lq);
   if (p.scale < 0.f) {   // the maximum is taken over unscaled scores
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
+    for (int s = 0; s < W / 16; ++s) {
       uint4 v = __builtin_bit_cast(uint4, q[s]);
       v.x ^= 0x80008000u; v.y ^= 0x80008000u; v.z ^= 0x80008000u; v.w ^= 0x80008000u;
       q[s] = __builtin_bit_cast(bf16x8_t, v);
     }
   }
-  f32x16_t o[D / 32];
+  f32x16_t o[W / 32];
 #pragma unroll
-  for (int t = 0; t < D / 32; ++t) o[t] = zero16();
+  for (int t = 0; t < W / 32; ++t) o[t] = zero16();
   float m = -INFINITY, l = 0.f;
 
   // rows of tile t that may be used; the padding byte comes a round ahead, so that no wait for it waits for a tile too
@@ -227,7 +228,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void fwd_kernel(WinParams p, 
     for (int k = 0; k < 2; ++k) {
       sc[k] = zero16();
 #pragma unroll
-      for (int s = 0; s < D / 16; ++s) sc[k] = mfma(x_rows<D>(Ks, 32 * k, s, lane), q[s], sc[k]);
+      for (int s = 0; s < W / 16; ++s) sc[k] = mfma(x_rows<D>(Ks, 32 * k, s, lane), q[s], sc[k]);
     }
     const bool whole = use == ~0ull && j0 + NT - 1 <= pmin + p.right && (j0 >= pmax - p.left || j0 + NT <= p.sinks);
     if (!whole) {
@@ -253,7 +254,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void fwd_kernel(WinParams p, 
       m = mn;
       l *= alpha;
 #pragma unroll
-      for (int x = 0; x < D / 32; ++x) o[x] *= alpha;
+      for (int x = 0; x < W / 32; ++x) o[x] *= alpha;
     }
     const float mc = m == -INFINITY ? 0.f : m * cs;
     float sum = 0.f;
@@ -271,11 +272,11 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void fwd_kernel(WinParams p, 
       for (int s = 0; s < 2; ++s) {
         const bf16x8_t y = pack_y(sc[k], s);
 #pragma unroll
-        for (int x = 0; x < D / 32; ++x) o[x] = mfma(x_cols<D>(Vs, 32 * x, 32 * k + 16 * s, lane), y, o[x]);
+        for (int x = 0; x < W / 32; ++x) o[x] = mfma(x_cols<D>(Vs, 32 * x, 32 * k + 16 * s, lane), y, o[x]);
       }
   }
   l = other_sum(l);   // the halves summed different keys
-  store_own<D>((bf16_t*)p.Oout + (sq.qbase + min(i, sq.Lq - 1)) * p.ldo + (int64_t)h * p.d, o, l > 0.f || l != l ? 1.f / l : 0.f, p.d, hf,
+  store_own<W>((bf16_t*)p.Oout + (sq.qbase + min(i, sq.Lq - 1)) * p.ldo + (int64_t)h * p.d, o, l > 0.f || l != l ? 1.f / l : 0.f, p.d, hf,
                i < sq.Lq);
   if (i < sq.Lq && hf == 0)
     p.LSE[(int64_t)h * p.Tq + sq.qbase + i] = l > 0.f ? m * fabsf(p.scale) + logf(l) : (l != l ? l : -INFINITY);
@@ -289,7 +290,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void fwd_kernel(WinParams p, 
 // first rows of a text, rows behind it, small windows) take delta = sum_j P dP in fp32 from a sweep of its own: with four
 // visible keys dQ and dK are then 1.4 instead of 1.65 times as far from the exact values as a result rounded once.
 constexpr int FEW = 32;
-template <int D>
+template <int D, int W>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dq_kernel(WinParams p, int qtiles) {
   __shared__ __attribute__((aligned(1024))) char lds[2][2 * tile_bytes<D>()];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, hf = lane >> 5;
@@ -311,20 +312,20 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dq_kernel(WinParams p, i
   const bf16_t* V = (const bf16_t*)p.V + sq.kbase * p.ldv + (int64_t)kh * p.d;
   const uint8_t* pad = p.key_pad ? p.key_pad + (int64_t)b * p.Lk : nullptr;
   const float cs = p.scale * LOG2E;
-  bf16x8_t q[D / 16], g[D / 16];
-  load_own<D>(g, (const bf16_t*)p.dO + row * p.lddo + (int64_t)h * p.d, p.d, hf, i < sq.Lq);
-  load_own<D>(q, (const bf16_t*)p.O + row * p.ldo + (int64_t)h * p.d, p.d, hf, i < sq.Lq);
+  bf16x8_t q[W / 16], g[W / 16];
+  load_own<W>(g, (const bf16_t*)p.dO + row * p.lddo + (int64_t)h * p.d, p.d, hf, i < sq.Lq);
+  load_own<W>(q, (const bf16_t*)p.O + row * p.ldo + (int64_t)h * p.d, p.d, hf, i < sq.Lq);
   float dl = 0.f;
 #pragma unroll
-  for (int s = 0; s < D / 16; ++s)
+  for (int s = 0; s < W / 16; ++s)
 #pragma unroll
     for (int j = 0; j < 8; ++j) dl += (float)q[s][j] * (float)g[s][j];
   dl = other_sum(dl);
-  load_own<D>(q, (const bf16_t*)p.Q + row * p.ldq + (int64_t)h * p.d, p.d, hf, i < sq.Lq);
+  load_own<W>(q, (const bf16_t*)p.Q + row * p.ldq + (int64_t)h * p.d, p.d, hf, i < sq.Lq);
   const float lse2 = p.LSE[si] * LOG2E;
-  f32x16_t dq[D / 32];
+  f32x16_t dq[W / 32];
 #pragma unroll
-  for (int t = 0; t < D / 32; ++t) dq[t] = zero16();
+  for (int t = 0; t < W / 32; ++t) dq[t] = zero16();
 
   // rows of tile t that may be used; the padding byte comes a round ahead, so that no wait for it waits for a tile too
   auto padding = [&](int t) -> int { return pad && t < kt.n ? pad[min(kt.start<NT>(t) + lane, sq.Lk - 1)] : 0; };
@@ -345,7 +346,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dq_kernel(WinParams p, i
   auto half_tile = [&](auto delta_only, bool whole, const char* Ks, const char* Vs, int k, uint32_t mk) {
     f32x16_t sc = zero16(), dp = zero16();
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
+    for (int s = 0; s < W / 16; ++s) {
       sc = mfma(x_rows<D>(Ks, 32 * k, s, lane), q[s], sc);
       dp = mfma(x_rows<D>(Vs, 32 * k, s, lane), g[s], dp);
     }
@@ -369,7 +370,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dq_kernel(WinParams p, i
       for (int s = 0; s < 2; ++s) {
         const bf16x8_t y = pack_y(sc, s);
 #pragma unroll
-        for (int x = 0; x < D / 32; ++x) dq[x] = mfma(x_cols<D>(Ks, 32 * x, 32 * k + 16 * s, lane), y, dq[x]);
+        for (int x = 0; x < W / 32; ++x) dq[x] = mfma(x_cols<D>(Ks, 32 * x, 32 * k + 16 * s, lane), y, dq[x]);
       }
     }
     return part;
@@ -409,15 +410,16 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dq_kernel(WinParams p, i
     p.delta[si] = -dl;
     p.delta[(int64_t)p.H * p.Tq + si] = -p.LSE[si] / p.scale;
   }
-  store_own<D>((bf16_t*)p.dQ + row * p.lddq + (int64_t)h * p.d, dq, p.scale, p.d, hf, i < sq.Lq);
+  store_own<W>((bf16_t*)p.dQ + row * p.lddq + (int64_t)h * p.d, dq, p.scale, p.d, hf, i < sq.Lq);
 }
 
 // ------------------------------------------------------------------------------ dK, dV
 // Own rows are keys; the tiles hold 64 queries and their output gradients, head after head of the group that shares them.
-// WHAT: 1 = dK, 2 = dV, 3 = both.  At a width of 64 one launch computes both.  At 128 the two sums and the own rows alone
+// WHAT: 1 = dK, 2 = dV, 3 = both.  Up to a width of 96 one launch computes both (4 x 4096 tokens, 8 heads of 80, window 512,
+// forward and backward: 240 us, apart 295).  At 128 the two sums and the own rows alone
 // are 192 registers, and with them only one wave fits a SIMD: dK and dV as launches of their own cost the scores twice
 // (10 instead of 8 products) but keep two (16384 tokens, causal, 16 heads: 3.73 ms together, 1.67 + 1.25 ms apart).
-template <int D, int WHAT>
+template <int D, int W, int WHAT>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dkv_kernel(WinParams p, int ktiles) {
   constexpr bool DK = WHAT & 1, DV = WHAT & 2;
   __shared__ __attribute__((aligned(1024))) char lds[2][2 * tile_bytes<D>()];
@@ -442,13 +444,13 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dkv_kernel(WinParams p, 
   const int jw = j0 + 32 * wave, j = jw + c, jrow = min(j, sq.Lk - 1), jl = min(jw + 31, sq.Lk - 1);
   const bool alive = j < sq.Lk && !(p.key_pad && p.key_pad[(int64_t)b * p.Lk + jrow]);
   const bool all_alive = __all(alive), busy = jw < sq.Lk && (chunk < 0 || jw < p.sinks);   // wave-uniform
-  bf16x8_t fk[D / 16], fv[D / 16];
-  load_own<D>(fk, (const bf16_t*)p.K + (sq.kbase + jrow) * p.ldk + (int64_t)kh * p.d, p.d, hf, alive);
-  if (DK) load_own<D>(fv, (const bf16_t*)p.V + (sq.kbase + jrow) * p.ldv + (int64_t)kh * p.d, p.d, hf, alive);
+  bf16x8_t fk[W / 16], fv[W / 16];
+  load_own<W>(fk, (const bf16_t*)p.K + (sq.kbase + jrow) * p.ldk + (int64_t)kh * p.d, p.d, hf, alive);
+  if (DK) load_own<W>(fv, (const bf16_t*)p.V + (sq.kbase + jrow) * p.ldv + (int64_t)kh * p.d, p.d, hf, alive);
   const float cs = p.scale * LOG2E;
-  f32x16_t dk[D / 32], dv[D / 32];
+  f32x16_t dk[W / 32], dv[W / 32];
 #pragma unroll
-  for (int t = 0; t < D / 32; ++t) dk[t] = dv[t] = zero16();
+  for (int t = 0; t < W / 32; ++t) dk[t] = dv[t] = zero16();
 
   const int per = (i_hi - i_lo + NT - 1) / NT, n = per * rep;
   auto fetch = [&](int t) {
@@ -473,7 +475,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dkv_kernel(WinParams p, 
       dp[4 * u] = de.x; dp[4 * u + 1] = de.y; dp[4 * u + 2] = de.z; dp[4 * u + 3] = de.w;
     }
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
+    for (int s = 0; s < W / 16; ++s) {
       sc = mfma(x_rows<D>(Qs, 32 * k, s, lane), fk[s], sc);
       if (DK) dp = mfma(x_rows<D>(Gs, 32 * k, s, lane), fv[s], dp);
     }
@@ -495,7 +497,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dkv_kernel(WinParams p, 
     for (int s = 0; s < 2; ++s) {
       const bf16x8_t yp = pack_y(sc, s), ys = pack_y(dp, s);
 #pragma unroll
-      for (int x = 0; x < D / 32; ++x) {
+      for (int x = 0; x < W / 32; ++x) {
         if (DV) dv[x] = mfma(x_cols<D>(Gs, 32 * x, 32 * k + 16 * s, lane), yp, dv[x]);
         if (DK) dk[x] = mfma(x_cols<D>(Qs, 32 * x, 32 * k + 16 * s, lane), ys, dk[x]);
       }
@@ -520,22 +522,42 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dkv_kernel(WinParams p, 
   }
   if (p.parts > 1 && chunk < 0) {
     if (j >= sq.Lk) return;
-    if (DK) store_own_f32<D>(split_row(p, kw.part, 0, b, j, kh), dk, p.scale, p.d, hf);
-    if (DV) store_own_f32<D>(split_row(p, kw.part, 1, b, j, kh), dv, 1.f, p.d, hf);
+    if (DK) store_own_f32<W>(split_row(p, kw.part, 0, b, j, kh), dk, p.scale, p.d, hf);
+    if (DV) store_own_f32<W>(split_row(p, kw.part, 1, b, j, kh), dv, 1.f, p.d, hf);
     return;
   }
   const bool sink = p.nst && j < p.sinks;   // (a sink's sum has further parts)
   if (sink && j < sq.Lk) {
     float* s = slab(p, b, kh, tile, 1 + chunk, OWN) + (int64_t)(j - j0) * p.d;
-    if (DK) store_own_f32<D>(s, dk, p.scale, p.d, hf);
-    if (DV) store_own_f32<D>(s + (int64_t)slab_rows(p, OWN) * p.d, dv, 1.f, p.d, hf);
+    if (DK) store_own_f32<W>(s, dk, p.scale, p.d, hf);
+    if (DV) store_own_f32<W>(s + (int64_t)slab_rows(p, OWN) * p.d, dv, 1.f, p.d, hf);
   }
   if (chunk >= 0) return;
-  if (DK) store_own<D>((bf16_t*)p.dK + (sq.kbase + jrow) * p.lddk + (int64_t)kh * p.d, dk, p.scale, p.d, hf, j < sq.Lk && !sink);
-  if (DV) store_own<D>((bf16_t*)p.dV + (sq.kbase + jrow) * p.lddv + (int64_t)kh * p.d, dv, 1.f, p.d, hf, j < sq.Lk && !sink);
+  if (DK) store_own<W>((bf16_t*)p.dK + (sq.kbase + jrow) * p.lddk + (int64_t)kh * p.d, dk, p.scale, p.d, hf, j < sq.Lk && !sink);
+  if (DV) store_own<W>((bf16_t*)p.dV + (sq.kbase + jrow) * p.lddv + (int64_t)kh * p.d, dv, 1.f, p.d, hf, j < sq.Lk && !sink);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+template <int D, int W>
+void launch_fwd(const WinParams& p, hipStream_t stream) {
+  const int qtiles = std::max(1, (p.Lq + OWN - 1) / OWN);
+  const dim3 grid(work_blocks(p, qtiles, p.H / p.G));
+  hipLaunchKernelGGL((fwd_kernel<D, W>), grid, dim3(256), 0, stream, p, qtiles);
+}
+template <int D, int W>
+void launch_bwd(const WinParams& p, hipStream_t stream) {
+  const int qtiles = std::max(1, (p.Lq + OWN - 1) / OWN), ktiles = std::max(1, (p.Lk + OWN - 1) / OWN);
+  const dim3 gq(work_blocks(p, qtiles, p.H / p.G)), gk(work_blocks(p, key_tiles_of_grid(p, ktiles), 1));
+  if (p.Tq) hipLaunchKernelGGL((dq_kernel<D, W>), gq, dim3(256), 0, stream, p, qtiles);
+  if (!p.Tk) return;
+  if constexpr (W <= TOGETHER) {
+    hipLaunchKernelGGL((dkv_kernel<D, W, 3>), gk, dim3(256), 0, stream, p, ktiles);
+  } else {
+    hipLaunchKernelGGL((dkv_kernel<D, W, 1>), gk, dim3(256), 0, stream, p, ktiles);
+    hipLaunchKernelGGL((dkv_kernel<D, W, 2>), gk, dim3(256), 0, stream, p, ktiles);
+  }
+}
 
 }  // namespace
 
@@ -553,25 +575,19 @@ bool sk_window_mfma_supported(const WinParams& p, int dtype) {
 }
 
 int sk_window_fwd_mfma(const WinParams& p, hipStream_t stream) {
-  const int qtiles = std::max(1, (p.Lq + OWN - 1) / OWN);
-  const dim3 grid(work_blocks(p, qtiles, p.H / p.G));
-  if (p.d <= 64) hipLaunchKernelGGL((fwd_kernel<64>), grid, dim3(256), 0, stream, p, qtiles);
-  else hipLaunchKernelGGL((fwd_kernel<128>), grid, dim3(256), 0, stream, p, qtiles);
+  if (p.d <= 32) launch_fwd<64, 32>(p, stream);
+  else if (p.d <= 64) launch_fwd<64, 64>(p, stream);
+  else if (p.d <= 96) launch_fwd<128, 96>(p, stream);
+  else launch_fwd<128, 128>(p, stream);
   SK_CHECK_LAUNCH("skhip_window_attn_fwd(mfma)");
   return SK_OK;
 }
 
 int sk_window_bwd_mfma(const WinParams& p, hipStream_t stream) {
-  const int qtiles = std::max(1, (p.Lq + OWN - 1) / OWN), ktiles = std::max(1, (p.Lk + OWN - 1) / OWN);
-  const dim3 gq(work_blocks(p, qtiles, p.H / p.G)), gk(work_blocks(p, key_tiles_of_grid(p, ktiles), 1));
-  if (p.d <= 64) {
-    if (p.Tq) hipLaunchKernelGGL((dq_kernel<64>), gq, dim3(256), 0, stream, p, qtiles);
-    if (p.Tk) hipLaunchKernelGGL((dkv_kernel<64, 3>), gk, dim3(256), 0, stream, p, ktiles);
-  } else {
-    if (p.Tq) hipLaunchKernelGGL((dq_kernel<128>), gq, dim3(256), 0, stream, p, qtiles);
-    if (p.Tk) hipLaunchKernelGGL((dkv_kernel<128, 1>), gk, dim3(256), 0, stream, p, ktiles);
-    if (p.Tk) hipLaunchKernelGGL((dkv_kernel<128, 2>), gk, dim3(256), 0, stream, p, ktiles);
-  }
+  if (p.d <= 32) launch_bwd<64, 32>(p, stream);
+  else if (p.d <= 64) launch_bwd<64, 64>(p, stream);
+  else if (p.d <= 96) launch_bwd<128, 96>(p, stream);
+  else launch_bwd<128, 128>(p, stream);
   SK_CHECK_LAUNCH("skhip_window_attn_bwd(mfma)");
   return SK_OK;
 }
