@@ -68,11 +68,24 @@ __device__ __forceinline__ float2 turn_cos_sin(uint64_t phase) {
   return r;
 }
 
-// The 16 elements of lane l of a head: v[j], v[8 + j] = the two halves of pair 8 l + j, or 16 consecutive passing ones.
-template <typename T, bool IL, bool VEC>
+// How the elements of a head are dealt to its lanes.
+//  PAIRS     lane l holds 8 pairs, v[j] and v[8 + j] = the two halves of pair 8 l + j, or 16 consecutive passing elements;
+//            16-byte loads where rot and d are multiples of 16.
+//  ELEMENTS  lane l holds elements 16 l .. 16 l + 15, loaded 16 bytes at a time whatever rot is (d a multiple of 8); the other
+//            half of a pair may lie with another lane of the head and is fetched through LDS.
+//  SCALARS   the pairs, element by element: odd sizes and rows that are not 16-byte aligned.
+// (46626 rows of 4 + 1 bf16 heads of 64, 36 elements turned, forward and backward: SCALARS 131 us, ELEMENTS 47.)
+enum Deal { SCALARS, PAIRS, ELEMENTS };
+
+template <typename T, bool IL, Deal DEAL>
 struct Own {
   static constexpr int VN = Vec16<T>::N;
+  static constexpr bool VEC = DEAL == PAIRS, ELEM = DEAL == ELEMENTS;
+  static __device__ __forceinline__ int lanes(const RotParams& p) {
+    return ELEM ? (p.d + 15) >> 4 : (((p.rot >> 1) + 7) >> 3) + ((p.d - p.rot + 15) >> 4);
+  }
   static __device__ __forceinline__ int index(const RotParams& p, int l, int j) {   // j in 0 .. 15; -1: no element
+    if (ELEM) return 16 * l + j < p.d ? 16 * l + j : -1;
     const int np = p.rot >> 1, nrl = (np + 7) >> 3;
     if (l < nrl) {
       const int pr = 8 * l + (j & 7);
@@ -84,6 +97,7 @@ struct Own {
   }
   // base: the head's first element.  Vector form (rot and d multiples of 16, 16-byte rows): two runs of 8 elements.
   static __device__ __forceinline__ int run(const RotParams& p, int l, int half) {
+    if (ELEM) return 16 * l + 8 * half;
     const int np = p.rot >> 1, nrl = np >> 3;
     if (l < nrl) return IL ? 16 * l + 8 * half : 8 * l + half * np;
     return p.rot + 16 * (l - nrl) + 8 * half;
@@ -93,12 +107,13 @@ struct Own {
   static constexpr int NR = 16 / VN;
   struct Raw { raw_t r[NR]; };
   static __device__ __forceinline__ void load(Raw& w, const T* base, const RotParams& p, int l, bool active) {
-    if constexpr (VEC) {
+    if constexpr (VEC || ELEM) {
       if (active) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int i = 0; i < NR / 2; ++i) w.r[h * (NR / 2) + i] = *(const raw_t*)(base + run(p, l, h) + i * VN);
+          for (int i = 0; i < NR / 2; ++i)
+            w.r[h * (NR / 2) + i] = !ELEM || run(p, l, h) < p.d ? *(const raw_t*)(base + run(p, l, h) + i * VN) : raw_t{};
       }
     } else {
       T* e = (T*)w.r;
@@ -121,10 +136,10 @@ struct Own {
     }
   }
   static __device__ __forceinline__ void store(T* base, const float (&v)[16], const RotParams& p, int l, bool rotates) {
-    if constexpr (VEC) {
+    if constexpr (VEC || ELEM) {
       Raw w;
       T* e = (T*)w.r;
-      if (IL && rotates) {
+      if (VEC && IL && rotates) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) { e[2 * j] = Cvt<T>::from_f32(v[j]); e[2 * j + 1] = Cvt<T>::from_f32(v[8 + j]); }
       } else {
@@ -134,7 +149,8 @@ struct Own {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < NR / 2; ++i) *(raw_t*)(base + run(p, l, h) + i * VN) = w.r[h * (NR / 2) + i];
+        for (int i = 0; i < NR / 2; ++i)
+          if (!ELEM || run(p, l, h) < p.d) *(raw_t*)(base + run(p, l, h) + i * VN) = w.r[h * (NR / 2) + i];
     } else {
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
@@ -190,6 +206,36 @@ __device__ __forceinline__ void turn(float (&v)[16], const float2* cs, int valid
   }
 }
 
+// The turn of elements 16 l + j.  The other halves come from `mine`, the wave's own piece of LDS: [16][64 lanes], no barrier.
+template <bool IL, int DIR>
+__device__ __forceinline__ void turn_elements(float (&v)[16], float* mine, const float2* cs, const RotParams& p, int l) {
+  const int np = p.rot >> 1, lane = threadIdx.x & 63, e0 = 16 * l;
+  float other[16];
+  if constexpr (IL) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) other[j] = v[j ^ 1];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) mine[j * 64 + lane] = v[j];
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int e = e0 + j, o = e < np ? e + np : e < p.rot ? e - np : e;
+      other[j] = mine[(o & 15) * 64 + lane - l + (o >> 4)];
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const int e = e0 + j;
+    if (e < p.rot) {
+      const float2 t = cs[IL ? e >> 1 : e < np ? e : e - np];
+      const bool first = IL ? !(j & 1) : e < np;
+      v[j] = v[j] * t.x + (first == (DIR > 0) ? -other[j] : other[j]) * t.y;
+    }
+  }
+}
+
 // item e of a group: token and head (rows and heads are addressed from the group's first token)
 struct Item { int t, head; bool on; };
 __device__ __forceinline__ Item item_of(const RotParams& p, const Side& s, int e, int n, int lanes, int lshift) {
@@ -201,14 +247,16 @@ __device__ __forceinline__ Item item_of(const RotParams& p, const Side& s, int e
   return it;
 }
 
-template <typename T, bool NORM, bool IL, bool VEC>
+template <typename T, bool NORM, bool IL, Deal DEAL>
 __global__ __launch_bounds__(256) void qk_rotary_kernel(RotParams p) {
-  typedef Own<T, IL, VEC> O;
+  typedef Own<T, IL, DEAL> O;
   __shared__ float2 cs[ANGLES];
+  __shared__ float other[O::ELEM && !IL ? 4 * 1024 : 1];
+  float* mine = other + (O::ELEM && !IL ? (threadIdx.x >> 6) * 1024 : 0);
   const bool keys = (int)blockIdx.x >= p.side[0].blocks;
   const Side s = p.side[keys];
   const int blk = (int)blockIdx.x - (keys ? p.side[0].blocks : 0);
-  const int np = p.rot >> 1, nrl = (np + 7) >> 3, lanes = nrl + ((p.d - p.rot + 15) >> 4);
+  const int np = p.rot >> 1, nrl = (np + 7) >> 3, lanes = O::lanes(p);
   const int lshift = __ffs(p.lph) - 1;
   const int l = threadIdx.x & (p.lph - 1);     // the same for every item of the thread: width and 256 are multiples of lph
   const bool rotates = l < nrl;
@@ -243,7 +291,8 @@ __global__ __launch_bounds__(256) void qk_rotary_kernel(RotParams p) {
         for (int j = 0; j < 16; ++j) v[j] = v[j] * rstd * gm[j];
       }
       if (it.on) {
-        if (rotates) turn<1>(v, cs + it.t * np + 8 * l, VEC ? 8 : valid);
+        if constexpr (O::ELEM) turn_elements<IL, 1>(v, mine, cs + it.t * np, p, l);
+        else if (rotates) turn<1>(v, cs + it.t * np + 8 * l, O::VEC ? 8 : valid);
         O::store(out + it.t * s.ldo + it.head * p.d, v, p, l, rotates);
       }
     }
@@ -253,15 +302,20 @@ __global__ __launch_bounds__(256) void qk_rotary_kernel(RotParams p) {
 // Backward of norm and rotation.  dgamma: every thread sums its own elements of the head over the items it meets, then
 // lanes with the same elements, the waves and (second kernel) the blocks are added in a fixed order: no atomics, results
 // do not change from run to run.
-template <typename T, bool IL, bool VEC>
-__global__ __launch_bounds__(256, 4) void qk_norm_rotary_bwd_kernel(RotParams p) {
-  typedef Own<T, IL, VEC> O;
+// Waves per SIMD: halves of pairs fetched through LDS need 164 registers (8629 rows of 24 fp32 heads of 128, forward and
+// backward: with four waves and 39 registers spilled 191 us, with three 141); element by element four are better (6896 rows
+// of 24 bf16 heads of 80, 40 of them turned: 58 us, with three 65).
+template <typename T, bool IL, Deal DEAL>
+__global__ __launch_bounds__(256, DEAL == ELEMENTS && !IL ? 3 : 4) void qk_norm_rotary_bwd_kernel(RotParams p) {
+  typedef Own<T, IL, DEAL> O;
   __shared__ float2 cs[ANGLES];
   __shared__ float red[4][MAX_D];
+  __shared__ float other[O::ELEM && !IL ? 4 * 1024 : 1];
+  float* mine = other + (O::ELEM && !IL ? (threadIdx.x >> 6) * 1024 : 0);
   const bool keys = (int)blockIdx.x >= p.side[0].blocks;
   const Side s = p.side[keys];
   const int blk = (int)blockIdx.x - (keys ? p.side[0].blocks : 0);
-  const int np = p.rot >> 1, nrl = (np + 7) >> 3, lanes = nrl + ((p.d - p.rot + 15) >> 4);
+  const int np = p.rot >> 1, nrl = (np + 7) >> 3, lanes = O::lanes(p);
   const int lshift = __ffs(p.lph) - 1;
   const int l = threadIdx.x & (p.lph - 1);
   const bool rotates = l < nrl;
@@ -292,7 +346,8 @@ __global__ __launch_bounds__(256, 4) void qk_norm_rotary_bwd_kernel(RotParams p)
       O::unpack(g, rd, rotates);
       float ss = 0.f, sg = 0.f;
       if (it.on) {
-        if (rotates) turn<-1>(g, cs + it.t * np + 8 * l, VEC ? 8 : valid);
+        if constexpr (O::ELEM) turn_elements<IL, -1>(g, mine, cs + it.t * np, p, l);
+        else if (rotates) turn<-1>(g, cs + it.t * np + 8 * l, O::VEC ? 8 : valid);
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           ss += v[j] * (v[j] * inv_d);
@@ -319,7 +374,7 @@ __global__ __launch_bounds__(256, 4) void qk_norm_rotary_bwd_kernel(RotParams p)
   if (lane < p.lph && l < lanes) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) {   // (sums are in pair order whatever the storage order)
-      const int i = Own<T, IL, false>::index(p, l, j);
+      const int i = O::index(p, l, j);
       if (i >= 0) red[wave][i] = acc[j];
     }
   }
@@ -361,8 +416,8 @@ __global__ __launch_bounds__(1024) void dgamma_sum_kernel(const float* __restric
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // Lanes per head, tokens per group and blocks of each side; `most`: blocks of both sides.
-void plan(RotParams& p, int n_head, int n_kv, int rounds, int64_t most) {
-  const int np = p.rot / 2, lanes = (np + 7) / 8 + (p.d - p.rot + 15) / 16;
+void plan(RotParams& p, Deal deal, int n_head, int n_kv, int rounds, int64_t most) {
+  const int np = p.rot / 2, lanes = deal == ELEMENTS ? (p.d + 15) / 16 : (np + 7) / 8 + (p.d - p.rot + 15) / 16;
   p.lph = 1;
   while (p.lph < lanes) p.lph *= 2;
   for (int i = 0; i < 2; ++i) {
@@ -382,28 +437,36 @@ void plan(RotParams& p, int n_head, int n_kv, int rounds, int64_t most) {
   }
 }
 
-template <typename T, bool NORM>
-void launch_fwd(const RotParams& p, bool il, bool vec, hipStream_t stream) {
+template <typename T, bool NORM, bool IL>
+void launch_fwd(const RotParams& p, Deal deal, hipStream_t stream) {
   const dim3 grid((unsigned)(p.side[0].blocks + p.side[1].blocks));
-  if (il) {
-    if (vec) hipLaunchKernelGGL((qk_rotary_kernel<T, NORM, true, true>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((qk_rotary_kernel<T, NORM, true, false>), grid, dim3(256), 0, stream, p);
-  } else {
-    if (vec) hipLaunchKernelGGL((qk_rotary_kernel<T, NORM, false, true>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((qk_rotary_kernel<T, NORM, false, false>), grid, dim3(256), 0, stream, p);
-  }
+  if (deal == PAIRS) hipLaunchKernelGGL((qk_rotary_kernel<T, NORM, IL, PAIRS>), grid, dim3(256), 0, stream, p);
+  else if (deal == ELEMENTS) hipLaunchKernelGGL((qk_rotary_kernel<T, NORM, IL, ELEMENTS>), grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((qk_rotary_kernel<T, NORM, IL, SCALARS>), grid, dim3(256), 0, stream, p);
+}
+template <typename T>
+void launch_fwd(const RotParams& p, bool norm, bool il, Deal deal, hipStream_t stream) {
+  if (norm && il) launch_fwd<T, true, true>(p, deal, stream);
+  else if (norm) launch_fwd<T, true, false>(p, deal, stream);
+  else if (il) launch_fwd<T, false, true>(p, deal, stream);
+  else launch_fwd<T, false, false>(p, deal, stream);
 }
 
-template <typename T>
-void launch_bwd(const RotParams& p, bool il, bool vec, hipStream_t stream) {
+template <typename T, bool IL>
+void launch_bwd(const RotParams& p, Deal deal, hipStream_t stream) {
   const dim3 grid((unsigned)(p.side[0].blocks + p.side[1].blocks));
-  if (il) {
-    if (vec) hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, true, true>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, true, false>), grid, dim3(256), 0, stream, p);
-  } else {
-    if (vec) hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, false, true>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, false, false>), grid, dim3(256), 0, stream, p);
-  }
+  if (deal == PAIRS) hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, IL, PAIRS>), grid, dim3(256), 0, stream, p);
+  else if (deal == ELEMENTS) hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, IL, ELEMENTS>), grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<T, IL, SCALARS>), grid, dim3(256), 0, stream, p);
+}
+template <typename T>
+void launch_bwd(const RotParams& p, bool il, Deal deal, hipStream_t stream) {
+  if (il) launch_bwd<T, true>(p, deal, stream);
+  else launch_bwd<T, false>(p, deal, stream);
+}
+
+Deal deal_of(bool rows16, int d, int rot) {
+  return !rows16 || d % 8 ? SCALARS : d % 16 == 0 && rot % 16 == 0 ? PAIRS : ELEMENTS;
 }
 
 int check_shape(const char* who, const int64_t* pos, const uint64_t* turns, int64_t T, int n_head, int n_kv, int d, int rot,
@@ -442,15 +505,10 @@ extern "C" int skhip_qk_rotary(const void* q, const void* k, void* q_out, void* 
   const int64_t per = dtype == SK_BF16 ? 8 : 4;
   bool vec = aligned16(q) && aligned16(q_out) && (ldq | ldq_out) % per == 0;
   if (n_kv) vec = vec && aligned16(k) && aligned16(k_out) && (ldk | ldk_out) % per == 0;
-  vec = vec && rot % 16 == 0 && d % 16 == 0;
-  plan(p, n_head, n_kv, gamma_q ? 2 : 1, (int64_t)sk_num_cus() * 64);
-  if (dtype == SK_BF16) {
-    if (gamma_q) launch_fwd<bf16_t, true>(p, interleaved, vec, stream);
-    else launch_fwd<bf16_t, false>(p, interleaved, vec, stream);
-  } else {
-    if (gamma_q) launch_fwd<float, true>(p, interleaved, vec, stream);
-    else launch_fwd<float, false>(p, interleaved, vec, stream);
-  }
+  const Deal deal = deal_of(vec, d, rot);
+  plan(p, deal, n_head, n_kv, gamma_q ? 2 : 1, (int64_t)sk_num_cus() * 64);
+  if (dtype == SK_BF16) launch_fwd<bf16_t>(p, gamma_q, interleaved, deal, stream);
+  else launch_fwd<float>(p, gamma_q, interleaved, deal, stream);
   SK_CHECK_LAUNCH(who);
   return SK_OK;
 }
@@ -478,8 +536,8 @@ extern "C" int skhip_qk_norm_rotary_bwd(const void* q, const void* k, const void
   const int64_t per = dtype == SK_BF16 ? 8 : 4;
   bool vec = aligned16(q) && aligned16(dq_out) && aligned16(dq) && (ldq | lddq_out | lddq) % per == 0;
   if (n_kv) vec = vec && aligned16(k) && aligned16(dk_out) && aligned16(dk) && (ldk | lddk_out | lddk) % per == 0;
-  vec = vec && rot % 16 == 0 && d % 16 == 0;
-  plan(p, n_head, n_kv, 2, BWD_BLOCKS);
+  const Deal deal = deal_of(vec, d, rot);
+  plan(p, deal, n_head, n_kv, 2, BWD_BLOCKS);
   const int64_t need = (int64_t)(sq.blocks + sk.blocks) * d;
   if (need > 0 && (!workspace || workspace_floats < need)) {
     sk_set_error("%s: workspace of %lld floats needed", who, (long long)need);
@@ -488,8 +546,8 @@ extern "C" int skhip_qk_norm_rotary_bwd(const void* q, const void* k, const void
   sq.partial = workspace;
   sk.partial = workspace + (int64_t)sq.blocks * d;
   if (T > 0) {
-    if (dtype == SK_BF16) launch_bwd<bf16_t>(p, interleaved, vec, stream);
-    else launch_bwd<float>(p, interleaved, vec, stream);
+    if (dtype == SK_BF16) launch_bwd<bf16_t>(p, interleaved, deal, stream);
+    else launch_bwd<float>(p, interleaved, deal, stream);
     SK_CHECK_LAUNCH(who);
   }
   hipLaunchKernelGGL(dgamma_sum_kernel, dim3((d + 15) / 16, n_kv ? 2 : 1), dim3(1024), 0, stream, sq.partial, sk.partial, dgamma_q,

@@ -60,7 +60,7 @@ def rotary_case(T, H, G, d, rot, dtype, il, far, gen, **kw):
 
 SHAPES = [  # T, H, G, d, rot
     (1, 1, 1, 64, 64), (640, 8, 8, 64, 64), (37, 8, 2, 128, 64), (5, 3, 1, 80, 80), (19, 4, 4, 96, 48), (1030, 2, 1, 32, 32),
-    (7, 5, 5, 37, 18), (3, 2, 2, 256, 256), (66, 16, 16, 16, 2), (2, 40, 8, 128, 128), (9, 1, 1, 3, 2), (8, 512, 512, 64, 30)]
+    (700, 4, 2, 64, 36), (33, 3, 1, 72, 40), (9, 2, 2, 96, 86), (50, 2, 1, 24, 6), (21, 1, 1, 248, 130), (300, 4, 1, 128, 2), (7, 5, 5, 37, 18), (3, 2, 2, 256, 256), (66, 16, 16, 16, 2), (2, 40, 8, 128, 128), (9, 1, 1, 3, 2), (8, 512, 512, 64, 30)]
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
@@ -108,6 +108,13 @@ def test_rotary_reads_slices_and_odd_strides(dtype):
         assert torch.equal(got, want), off
     got, _ = ops.rotary(x.t().contiguous().t(), None, pos, f, H)
     assert torch.equal(got, want)
+    part = ops.RotaryFrequencies(36, device=DEV)   # halves of a pair with different lanes, or element by element
+    for il in (False, True):
+        want36, _ = ops.rotary(x, None, pos, part, H, interleaved=il)
+        for off in (8, 1):
+            wide[:, off:off + H * d] = x
+            got, _ = ops.rotary(wide[:, off:off + H * d], None, pos, part, H, interleaved=il)
+            assert torch.equal(got, want36), (il, off)
     one, _ = ops.rotary(x[:1].expand(T, -1), None, pos, f, H)
     assert torch.equal(one, ops.rotary(x[:1].repeat(T, 1), None, pos, f, H)[0])
 
