@@ -26,7 +26,7 @@ struct StepParams {
   const int32_t* len;
   float* part;              // [R][H][splits][d + 2]: weighted values, maximum, sum
   int64_t ldq, ldn, ldo, ks, kp, vs, vp;   // strides: sequence (s) and position (p) of the caches
-  int R, H, G, d, cap, window, sinks, splits, per;   // per: visible positions of a split
+  int R, H, G, d, cap, window, sinks, splits;
   float scale;
 };
 
@@ -38,6 +38,11 @@ struct Visible {
     lo = max(0, n - p.window);
     ns = min(p.sinks, lo);
     count = ns + (n - lo);
+  }
+  // Positions of a split: the sequence's own, shared out evenly, `unit` at a time and four units at least, so that a short
+  // sequence in a batch planned for long ones is spread as widely.
+  __device__ __forceinline__ int per_split(const StepParams& p, int unit) const {
+    return max(4 * unit, (count + p.splits * unit - 1) / (p.splits * unit) * unit);
   }
   __device__ __forceinline__ int pos(int u) const { return u < ns ? u : lo + (u - ns); }
   __device__ __forceinline__ int slot(const StepParams& p, int j) const {
@@ -60,8 +65,8 @@ __global__ __launch_bounds__(256) void step_kernel(StepParams p, int vec) {
   const T* vn = p.vn ? (const T*)p.vn + r * p.ldn + (int64_t)kh * p.d : nullptr;
   const bool writer = h % rep == 0;
   float m = -INFINITY, l = 0.f, a0 = 0.f, a1 = 0.f;
-  const int u_end = min(vis.count, (split + 1) * p.per);
-  for (int u0 = split * p.per + wave * KT; u0 < u_end; u0 += 4 * KT) {
+  const int per = vis.per_split(p, KT), u_end = min(vis.count, (split + 1) * per);
+  for (int u0 = split * per + wave * KT; u0 < u_end; u0 += 4 * KT) {
     const int u = u0 + lane;
     const bool on = u < u_end;
     int64_t row = 0;
@@ -225,7 +230,7 @@ __global__ __launch_bounds__(256, 2) void step_mfma_kernel(StepParams p, int chu
   const int r = blockIdx.z, kh = blockIdx.y / chunks, hc = blockIdx.y - kh * chunks, split = blockIdx.x;
   const int rep = p.H / p.G, h0 = kh * rep + hc * HEADS, nh = min(HEADS, rep - hc * HEADS);
   const Visible vis(p, r);
-  const int u_beg = split * p.per, u_end = min(vis.count, u_beg + p.per);
+  const int per = vis.per_split(p, MT), u_beg = split * per, u_end = min(vis.count, u_beg + per);
   T* K = (T*)p.kc + r * p.ks + (int64_t)kh * p.d;
   T* V = (T*)p.vc + r * p.vs + (int64_t)kh * p.d;
   const T* kn = p.kn ? (const T*)p.kn + r * p.ldn + (int64_t)kh * p.d : nullptr;
@@ -426,8 +431,7 @@ void plan(StepParams& p, bool mfma, int dtype) {
   if (uneven(s))
     for (int64_t t = s + 1; t <= std::min<int64_t>(MAX_SPLITS, units / 16) && t * blocks <= 8 * cus; ++t)
       if (!uneven(t)) { s = t; break; }
-  p.per = (int)(per(s) * unit);
-  p.splits = (int)((most + p.per - 1) / p.per);
+  p.splits = (int)((units + per(s) - 1) / per(s));
 }
 
 int64_t ws_floats(const StepParams& p) { return p.splits > 1 ? (int64_t)p.R * p.H * p.splits * (p.d + 2) : 0; }
