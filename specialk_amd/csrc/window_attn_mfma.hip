@@ -157,10 +157,17 @@ __device__ __forceinline__ float keep_or(float v, uint32_t m, uint32_t other) {
 }
 
 // ------------------------------------------------------------------------------ forward
-// Bound by the vector ALU: a 32 x 32 score tile costs 8 (d = 64) or 16 (d = 128) matrix instructions of 32 cycles and 16
-// exponentials of 16 cycles plus some five full-rate instructions per register.  The scale goes into the exponent's
+// Bound by matrix and vector unit together: a 32 x 32 score tile costs 8 (d = 64) or 16 (d = 128) matrix instructions of 32
+// cycles and some 100 vector instructions, 16 of them exponentials, and the two units' busy times add up to all of the
+// kernel's (50 + 52 % at d = 128, 34 + 71 % at 64).  Dealing the matrix instructions out among the vector ones (scores of
+// the next half tile beside the probabilities of this one) does not help: the chip, at 1.8 of 2.4 GHz in this kernel, is
+// held by power as well (32771 tokens of 32 / 8 heads of 128, window 4096: 2.05 ms, 1000 TFLOP/s; so dealt 2.2; a product of
+// two 8192 x 8192 matrices reaches 1214).  So the arithmetic itself is kept small: the scale goes into the exponent's
 // multiply-add, and the accumulators are rescaled only when a row's maximum has grown by more than 2^8 since the last
 // time: until then probabilities stay below 256, which bf16 holds as precisely as values below one.
+// Small windows are bound by the rows' way from memory instead: 256 packed sentences of 3 - 400 tokens, 8 heads of 64,
+// window 64 both ways: 61 us (3.4 TB/s of q, k, v, o), dQ 95 (3.4), dK and dV 98 (3.2), half of it waiting, at 2.2 waves a
+// SIMD; a third tile buffer, a sentence's tiles closer together and earlier first loads changed nothing.
 template <int D, int W>
 __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void fwd_kernel(WinParams p, int qtiles) {
   __shared__ __attribute__((aligned(1024))) char lds[2][2 * tile_bytes<D>()];
