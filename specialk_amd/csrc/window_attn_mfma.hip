@@ -256,7 +256,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void fwd_kernel(WinParams p, 
     for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[1][r]);
     mx = other_max(mx);
     if (__any((mx - m) * cs > 8.f)) {   // (also from -inf; both -inf: NaN, no)
-      const float mn = fmaxf(m, mx);
+      const float mn = m == -INFINITY || (mx - m) * cs > 8.f ? fmaxf(m, mx) : m;   // (a row's own scores decide, not its neighbours')
       const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mn) * cs);
       m = mn;
       l *= alpha;

@@ -751,6 +751,11 @@ def test_nan_query_stays_in_its_row(d, dtype):
     assert got[77, d:].isnan().all()
     got[77, d:] = want[77, d:]
     assert torch.equal(got, want)
+    big = q.clone()   # nor do large scores change what other rows get, to the last bit
+    big[77] *= 300
+    got = ops.window_attention(big, k, v, 1, n, n, H, None, 40, 2)
+    got[77] = want[77]
+    assert torch.equal(got, want)
     # one step, one split and several, with positions in one split only and in all
     for cap, lens in ((64, [1, 60, 64]), (6000, [1, 50, 5000])):
         kc, vc = rnd((3, cap, H * d), dtype, g).to(DEV), rnd((3, cap, H * d), dtype, g).to(DEV)
