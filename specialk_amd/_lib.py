@@ -337,12 +337,17 @@ def on_device(t):
     return _same_device if t.device.index == here else torch.cuda.device(t.device)
 
 
+def _fresh(x):
+    """Uninitialised contiguous rows of x's shape and type."""
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+
+
 def qk_rotary(q, k, pos, turns, amplitude, gamma_q, gamma_k, eps, n_head, n_kv, d, rot, interleaved, inverse=False):
     """(q', k') of the rows q (T, n_head * d) and k (T, n_kv * d) or None; gamma_q / gamma_k None: no norm."""
     lib = load()
     T = q.shape[0]
-    qo = q.new_empty((T, n_head * d))
-    ko = None if k is None else k.new_empty((T, n_kv * d))
+    qo = _fresh(q)
+    ko = None if k is None else _fresh(k)
     rc = lib.skhip_qk_rotary(_ptr(q), _ptr(k), _ptr(qo), _ptr(ko), _ptr(pos), _ptr(turns), float(amplitude), _ptr(gamma_q),
                              _ptr(gamma_k), float(eps), T, n_head, 0 if k is None else n_kv, d, rot, q.stride(0),
                              0 if k is None else k.stride(0), n_head * d, n_kv * d, int(interleaved), int(inverse),
@@ -355,8 +360,8 @@ def qk_norm_rotary_bwd(q, k, dqo, dko, pos, turns, amplitude, gamma_q, gamma_k, 
     """(dq, dk, dgamma_q, dgamma_k) from the inputs of qk_rotary and its output gradients."""
     lib = load()
     T, dev = q.shape[0], q.device
-    dq = q.new_empty((T, n_head * d))
-    dk = None if k is None else torch.empty((T, n_kv * d), dtype=k.dtype, device=dev)
+    dq = _fresh(q)
+    dk = None if k is None else _fresh(k)
     dgq = torch.empty(d, dtype=torch.float32, device=dev)
     dgk = None if k is None else torch.empty(d, dtype=torch.float32, device=dev)
     n = int(lib.skhip_qk_norm_rotary_bwd_ws_floats(d))
@@ -374,7 +379,7 @@ def qk_norm_rotary_bwd(q, k, dqo, dko, pos, turns, amplitude, gamma_q, gamma_k, 
 def window_attn_fwd(q, k, v, B, Lq, Lk, n_head, n_kv, d, scale, window, sinks, causal, key_pad=None, q_off=None, k_off=None):
     """(o (Tq, n_head * d), lse fp32 (n_head, Tq))."""
     lib = load()
-    o = q.new_empty((q.shape[0], n_head * d))
+    o = _fresh(q)
     lse = torch.empty((n_head, q.shape[0]), dtype=torch.float32, device=q.device)
     rc = lib.skhip_window_attn_fwd(_ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse), _ptr(key_pad), _ptr(q_off), _ptr(k_off), B,
                                    n_head, n_kv, q.shape[0], k.shape[0], Lq, Lk, d, q.stride(0), k.stride(0), v.stride(0),
@@ -387,9 +392,7 @@ def window_attn_bwd(q, k, v, o, do, lse, B, Lq, Lk, n_head, n_kv, d, scale, wind
                     k_off=None):
     """(dq, dk, dv), contiguous."""
     lib = load()
-    dq = q.new_empty((q.shape[0], n_head * d))
-    dk = k.new_empty((k.shape[0], n_kv * d))
-    dv = k.new_empty((k.shape[0], n_kv * d))
+    dq, dk, dv = _fresh(q), _fresh(k), _fresh(v)
     n = int(lib.skhip_window_attn_bwd_ws_floats(B, n_head, n_kv, q.shape[0], Lq, Lk, d, window, sinks, int(causal)))
     ws = torch.empty(n, dtype=torch.float32, device=q.device)
     rc = lib.skhip_window_attn_bwd(_ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(do), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv),
@@ -409,7 +412,7 @@ def window_attn_step(q, k_new, v_new, k_cache, v_cache, kv_len, n_head, n_kv, d,
     """o (R, n_head * d); k_new / v_new (R, n_kv * d; one row stride) or None; caches (R, cap, n_kv * d), written in place."""
     lib = load()
     R, cap, _ = k_cache.shape
-    o = q.new_empty((R, n_head * d))
+    o = _fresh(q)
     n = _step_ws(R, n_head, n_kv, d, cap, window, sinks)
     ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
     rc = lib.skhip_window_attn_step(_ptr(q), _ptr(k_new), _ptr(v_new), _ptr(k_cache), _ptr(v_cache), _ptr(o), _ptr(kv_len), R,
