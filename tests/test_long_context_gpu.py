@@ -770,6 +770,28 @@ def test_nan_query_stays_in_its_row(d, dtype):
             assert torch.equal(got, want), (cap, r)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("d", [64, 37])
+def test_query_gradient_depends_on_its_own_row(d, dtype):
+    """Other queries and output gradients change nothing in a row of dQ, to the last bit."""
+    g = torch.Generator().manual_seed(19)
+    n, H = 150, 2
+    q, k, v, do = (rnd((n, H * d), dtype, g).to(DEV) for _ in range(4))
+
+    def dq(q, do):
+        leaf = q.clone().requires_grad_()
+        return torch.autograd.grad(ops.window_attention(leaf, k, v, 1, n, n, H, None, 60, 1), leaf, do)[0]
+
+    want = dq(q, do)
+    q2, do2 = q.clone(), do.clone()
+    q2[40:44] *= 100
+    do2[3] = 1000
+    got = dq(q2, do2)
+    for r in (3, 40, 41, 42, 43):
+        got[r] = want[r]
+    assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("scale", [0.0, 1e-35, -0.2])
 def test_window_scales(scale):
     """A scale of nothing and next to it (every visible key counts alike), and a negative one."""
