@@ -208,7 +208,8 @@ int skhip_qk_norm_rotary_bwd(const void* q, const void* k, const void* dq_out, c
  * Rows as in skhip_attn_fwd: padded (row b*Lq + i; Tq = B*Lq, Tk = B*Lk) or, with q_off and k_off (int32 [B+1], no
  * key_pad), packed, Lq and Lk then being at least the longest lengths; rows of a packed tensor outside every sequence get
  * zeros in O, dQ, dK and dV.  LSE fp32 [n_head][Tq] receives the log-sum-exp of the scaled visible scores.
- * Backward writes dQ, dK, dV; workspace: skhip_window_attn_bwd_ws_floats() floats.  Fixed summation orders.
+ * Backward writes dQ, dK, dV.  Workspaces: skhip_window_attn_fwd_ws_floats() (0 unless few rows see many keys) and
+ * skhip_window_attn_bwd_ws_floats() floats, 16-byte aligned.  Fixed summation orders.
  *
  * skhip_window_attn_step: the causal form for ONE new query per sequence against a cache.  kv_len[r] positions, the new
  * one included, the last of which is the query's.  Position j lives in slot  j < sinks ? j : sinks + (j - sinks) %
@@ -216,10 +217,13 @@ int skhip_qk_norm_rotary_bwd(const void* q, const void* k, const void* dq_out, c
  * position, one with cap = sinks + window is a ring of what can still be seen.  cap - sinks >= window.  k_new, v_new
  * (optional, [R][ld_new]): the newest position's key and value, which this call uses and stores in its slot.
  * kv_len[r] <= 0: zeros, nothing stored.  workspace: skhip_window_attn_step_ws_floats() floats (may be 0).       */
+int64_t skhip_window_attn_fwd_ws_floats(int B, int n_head, int n_kv, int64_t Tq, int Lq, int Lk, int d, int window,
+                                        int sinks, int causal);
 int skhip_window_attn_fwd(const void* Q, const void* K, const void* V, void* O, float* LSE, const uint8_t* key_pad,
                           const int32_t* q_off, const int32_t* k_off, int B, int n_head, int n_kv, int64_t Tq,
                           int64_t Tk, int Lq, int Lk, int d, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo,
-                          float scale, int window, int sinks, int causal, int dtype, void* stream);
+                          float scale, int window, int sinks, int causal, float* workspace, int64_t workspace_floats,
+                          int dtype, void* stream);
 int64_t skhip_window_attn_bwd_ws_floats(int B, int n_head, int n_kv, int64_t Tq, int Lq, int Lk, int d, int window,
                                         int sinks, int causal);
 int skhip_window_attn_bwd(const void* Q, const void* K, const void* V, const void* O, const void* dO, const float* LSE,

@@ -29,7 +29,7 @@ EXPORTS = [
     "skhip_softmax_rows", "skhip_conv_windows", "skhip_cnn_head", "skhip_collate", "skhip_set_reserved_cus",
     "skhip_rowpanel_rows", "skhip_rowpanel_pattern_bytes", "skhip_rowpanel_set_stamps", "skhip_rowpanel_gemm", "skhip_rowpanel_gemm_ln",
     "skhip_qk_rotary", "skhip_qk_norm_rotary_bwd_ws_floats", "skhip_qk_norm_rotary_bwd",
-    "skhip_window_attn_fwd", "skhip_window_attn_bwd_ws_floats", "skhip_window_attn_bwd",
+    "skhip_window_attn_fwd_ws_floats", "skhip_window_attn_fwd", "skhip_window_attn_bwd_ws_floats", "skhip_window_attn_bwd",
     "skhip_window_attn_step_ws_floats", "skhip_window_attn_step",
     "skhip_generator_chunk_cols", "skhip_generator_rowstats", "skhip_beam_backtrack",
 ]
@@ -101,7 +101,9 @@ def load():
     lib.skhip_qk_norm_rotary_bwd.argtypes = ([c_p] * 10 + [c_f32, c_p, c_p, c_f32, c_i64] + [c_int] * 4 + [c_i64] * 6 +
                                              [c_int, c_p, c_i64, c_int, c_p])
     lib.skhip_window_attn_fwd.argtypes = ([c_p] * 8 + [c_int] * 3 + [c_i64] * 2 + [c_int] * 3 + [c_i64] * 4 +
-                                          [c_f32] + [c_int] * 4 + [c_p])
+                                          [c_f32] + [c_int] * 3 + [c_p, c_i64, c_int, c_p])
+    lib.skhip_window_attn_fwd_ws_floats.argtypes = [c_int] * 3 + [c_i64] + [c_int] * 6
+    lib.skhip_window_attn_fwd_ws_floats.restype = c_i64
     lib.skhip_window_attn_bwd_ws_floats.argtypes = [c_int] * 3 + [c_i64] + [c_int] * 6
     lib.skhip_window_attn_bwd_ws_floats.restype = c_i64
     lib.skhip_window_attn_bwd.argtypes = ([c_p] * 12 + [c_int] * 3 + [c_i64] * 2 + [c_int] * 3 + [c_i64] * 8 +
@@ -376,14 +378,21 @@ def qk_norm_rotary_bwd(q, k, dqo, dko, pos, turns, amplitude, gamma_q, gamma_k, 
 
 
 # --------------------------------------------------------------------------- attention within a window
+@functools.lru_cache(maxsize=256)
+def _fwd_ws(*sizes):
+    return int(load().skhip_window_attn_fwd_ws_floats(*sizes))
+
+
 def window_attn_fwd(q, k, v, B, Lq, Lk, n_head, n_kv, d, scale, window, sinks, causal, key_pad=None, q_off=None, k_off=None):
     """(o (Tq, n_head * d), lse fp32 (n_head, Tq))."""
     lib = load()
     o = _fresh(q)
     lse = torch.empty((n_head, q.shape[0]), dtype=torch.float32, device=q.device)
+    n = _fwd_ws(B, n_head, n_kv, q.shape[0], Lq, Lk, d, window, sinks, int(causal))
+    ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
     rc = lib.skhip_window_attn_fwd(_ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse), _ptr(key_pad), _ptr(q_off), _ptr(k_off), B,
                                    n_head, n_kv, q.shape[0], k.shape[0], Lq, Lk, d, q.stride(0), k.stride(0), v.stride(0),
-                                   n_head * d, float(scale), window, sinks, int(causal), dcode(q.dtype), _stream())
+                                   n_head * d, float(scale), window, sinks, int(causal), _ptr(ws), n, dcode(q.dtype), _stream())
     _check(rc, "skhip_window_attn_fwd")
     return o, lse
 

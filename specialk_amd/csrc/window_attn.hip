@@ -158,14 +158,17 @@ template <typename T, int D> struct KeySweep {
   const T *K, *V;
   const uint8_t* pad;
   Stage<T, D> k, v;
-  int gone;
-  __device__ __forceinline__ KeySweep(const WinParams& p_, const Seq& sq_, int b, int kh, int i0)
+  int gone, beg, end;
+  // the `cut`-th of `cuts` shares of the tiles that queries i0 .. i0 + 63 see
+  __device__ __forceinline__ KeySweep(const WinParams& p_, const Seq& sq_, int b, int kh, int i0, int cut = 0, int cuts = 1)
       : p(p_), sq(sq_), kt(KeyTiles::of<NT>(p_, sq_, i0, min(i0 + 64, sq_.Lq))) {
+    beg = (int)((int64_t)max(0, kt.n) * cut / cuts);
+    end = (int)((int64_t)max(0, kt.n) * (cut + 1) / cuts);
     K = (const T*)p.K + sq.kbase * p.ldk + (int64_t)kh * p.d;
     V = (const T*)p.V + sq.kbase * p.ldv + (int64_t)kh * p.d;
     pad = p.key_pad ? p.key_pad + (int64_t)b * p.Lk : nullptr;
     gone = 0;
-    if (kt.n > 0) load(0);
+    if (beg < end) load(beg);
   }
   __device__ __forceinline__ int start(int t) const { return kt.start<NT>(t); }
   __device__ __forceinline__ void load(int t) {
@@ -181,7 +184,7 @@ template <typename T, int D> struct KeySweep {
     k.store(Ks, ok, p.d);
     v.store(Vs, ok, p.d);
     __syncthreads();
-    if (t + 1 < kt.n) load(t + 1);
+    if (t + 1 < end) load(t + 1);
     return ok;
   }
 };
@@ -196,25 +199,25 @@ __global__ __launch_bounds__(256, BLOCKS(D)) void window_fwd_kernel(WinParams p)
   __shared__ __attribute__((aligned(16))) Tile<D> Vs;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
   const int qtiles = max(1, (p.Lq + 63) / 64);
-  const Work work = work_of_block(p, qtiles, p.H / p.G, true);
+  const Work work = work_of_block(p, qtiles * p.cuts, p.H / p.G, true);
   if (work.none) return;
-  const int b = work.b, h = work.h, kh = h / (p.H / p.G);
+  const int b = work.b, h = work.h, kh = h / (p.H / p.G), cut = work.tile % p.cuts;
   if (b == p.B) {   // packed: rows of no sequence
     zero_rest<T>((T*)p.Oout, p.ldo, (int64_t)h * p.d, p.d, p.q_off, p.B, p.Tq, work.tile, TAIL);
     return;
   }
   const Seq sq = seq_of(p, b);
-  const int i0 = work.tile * 64;
+  const int i0 = work.tile / p.cuts * 64;
   if (i0 >= sq.Lq) return;   // block-uniform
   const int i = i0 + wave * 16 + c, pos = i + sq.off;
-  KeySweep<T, D> keys(p, sq, b, kh, i0);
+  KeySweep<T, D> keys(p, sq, b, kh, i0, cut, p.cuts);
   f32x4_t fq[D / 16], o[D / 16];
   load_own<T, D>(fq, (const T*)p.Q + (sq.qbase + min(i, sq.Lq - 1)) * p.ldq + (int64_t)h * p.d, p.d, g, i < sq.Lq);
 #pragma unroll
   for (int t = 0; t < D / 16; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   const float cs = p.scale * LOG2E;   // scores in units of log 2: exp2 is one instruction, exp a dozen
   float m = -INFINITY, l = 0.f;
-  for (int t = 0; t < keys.kt.n; ++t) {
+  for (int t = keys.beg; t < keys.end; ++t) {
     const uint64_t ok = keys.next(t, Ks, Vs), see = i < sq.Lq ? keys_seen(p, pos, keys.start(t), ok) : 0;
     const uint64_t mk = see >> (4 * g);
     f32x4_t sc[4];
@@ -247,6 +250,13 @@ __global__ __launch_bounds__(256, BLOCKS(D)) void window_fwd_kernel(WinParams p)
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (piece(see, k)) add_cols<D>(o, Vs, 16 * k, sc[k], lane);
+  }
+  if (p.cuts > 1) {
+    if (i >= sq.Lq) return;
+    const int64_t row = ((int64_t)cut * p.H + h) * p.Tq + sq.qbase + i;
+    store_own<float, D>(p.cut_o + row * p.d, o, 1.f, p.d, g);
+    if (g == 0) { p.cut_ml[2 * row] = m; p.cut_ml[2 * row + 1] = l; }
+    return;
   }
   if (i < sq.Lq) {
     store_own<T, D>((T*)p.Oout + (sq.qbase + i) * p.ldo + (int64_t)h * p.d, o, l > 0.f || l != l ? 1.f / l : 0.f, p.d, g);
@@ -445,6 +455,29 @@ __global__ __launch_bounds__(256) void window_split_join_kernel(WinParams p, int
   ((T*)p.dV)[(sq.kbase + j) * p.lddv + col] = Cvt<T>::from_f32(v);
 }
 
+// O and log-sum-exp of rows whose keys were cut: a thread per element.
+template <typename T>
+__global__ __launch_bounds__(256) void window_cut_join_kernel(WinParams p) {
+  const int b = blockIdx.y, width = p.H * p.d;
+  const Seq sq = seq_of(p, b);
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int i = (int)(e / width), col = (int)(e - (int64_t)i * width), h = col / p.d, c = col - h * p.d;
+  if (i >= sq.Lq) return;
+  const int64_t row = (int64_t)h * p.Tq + sq.qbase + i, step = (int64_t)p.H * p.Tq;
+  float m = -INFINITY, l = 0.f, o = 0.f;
+  for (int s = 0; s < p.cuts; ++s) m = fmaxf(m, p.cut_ml[2 * (row + s * step)]);
+#pragma unroll 4
+  for (int s = 0; s < p.cuts; ++s) {
+    const float2 ml = *(const float2*)&p.cut_ml[2 * (row + s * step)];
+    const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ml.x - m);   // (a sum of NaN scores has no maximum)
+    l += f * ml.y;
+    o += f * p.cut_o[(row + s * step) * p.d + c];
+  }
+  const bool some = l > 0.f || l != l;
+  ((T*)p.Oout)[(sq.qbase + i) * p.ldo + col] = Cvt<T>::from_f32(some ? o / l : 0.f);
+  if (c == 0) p.LSE[row] = l > 0.f ? m * LN2 + logf(l) : (some ? l : -INFINITY);
+}
+
 // whether every row of the operands that go through LDS is made of whole 4-element pieces
 bool whole_pieces(const WinParams& p, int dtype) {
   const int64_t size = dtype == SK_BF16 ? 2 : 4;
@@ -492,10 +525,22 @@ void plan_keys(WinParams& p, int rows) {
   p.nch = far ? (p.Lq + p.ch - 1) / p.ch : 0;
 }
 
+// Cuts of a query tile's keys: two blocks for every CU, each with at least 12 tiles of 64 keys (fp32 arithmetic: 8).  64
+// queries at the end of 32768 keys, 8 heads of 128, all visible: 8 blocks alone 649 us, cut 54 (fp32 4276 and 148); 4096
+// tokens, 4 heads of 64, causal: 74 and 41.  Shorter sweeps are not worth the join: 2048 tokens, 8 heads of 128, window 1024
+// (18 tiles): uncut 30, in two 38.
+void plan_cuts(WinParams& p, int rows) {
+  const int64_t blocks = std::max<int64_t>(1, (int64_t)p.B * p.H * ((p.Lq + rows - 1) / rows));
+  const int64_t tiles = std::min<int64_t>(p.Lk, (int64_t)rows + p.left + p.right + p.sinks) / 64;
+  p.cuts = (int)std::max<int64_t>(1, std::min({2 * (int64_t)sk_num_cus() / blocks, tiles / (rows == NT ? 8 : 12), (int64_t)64}));
+}
+int64_t cut_o_floats(const WinParams& p) { return ((int64_t)p.cuts * p.H * p.Tq * p.d + 3) / 4 * 4; }
+int64_t cut_floats(const WinParams& p) { return p.cuts > 1 ? cut_o_floats(p) + 2ll * p.cuts * p.H * p.Tq : 0; }
+
 // Grids of 256 threads a block whose threads are counted in 32 bits (tiles of 64 rows: the most that any kernel has).
 bool grids_fit(const WinParams& p) {
   const int64_t tiles = std::max(p.Lq, p.Lk) / 64 + 1, units = (int64_t)p.B * p.G + 7;
-  return units * tiles * (p.H / p.G) + TAIL * p.H < (1 << 24) && units * (tiles * p.parts + (int64_t)p.nst * p.nch) + TAIL * p.G < (1 << 24) &&
+  return units * tiles * std::max(1, p.cuts) * (p.H / p.G) + TAIL * p.H < (1 << 24) && units * (tiles * p.parts + (int64_t)p.nst * p.nch) + TAIL * p.G < (1 << 24) &&
          (p.nst == 0 || (int64_t)p.sinks * p.d < (1ll << 31));
 }
 
@@ -506,7 +551,7 @@ int64_t split_floats(const WinParams& p) { return p.parts > 1 ? 2ll * p.parts * 
 
 template <typename T, int D>
 void launch_fwd_at(const WinParams& p, hipStream_t stream) {
-  const dim3 grid(work_blocks(p, std::max(1, (p.Lq + 63) / 64), p.H / p.G));
+  const dim3 grid(work_blocks(p, std::max(1, (p.Lq + 63) / 64) * p.cuts, p.H / p.G));
   hipLaunchKernelGGL((window_fwd_kernel<T, D>), grid, dim3(256), 0, stream, p);
 }
 template <typename T, int D>
@@ -551,6 +596,28 @@ int sk_window_join(const WinParams& p, int rows, int dtype, hipStream_t stream) 
   return SK_OK;
 }
 
+int sk_window_cut_join(const WinParams& p, int dtype, hipStream_t stream) {
+  if (p.cuts == 1) return SK_OK;
+  const dim3 all((unsigned)(((int64_t)p.Lq * p.H * p.d + 255) / 256), p.B);
+  if (dtype == SK_BF16) hipLaunchKernelGGL((window_cut_join_kernel<bf16_t>), all, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((window_cut_join_kernel<float>), all, dim3(256), 0, stream, p);
+  SK_CHECK_LAUNCH("skhip_window_attn_fwd(join)");
+  return SK_OK;
+}
+
+extern "C" int64_t skhip_window_attn_fwd_ws_floats(int B, int n_head, int n_kv, int64_t Tq, int Lq, int Lk, int d, int window,
+                                                   int sinks, int causal) {
+  if (B < 0 || n_head <= 0 || n_kv <= 0 || Tq < 0 || Lq < 0 || Lk < 0 || d <= 0 || window < 1 || sinks < 0) return 0;
+  WinParams p = {};
+  p.B = B; p.H = n_head; p.G = n_kv; p.Tq = Tq; p.Lq = Lq; p.Lk = Lk; p.d = d; p.sinks = sinks;
+  set_window(p, window, causal);
+  // the larger of the two paths' needs: which one a call takes depends on its pointers and strides
+  plan_cuts(p, NT);
+  const int64_t plain = cut_floats(p);
+  plan_cuts(p, MFMA_ROWS);
+  return std::max(plain, cut_floats(p));
+}
+
 extern "C" int64_t skhip_window_attn_bwd_ws_floats(int B, int n_head, int n_kv, int64_t Tq, int Lq, int Lk, int d, int window,
                                                    int sinks, int causal) {
   if (B < 0 || n_head <= 0 || n_kv <= 0 || Tq < 0 || Lq < 0 || Lk < 0 || d <= 0 || window < 1 || sinks < 0) return 0;
@@ -567,7 +634,8 @@ extern "C" int64_t skhip_window_attn_bwd_ws_floats(int B, int n_head, int n_kv, 
 extern "C" int skhip_window_attn_fwd(const void* Q, const void* K, const void* V, void* O, float* LSE, const uint8_t* key_pad,
                                      const int32_t* q_off, const int32_t* k_off, int B, int n_head, int n_kv, int64_t Tq,
                                      int64_t Tk, int Lq, int Lk, int d, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo,
-                                     float scale, int window, int sinks, int causal, int dtype, void* stream_) {
+                                     float scale, int window, int sinks, int causal, float* workspace,
+                                     int64_t workspace_floats, int dtype, void* stream_) {
   const char* who = "skhip_window_attn_fwd";
   hipStream_t stream = (hipStream_t)stream_;
   WinParams p = {};
@@ -579,8 +647,21 @@ extern "C" int skhip_window_attn_fwd(const void* Q, const void* K, const void* V
   if (Tq == 0) return SK_OK;
   SK_CHECK_ARG(Q && O && LSE && (Tk == 0 || (K && V)), "%s: null pointer", who);
   set_window(p, window, causal);
+  const bool mfma = sk_window_mfma_supported(p, dtype);
+  plan_cuts(p, mfma ? MFMA_ROWS : NT);
   SK_CHECK_ARG(grids_fit(p), "%s: more than 2^24 tiles of 64 rows", who);
-  if (sk_window_mfma_supported(p, dtype)) return sk_window_fwd_mfma(p, stream);
+  const int64_t need = cut_floats(p);
+  if (need > 0 && (!workspace || workspace_floats < need)) {
+    sk_set_error("%s: workspace of %lld floats needed", who, (long long)need);
+    return SK_ERR_WORKSPACE;
+  }
+  SK_CHECK_ARG(need == 0 || ((uintptr_t)workspace & 15) == 0, "%s: workspace not aligned to 16 bytes", who);
+  p.cut_o = workspace;
+  p.cut_ml = workspace + cut_o_floats(p);
+  if (mfma) {
+    rc = sk_window_fwd_mfma(p, stream);
+    return rc ? rc : sk_window_cut_join(p, dtype, stream);
+  }
   p.vec = whole_pieces(p, dtype);
   if (dtype == SK_BF16) {
     launch_fwd<bf16_t>(p, stream);
@@ -588,7 +669,7 @@ extern "C" int skhip_window_attn_fwd(const void* Q, const void* K, const void* V
     launch_fwd<float>(p, stream);
   }
   SK_CHECK_LAUNCH(who);
-  return SK_OK;
+  return sk_window_cut_join(p, dtype, stream);
 }
 
 extern "C" int skhip_window_attn_bwd(const void* Q, const void* K, const void* V, const void* O, const void* dO,
@@ -622,6 +703,7 @@ extern "C" int skhip_window_attn_bwd(const void* Q, const void* K, const void* V
     sk_set_error("%s: workspace of %lld floats needed", who, (long long)need);
     return SK_ERR_WORKSPACE;
   }
+  SK_CHECK_ARG(need == 0 || ((uintptr_t)workspace & 15) == 0, "%s: workspace not aligned to 16 bytes", who);
   p.delta = workspace;
   p.slabs = workspace + (head + 3) / 4 * 4;   // (16-byte stores)
   p.split = p.slabs + slab_floats(p, rows);

@@ -172,15 +172,15 @@ template <int D, int W>
 __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void fwd_kernel(WinParams p, int qtiles) {
   __shared__ __attribute__((aligned(1024))) char lds[2][2 * tile_bytes<D>()];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, hf = lane >> 5;
-  const Work work = work_of_block(p, qtiles, p.H / p.G, true);
+  const Work work = work_of_block(p, qtiles * p.cuts, p.H / p.G, true);
   if (work.none) return;
-  const int tile = work.tile, h = work.h, b = work.b, kh = h / (p.H / p.G);
+  const int h = work.h, b = work.b, kh = h / (p.H / p.G), cut = work.tile % p.cuts;
   if (b == p.B) {
-    zero_rest<bf16_t>((bf16_t*)p.Oout, p.ldo, (int64_t)h * p.d, p.d, p.q_off, p.B, p.Tq, tile, TAIL);
+    zero_rest<bf16_t>((bf16_t*)p.Oout, p.ldo, (int64_t)h * p.d, p.d, p.q_off, p.B, p.Tq, work.tile, TAIL);
     return;
   }
   const Seq sq = seq_of(p, b);
-  const int i0 = tile * OWN;
+  const int i0 = work.tile / p.cuts * OWN;
   if (i0 >= sq.Lq) return;
   const KeyTiles kt = KeyTiles::of<NT>(p, sq, i0, min(i0 + OWN, sq.Lq));
   const int w0 = i0 + 32 * wave, i = w0 + c, pos = i + sq.off;
@@ -213,15 +213,16 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void fwd_kernel(WinParams p, 
     load_tile<D>(buf, K + j0 * p.ldk, p.ldk, p.d, ok, wave, lane);
     load_tile<D>(buf + tile_bytes<D>(), V + j0 * p.ldv, p.ldv, p.d, ok, wave, lane);
   };
+  const int n = max(0, kt.n), t_beg = (int)((int64_t)n * cut / p.cuts), t_end = (int)((int64_t)n * (cut + 1) / p.cuts);
   uint64_t ok = 0;
-  int gone = padding(0);
-  if (kt.n > 0) { ok = usable(0, gone); fetch(0, ok); }
-  gone = padding(1);
-  for (int t = 0; t < kt.n; ++t) {
+  int gone = padding(t_beg);
+  if (t_beg < t_end) { ok = usable(t_beg, gone); fetch(t_beg, ok); }
+  gone = padding(t_beg + 1);
+  for (int t = t_beg; t < t_end; ++t) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();     // tile t is in LDS, and every wave is done with the other buffer
     const uint64_t use = ok;
-    if (t + 1 < kt.n) {
+    if (t + 1 < t_end) {
       ok = usable(t + 1, gone);
       fetch(t + 1, ok);
       gone = padding(t + 2);
@@ -283,6 +284,13 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void fwd_kernel(WinParams p, 
       }
   }
   l = other_sum(l);   // the halves summed different keys
+  if (p.cuts > 1) {
+    if (i >= sq.Lq) return;
+    const int64_t row = ((int64_t)cut * p.H + h) * p.Tq + sq.qbase + i;
+    store_own_f32<W>(p.cut_o + row * p.d, o, 1.f, p.d, hf);
+    if (hf == 0) { p.cut_ml[2 * row] = m * cs; p.cut_ml[2 * row + 1] = l; }
+    return;
+  }
   store_own<W>((bf16_t*)p.Oout + (sq.qbase + min(i, sq.Lq - 1)) * p.ldo + (int64_t)h * p.d, o, l > 0.f || l != l ? 1.f / l : 0.f, p.d, hf,
                i < sq.Lq);
   if (i < sq.Lq && hf == 0)
@@ -560,7 +568,7 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 template <int D, int W>
 void launch_fwd(const WinParams& p, hipStream_t stream) {
   const int qtiles = std::max(1, (p.Lq + OWN - 1) / OWN);
-  const dim3 grid(work_blocks(p, qtiles, p.H / p.G));
+  const dim3 grid(work_blocks(p, qtiles * p.cuts, p.H / p.G));
   hipLaunchKernelGGL((fwd_kernel<D, W>), grid, dim3(256), 0, stream, p, qtiles);
 }
 template <int D, int W>

@@ -162,7 +162,7 @@ def test_entry_points_refuse_before_any_launch():
 
     def fwd(H=4, G=2, d=16, window=3, sinks=1, ldq=64, ldk=32, B=2, Lq=6, Tq=12, qo=None, ko=None, pad=None, lse=p):
         return lib.skhip_window_attn_fwd(p, p, p, p, lse, pad, qo, ko, B, H, G, Tq, 12, Lq, 6, d, ldq, ldk, 32, 64, 0.25, window,
-                                         sinks, 1, 0, None)
+                                         sinks, 1, None, 0, 0, None)
 
     for kw in (dict(G=3), dict(d=129, ldq=1000, ldk=1000), dict(window=0), dict(sinks=-1), dict(ldq=63), dict(ldk=31), dict(Tq=11),
                dict(qo=p), dict(qo=p, ko=p, pad=p), dict(lse=None), dict(B=65535, Lq=0, Tq=0),
@@ -186,5 +186,14 @@ def test_workspace_sizes():
     assert lib.skhip_window_attn_bwd_ws_floats(2, 4, 2, 12, 6, 6, 16, 3, 0, 1) == base
     assert lib.skhip_window_attn_bwd_ws_floats(2, 4, 2, 12, 6, 6, 16, 100, 2, 1) == base
     assert lib.skhip_window_attn_bwd_ws_floats(2, 4, 2, 12, 6, 6, 16, 3, 2, 1) > base
+    # forward: only where few rows see many keys, and then refused without it
+    assert lib.skhip_window_attn_fwd_ws_floats(2, 4, 2, 12, 6, 6, 16, 3, 0, 1) == 0
+    assert lib.skhip_window_attn_fwd_ws_floats(64, 8, 8, 64 * 2048, 2048, 2048, 64, 2048, 0, 1) == 0
+    p = 1 << 20   # stands for a pointer
+    need = lib.skhip_window_attn_fwd_ws_floats(1, 2, 2, 3, 3, 8192, 16, 8192, 0, 1)
+    assert need > 0
+    for ws, n, code in ((None, 0, -3), (p, 1, -3), (p + 4, need, -1)):
+        assert lib.skhip_window_attn_fwd(p, p, p, p, p, None, None, None, 1, 2, 2, 3, 8192, 3, 8192, 16, 32, 32, 32, 32, 0.25, 8192,
+                                         0, 1, ws, n, 0, None) == code
     assert lib.skhip_window_attn_step_ws_floats(65535, 8, 8, 64, 4096, 4096, 0) == 0
     assert lib.skhip_window_attn_step_ws_floats(1, 8, 8, 64, 4096, 4096, 0) > 0

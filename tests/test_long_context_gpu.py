@@ -449,6 +449,23 @@ def test_window_keys_in_parts(case, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("case", [  # few queries before many keys: the keys of a query tile come to several blocks
+    ([64], [4000], 2, 1, 64, None, 0, True), ([3], [3000], 4, 2, 128, 2500, 70, True), ([1], [2100], 1, 1, 37, None, 0, False),
+    ([200], [1500], 2, 2, 96, 1200, 3, True), ([1500], [1500], 1, 1, 32, None, 0, True)])
+def test_window_queries_in_cuts(case, dtype):
+    lens_q, lens_k, H, G, d, window, sinks, causal = case
+    run_window(lens_q, lens_k, H, G, d, window, sinks, causal, dtype, "dense", seed=6)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_window_queries_in_cuts_of_ragged_batches(dtype):
+    run_window([5, 0, 40, 7], [2000, 900, 1300, 0], 2, 1, 64, 1900, 4, True, dtype, "packed", seed=7)
+    pads = torch.zeros((3, 1800), dtype=torch.uint8)
+    pads[0, 100:1700], pads[1, :1790], pads[2, :] = 1, 1, 1
+    run_window([20] * 3, [1800] * 3, 2, 2, 80, None, 0, False, dtype, "padded", seed=8, pads=pads)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_window_keys_in_parts_of_ragged_batches(dtype):
     lens = [300, 1, 0, 170, 64]
     run_window(lens, lens, 8, 1, 64, 120, 4, True, dtype, "packed", seed=4)
