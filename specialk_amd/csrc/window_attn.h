@@ -34,8 +34,8 @@ struct WinParams {
   // blocks, each of which leaves fp32 sums in split, [parts][dK, dV][B * Lk][G * d], added in a fixed order as well.
   int parts;
   float* split;
-  // Forward with few query rows before many keys: a block's key tiles cut into `cuts` blocks, which leave unnormalised
-  // outputs [cuts][H][Tq][d] in cut_o and (maximum in powers of two, sum) [cuts][H][Tq][2] in cut_ml.
+  // Few query rows before many keys: a block's key tiles cut into `cuts` blocks, which leave unnormalised outputs (backward:
+  // sums of dQ) [cuts][H][Tq][d] in cut_o and (maximum in powers of two, sum) [cuts][H][Tq][2] in cut_ml.
   int cuts;
   float *cut_o, *cut_ml;
 };

@@ -160,7 +160,7 @@ template <typename T, int D> struct KeySweep {
   Stage<T, D> k, v;
   int gone, beg, end;
   // the `cut`-th of `cuts` shares of the tiles that queries i0 .. i0 + 63 see
-  __device__ __forceinline__ KeySweep(const WinParams& p_, const Seq& sq_, int b, int kh, int i0, int cut = 0, int cuts = 1)
+  __device__ __forceinline__ KeySweep(const WinParams& p_, const Seq& sq_, int b, int kh, int i0, int cut, int cuts)
       : p(p_), sq(sq_), kt(KeyTiles::of<NT>(p_, sq_, i0, min(i0 + 64, sq_.Lq))) {
     beg = (int)((int64_t)max(0, kt.n) * cut / cuts);
     end = (int)((int64_t)max(0, kt.n) * (cut + 1) / cuts);
@@ -271,19 +271,19 @@ __global__ __launch_bounds__(256, BLOCKS(D)) void window_dq_kernel(WinParams p) 
   __shared__ __attribute__((aligned(16))) Tile<D> Vs;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
   const int qtiles = max(1, (p.Lq + 63) / 64);
-  const Work work = work_of_block(p, qtiles, p.H / p.G, true);
+  const Work work = work_of_block(p, qtiles * p.cuts, p.H / p.G, true);
   if (work.none) return;
-  const int b = work.b, h = work.h, kh = h / (p.H / p.G);
+  const int b = work.b, h = work.h, kh = h / (p.H / p.G), cut = work.tile % p.cuts;
   if (b == p.B) {
     zero_rest<T>((T*)p.dQ, p.lddq, (int64_t)h * p.d, p.d, p.q_off, p.B, p.Tq, work.tile, TAIL);
     return;
   }
   const Seq sq = seq_of(p, b);
-  const int i0 = work.tile * 64;
+  const int i0 = work.tile / p.cuts * 64;
   if (i0 >= sq.Lq) return;
   const int i = i0 + wave * 16 + c, pos = i + sq.off;
   const int64_t row = sq.qbase + min(i, sq.Lq - 1), si = (int64_t)h * p.Tq + row;
-  KeySweep<T, D> keys(p, sq, b, kh, i0);
+  KeySweep<T, D> keys(p, sq, b, kh, i0, cut, p.cuts);
   f32x4_t fq[D / 16], fd[D / 16], dq[D / 16];
   load_own<T, D>(fq, (const T*)p.O + row * p.ldo + (int64_t)h * p.d, p.d, g, i < sq.Lq);
   load_own<T, D>(fd, (const T*)p.dO + row * p.lddo + (int64_t)h * p.d, p.d, g, i < sq.Lq);
@@ -297,8 +297,8 @@ __global__ __launch_bounds__(256, BLOCKS(D)) void window_dq_kernel(WinParams p) 
   dl = quad_sum(dl);
   load_own<T, D>(fq, (const T*)p.Q + row * p.ldq + (int64_t)h * p.d, p.d, g, i < sq.Lq);
   const float cs = p.scale * LOG2E, lse2 = p.LSE[si] * LOG2E;
-  if (i < sq.Lq && g == 0) p.delta[si] = dl;
-  for (int t = 0; t < keys.kt.n; ++t) {
+  if (i < sq.Lq && g == 0 && cut == 0) p.delta[si] = dl;
+  for (int t = keys.beg; t < keys.end; ++t) {
     const uint64_t ok = keys.next(t, Ks, Vs), see = i < sq.Lq ? keys_seen(p, pos, keys.start(t), ok) : 0;
     const uint64_t mk = see >> (4 * g);
 #pragma unroll
@@ -311,6 +311,10 @@ __global__ __launch_bounds__(256, BLOCKS(D)) void window_dq_kernel(WinParams p) 
         ds[r] = keep_or(__builtin_amdgcn_exp2f(fmaf(ds[r], cs, -lse2)) * (dp[r] - dl), mk, k, r, 0u);
       add_cols<D>(dq, Ks, 16 * k, ds, lane);
     }
+  }
+  if (p.cuts > 1) {
+    if (i < sq.Lq) store_own<float, D>(p.cut_o + (((int64_t)cut * p.H + h) * p.Tq + row) * p.d, dq, p.scale, p.d, g);
+    return;
   }
   if (i < sq.Lq) store_own<T, D>((T*)p.dQ + (sq.qbase + i) * p.lddq + (int64_t)h * p.d, dq, p.scale, p.d, g);
 }
@@ -478,6 +482,21 @@ __global__ __launch_bounds__(256) void window_cut_join_kernel(WinParams p) {
   if (c == 0) p.LSE[row] = l > 0.f ? m * LN2 + logf(l) : (some ? l : -INFINITY);
 }
 
+// dQ of rows whose keys were cut.
+template <typename T>
+__global__ __launch_bounds__(256) void window_cut_sum_kernel(WinParams p) {
+  const int b = blockIdx.y, width = p.H * p.d;
+  const Seq sq = seq_of(p, b);
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int i = (int)(e / width), col = (int)(e - (int64_t)i * width), h = col / p.d, c = col - h * p.d;
+  if (i >= sq.Lq) return;
+  const float* x = p.cut_o + ((int64_t)h * p.Tq + sq.qbase + i) * p.d + c;
+  float a = 0.f;
+#pragma unroll 8
+  for (int s = 0; s < p.cuts; ++s) a += x[(int64_t)s * p.H * p.Tq * p.d];
+  ((T*)p.dQ)[(sq.qbase + i) * p.lddq + col] = Cvt<T>::from_f32(a);
+}
+
 // whether every row of the operands that go through LDS is made of whole 4-element pieces
 bool whole_pieces(const WinParams& p, int dtype) {
   const int64_t size = dtype == SK_BF16 ? 2 : 4;
@@ -526,7 +545,7 @@ void plan_keys(WinParams& p, int rows) {
 }
 
 // Cuts of a query tile's keys: two blocks for every CU, each with at least 12 tiles of 64 keys (fp32 arithmetic: 8).  64
-// queries at the end of 32768 keys, 8 heads of 128, all visible: 8 blocks alone 649 us, cut 54 (fp32 4276 and 148); 4096
+// queries at the end of 32768 keys, 8 heads of 128, all visible: 8 blocks alone 649 us, cut 54 (fp32 4276 and 148), forward and backward 1262 and 186; 4096
 // tokens, 4 heads of 64, causal: 74 and 41.  Shorter sweeps are not worth the join: 2048 tokens, 8 heads of 128, window 1024
 // (18 tiles): uncut 30, in two 38.
 void plan_cuts(WinParams& p, int rows) {
@@ -556,7 +575,7 @@ void launch_fwd_at(const WinParams& p, hipStream_t stream) {
 }
 template <typename T, int D>
 void launch_bwd_at(const WinParams& p, hipStream_t stream) {
-  const dim3 gq(work_blocks(p, std::max(1, (p.Lq + 63) / 64), p.H / p.G));
+  const dim3 gq(work_blocks(p, std::max(1, (p.Lq + 63) / 64) * p.cuts, p.H / p.G));
   const dim3 gk(work_blocks(p, key_tiles_of_grid(p, std::max(1, (p.Lk + NT - 1) / NT)), 1));
   if (p.Tq) hipLaunchKernelGGL((window_dq_kernel<T, D>), gq, dim3(256), 0, stream, p);
   if (p.Tk) hipLaunchKernelGGL((window_dkv_kernel<T, D>), gk, dim3(256), 0, stream, p);
@@ -581,6 +600,12 @@ void launch_bwd(const WinParams& p, hipStream_t stream) {
 }  // namespace
 
 int sk_window_join(const WinParams& p, int rows, int dtype, hipStream_t stream) {
+  if (p.cuts > 1 && p.Tq) {
+    const dim3 all((unsigned)(((int64_t)p.Lq * p.H * p.d + 255) / 256), p.B);
+    if (dtype == SK_BF16) hipLaunchKernelGGL((window_cut_sum_kernel<bf16_t>), all, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((window_cut_sum_kernel<float>), all, dim3(256), 0, stream, p);
+    SK_CHECK_LAUNCH("skhip_window_attn_bwd(join)");
+  }
   if ((!p.nst && p.parts == 1) || !p.Tk) return SK_OK;
   if (p.parts > 1) {
     const dim3 all((unsigned)(((int64_t)p.Lk * p.G * p.d + 255) / 256), p.B);
@@ -622,13 +647,15 @@ extern "C" int64_t skhip_window_attn_bwd_ws_floats(int B, int n_head, int n_kv, 
                                                    int sinks, int causal) {
   if (B < 0 || n_head <= 0 || n_kv <= 0 || Tq < 0 || Lq < 0 || Lk < 0 || d <= 0 || window < 1 || sinks < 0) return 0;
   WinParams p = {};
-  p.B = B; p.H = n_head; p.G = n_kv; p.Lq = Lq; p.Lk = Lk; p.d = d; p.sinks = sinks;
+  p.B = B; p.H = n_head; p.G = n_kv; p.Tq = Tq; p.Lq = Lq; p.Lk = Lk; p.d = d; p.sinks = sinks;
   set_window(p, window, causal);
   // the larger of the two paths' needs: which one a call takes depends on its pointers and strides
   plan_keys(p, NT);
-  const int64_t plain = ((int64_t)n_head * Tq + 3) / 4 * 4 + slab_floats(p, NT) + split_floats(p);
+  plan_cuts(p, NT);
+  const int64_t plain = ((int64_t)n_head * Tq + 3) / 4 * 4 + slab_floats(p, NT) + split_floats(p) + cut_floats(p);
   plan_keys(p, MFMA_ROWS);
-  return std::max(plain, (2 * (int64_t)n_head * Tq + 3) / 4 * 4 + slab_floats(p, MFMA_ROWS) + split_floats(p));
+  plan_cuts(p, MFMA_ROWS);
+  return std::max(plain, (2 * (int64_t)n_head * Tq + 3) / 4 * 4 + slab_floats(p, MFMA_ROWS) + split_floats(p) + cut_floats(p));
 }
 
 extern "C" int skhip_window_attn_fwd(const void* Q, const void* K, const void* V, void* O, float* LSE, const uint8_t* key_pad,
@@ -697,8 +724,9 @@ extern "C" int skhip_window_attn_bwd(const void* Q, const void* K, const void* V
   const bool mfma = sk_window_mfma_supported(p, dtype);
   const int rows = mfma ? MFMA_ROWS : NT;
   plan_keys(p, rows);
+  plan_cuts(p, rows);
   SK_CHECK_ARG(grids_fit(p), "%s: more than 2^24 tiles of 64 rows", who);
-  const int64_t head = (mfma ? 2 : 1) * (int64_t)n_head * Tq, need = (head + 3) / 4 * 4 + slab_floats(p, rows) + split_floats(p);
+  const int64_t head = (mfma ? 2 : 1) * (int64_t)n_head * Tq, need = (head + 3) / 4 * 4 + slab_floats(p, rows) + split_floats(p) + cut_floats(p);
   if (need > 0 && (!workspace || workspace_floats < need)) {
     sk_set_error("%s: workspace of %lld floats needed", who, (long long)need);
     return SK_ERR_WORKSPACE;
@@ -707,6 +735,7 @@ extern "C" int skhip_window_attn_bwd(const void* Q, const void* K, const void* V
   p.delta = workspace;
   p.slabs = workspace + (head + 3) / 4 * 4;   // (16-byte stores)
   p.split = p.slabs + slab_floats(p, rows);
+  p.cut_o = p.split + split_floats(p);   // (multiples of 4 floats up to here where 16-byte stores are made: d % 8 == 0)
   p.vec = whole_pieces(p, dtype);
   if (mfma) {
     rc = sk_window_bwd_mfma(p, stream);

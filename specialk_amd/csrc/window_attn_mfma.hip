@@ -311,15 +311,15 @@ template <int D, int W>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dq_kernel(WinParams p, int qtiles) {
   __shared__ __attribute__((aligned(1024))) char lds[2][2 * tile_bytes<D>()];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, hf = lane >> 5;
-  const Work work = work_of_block(p, qtiles, p.H / p.G, true);
+  const Work work = work_of_block(p, qtiles * p.cuts, p.H / p.G, true);
   if (work.none) return;
-  const int tile = work.tile, h = work.h, b = work.b, kh = h / (p.H / p.G);
+  const int h = work.h, b = work.b, kh = h / (p.H / p.G), cut = work.tile % p.cuts;
   if (b == p.B) {
-    zero_rest<bf16_t>((bf16_t*)p.dQ, p.lddq, (int64_t)h * p.d, p.d, p.q_off, p.B, p.Tq, tile, TAIL);
+    zero_rest<bf16_t>((bf16_t*)p.dQ, p.lddq, (int64_t)h * p.d, p.d, p.q_off, p.B, p.Tq, work.tile, TAIL);
     return;
   }
   const Seq sq = seq_of(p, b);
-  const int i0 = tile * OWN;
+  const int i0 = work.tile / p.cuts * OWN;
   if (i0 >= sq.Lq) return;
   const KeyTiles kt = KeyTiles::of<NT>(p, sq, i0, min(i0 + OWN, sq.Lq));
   const int w0 = i0 + 32 * wave, i = w0 + c, pos = i + sq.off;
@@ -392,20 +392,20 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dq_kernel(WinParams p, i
     }
     return part;
   };
-  auto sweep = [&](auto delta_only, bool resident) {
+  auto sweep = [&](auto delta_only, bool resident, int t_beg, int t_end) {
     uint64_t ok = 0;
-    int gone = padding(0);
+    int gone = padding(t_beg);
     float sum = 0.f;
-    if (kt.n > 0) ok = usable(0, gone);
-    if (kt.n > 0 && !resident) fetch(0, ok);
-    gone = padding(1);
-    for (int t = 0; t < kt.n; ++t) {
+    if (t_beg < t_end) ok = usable(t_beg, gone);
+    if (t_beg < t_end && !resident) fetch(t_beg, ok);
+    gone = padding(t_beg + 1);
+    for (int t = t_beg; t < t_end; ++t) {
       if (!resident) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
       }
       const uint64_t use = ok;
-      if (t + 1 < kt.n) {
+      if (t + 1 < t_end) {
         ok = usable(t + 1, gone);
         if (!resident) fetch(t + 1, ok);
         gone = padding(t + 2);
@@ -422,16 +422,21 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dq_kernel(WinParams p, i
     }
     return sum;
   };
-  const bool both = few && kt.n <= 2;   // (the tiles are then all in LDS when the first sweep ends)
+  const int n = max(0, kt.n);
+  const bool both = few && n <= 2 && p.cuts == 1;   // (the tiles are then all in LDS when the first sweep ends)
   if (few) {
-    const float exact = other_sum(sweep(std::true_type{}, false));
+    const float exact = other_sum(sweep(std::true_type{}, false, 0, n));
     dl = few_row ? exact : dl;
     if (!both) __syncthreads();   // every wave is done with the tiles
   }
-  sweep(std::false_type{}, both);
-  if (i < sq.Lq && hf == 0) {   // what the dK / dV kernel's accumulators start from
+  sweep(std::false_type{}, both, (int)((int64_t)n * cut / p.cuts), (int)((int64_t)n * (cut + 1) / p.cuts));
+  if (i < sq.Lq && hf == 0 && cut == 0) {   // what the dK / dV kernel's accumulators start from
     p.delta[si] = -dl;
     p.delta[(int64_t)p.H * p.Tq + si] = -p.LSE[si] / p.scale;
+  }
+  if (p.cuts > 1) {
+    if (i < sq.Lq) store_own_f32<W>(p.cut_o + (((int64_t)cut * p.H + h) * p.Tq + row) * p.d, dq, p.scale, p.d, hf);
+    return;
   }
   store_own<W>((bf16_t*)p.dQ + row * p.lddq + (int64_t)h * p.d, dq, p.scale, p.d, hf, i < sq.Lq);
 }
@@ -574,7 +579,7 @@ void launch_fwd(const WinParams& p, hipStream_t stream) {
 template <int D, int W>
 void launch_bwd(const WinParams& p, hipStream_t stream) {
   const int qtiles = std::max(1, (p.Lq + OWN - 1) / OWN), ktiles = std::max(1, (p.Lk + OWN - 1) / OWN);
-  const dim3 gq(work_blocks(p, qtiles, p.H / p.G)), gk(work_blocks(p, key_tiles_of_grid(p, ktiles), 1));
+  const dim3 gq(work_blocks(p, qtiles * p.cuts, p.H / p.G)), gk(work_blocks(p, key_tiles_of_grid(p, ktiles), 1));
   if (p.Tq) hipLaunchKernelGGL((dq_kernel<D, W>), gq, dim3(256), 0, stream, p, qtiles);
   if (!p.Tk) return;
   if constexpr (W <= TOGETHER) {
