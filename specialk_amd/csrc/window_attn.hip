@@ -545,9 +545,9 @@ void plan_keys(WinParams& p, int rows) {
 }
 
 // Cuts of a query tile's keys: two blocks for every CU, each with at least 12 tiles of 64 keys (fp32 arithmetic: 8).  64
-// queries at the end of 32768 keys, 8 heads of 128, all visible: 8 blocks alone 649 us, cut 54 (fp32 4276 and 148), forward and backward 1262 and 186; 4096
-// tokens, 4 heads of 64, causal: 74 and 41.  Shorter sweeps are not worth the join: 2048 tokens, 8 heads of 128, window 1024
-// (18 tiles): uncut 30, in two 38.
+// queries at the end of 32768 keys, 8 heads of 128, all visible: 8 blocks alone 649 us, cut 54, with the backward pass 1262
+// and 186 (fp32 4276 and 148, 5861 and 737); 4096 tokens, 4 heads of 64, causal: 74 and 41.  Shorter sweeps are not worth
+// the join: 2048 tokens, 8 heads of 128, window 1024 (18 tiles): uncut 30, in two 38.
 void plan_cuts(WinParams& p, int rows) {
   const int64_t blocks = std::max<int64_t>(1, (int64_t)p.B * p.H * ((p.Lq + rows - 1) / rows));
   const int64_t tiles = std::min<int64_t>(p.Lk, (int64_t)rows + p.left + p.right + p.sinks) / 64;
