@@ -97,8 +97,8 @@ __global__ __launch_bounds__(256) void step_kernel(StepParams p, int vec) {
       }
       s = acc;
     }
-    const float mn = fmaxf(m, wave_max(s));   // finite: the pass holds at least one position (NaN scores stay NaN)
-    const float alpha = m == -INFINITY ? 0.f : expf(m - mn), pr = on ? expf(s - mn) : 0.f;
+    const float mn = fmaxf(m, wave_max(s)), base = mn == -INFINITY ? 0.f : mn;   // (-inf: no score above -inf so far, or NaN scores only)
+    const float alpha = m == -INFINITY ? 0.f : expf(m - mn), pr = on ? expf(s - base) : 0.f;
     l = l * alpha + wave_sum(pr);
     m = mn;
     a0 *= alpha;

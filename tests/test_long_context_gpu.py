@@ -825,3 +825,50 @@ def test_step_scale_of_nothing():
         # the mean of 600 values in fp32 (n E of their mean size), rounded once
         bound = want.abs() * unit(BF) + 700 * E * vc[0].double().abs().mean(0)
         check(o[0], want, bound, scale)
+
+
+# ------------------------------------------------------------------------------ infinities at visible positions of a cache
+def step_without(dead, n, d, dtype, shift=0, H=2):
+    """A cache of n positions, those in `dead` with scores of -inf: the result is that of the others, within its bound."""
+    g = torch.Generator().manual_seed(n + d)
+    q = rnd((1, H * d), dtype, g).abs() + 0.1
+    kc, vc = rnd((1, n, H * d), dtype, g), rnd((1, n, H * d), dtype, g)
+    for h in range(H):
+        kc[0, dead, h * d] = -math.inf
+    alive = torch.ones(n, dtype=torch.bool)
+    alive[dead] = False
+    want, bound = torch.zeros((1, H * d), dtype=torch.float64), torch.full((1, H * d), TINY, dtype=torch.float64)
+    for h in range(H):
+        s = slice(h * d, h * d + d)
+        vis = torch.ones((1, int(alive.sum())), dtype=torch.bool)
+        (o, eo), *_ = attention64(q[:, s], kc[0, alive][:, s], vc[0, alive][:, s], q[:, s], vis, d ** -0.5, dtype)
+        want[:, s], bound[:, s] = o, bound[:, s] + eo
+    wide = torch.zeros((2, 1, n, H * d + shift), dtype=dtype, device=DEV)
+    k, v = wide[0, ..., shift:], wide[1, ..., shift:]
+    k.copy_(kc), v.copy_(vc)
+    o = ops.window_attention_step(q.to(DEV), None, None, k, v, torch.tensor([n], dtype=torch.int32, device=DEV), H)
+    check(o, want, bound, (n, d, shift))
+
+
+# one position alone in a wave's first pass; a wave's whole first pass; all passes of a wave, of a split; all but one position
+DEAD = [(65, [64]), (200, list(range(64))), (200, list(range(64, 128))), (700, list(range(256))), (6000, list(range(100, 4000))),
+        (300, list(range(299)))]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("d,shift", [(37, 0), (64, 1)])
+@pytest.mark.parametrize("n,dead", DEAD)
+def test_step_scores_of_minus_infinity_on_odd_rows(n, dead, d, shift, dtype):
+    step_without(dead, n, d, dtype, shift)
+
+
+def test_step_without_any_finite_score_gives_zeros():
+    """As a row of window_attention whose scores are all -inf, on odd rows and on whole 16-byte pieces."""
+    for d in (37, 64):
+        for n in (65, 6000):
+            k = torch.full((1, n, d), -math.inf, dtype=BF, device=DEV)
+            v = torch.ones((1, n, d), dtype=BF, device=DEV)
+            q = torch.ones((1, d), dtype=BF, device=DEV)
+            o = ops.window_attention_step(q, None, None, k, v, torch.tensor([n], dtype=torch.int32, device=DEV), 1)
+            assert not o.any(), (d, n)
+            assert torch.equal(o, ops.window_attention(q, k[0], v[0], 1, 1, n, 1)), (d, n)
