@@ -216,8 +216,8 @@ template <int D> struct Pass<float, D> {    // v_mfma_f32_16x16x4_f32
 };
 
 // Every wave keeps two passes in flight: the next pass's keys in registers and values in its own LDS buffer, by direct
-// loads, while this one is multiplied; nothing is shared between waves until the end.  Positions beyond the split read its
-// first one again and are masked, elements beyond the head its first piece against a zero query.
+// loads, while this one is multiplied; nothing is shared between waves until the end.  Positions beyond the split read the
+// pass's first one again, elements beyond the head its first piece: both are cleared before they are multiplied.
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void step_mfma_kernel(StepParams p, int chunks) {
   typedef Pass<T, D> P;
@@ -287,6 +287,17 @@ __global__ __launch_bounds__(256, 2) void step_mfma_kernel(StepParams p, int chu
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NV + P::PIECES * NK) : "memory");
     } else {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    if (p.d < D) {               // (pieces beyond the head: an infinity there must not meet the query's zeros,
+#pragma unroll
+      for (int s = 0; s < NK; ++s)
+#pragma unroll
+        for (int t = 0; t < P::PIECES; ++t) k[t][s] = P::first(s, g) < p.d ? k[t][s] : frag{};
+    }
+    if (u0 + MT > u_end) {       // nor one in the values read again the probabilities' zeros)
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (u0 + j * RPI + lane / CH >= u_end) *(uint4*)(vt + j * 1024 + lane * 16) = make_uint4(0, 0, 0, 0);
     }
     f32x4_t sc[P::PIECES];
     float mx = -INFINITY;

@@ -872,3 +872,26 @@ def test_step_without_any_finite_score_gives_zeros():
             o = ops.window_attention_step(q, None, None, k, v, torch.tensor([n], dtype=torch.int32, device=DEV), 1)
             assert not o.any(), (d, n)
             assert torch.equal(o, ops.window_attention(q, k[0], v[0], 1, 1, n, 1)), (d, n)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("d", [8, 64, 72, 80, 96, 128])
+@pytest.mark.parametrize("n,dead", DEAD)
+def test_step_scores_of_minus_infinity(n, dead, d, dtype):
+    """Head sizes below the width they are computed at: the infinity is the head's first element."""
+    step_without(dead, n, d, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("d", [37, 64, 80])
+@pytest.mark.parametrize("n,at", [(1, 0), (5, 0), (33, 32), (129, 128), (40, 32), (40, 35), (6000, 5999)])
+def test_step_infinite_value(n, at, d, dtype):
+    """An infinity in a visible value is one in its column of the output, and nothing but that."""
+    g = torch.Generator().manual_seed(n)
+    q, kc, vc = rnd((1, d), dtype, g).to(DEV), rnd((1, n, d), dtype, g).to(DEV), rnd((1, n, d), dtype, g).to(DEV)
+    length = torch.tensor([n], dtype=torch.int32, device=DEV)
+    want = ops.window_attention_step(q, None, None, kc, vc, length, 1)
+    vc[0, at, 3] = math.inf
+    got = ops.window_attention_step(q, None, None, kc, vc, length, 1)
+    want[0, 3] = math.inf
+    assert torch.equal(got, want)
