@@ -424,10 +424,12 @@ def window_attn_step(q, k_new, v_new, k_cache, v_cache, kv_len, n_head, n_kv, d,
     o = _fresh(q)
     n = _step_ws(R, n_head, n_kv, d, cap, window, sinks)
     ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
+    (k_row, k_pos, _), (v_row, v_pos, _) = k_cache.stride(), v_cache.stride()
+    if cap == 1:
+        k_pos = v_pos = n_kv * d   # (the stride of one position says nothing)
     rc = lib.skhip_window_attn_step(_ptr(q), _ptr(k_new), _ptr(v_new), _ptr(k_cache), _ptr(v_cache), _ptr(o), _ptr(kv_len), R,
                                     n_head, n_kv, d, cap, q.stride(0), 0 if k_new is None else k_new.stride(0), n_head * d,
-                                    *k_cache.stride()[:2], *v_cache.stride()[:2], float(scale), window, sinks, _ptr(ws), n,
-                                    dcode(q.dtype), _stream())
+                                    k_row, k_pos, v_row, v_pos, float(scale), window, sinks, _ptr(ws), n, dcode(q.dtype), _stream())
     _check(rc, "skhip_window_attn_step")
     return o
 

@@ -1010,7 +1010,11 @@ def _rows(x, width, what):
     if len(shape) != 2 or shape[1] != width:
         raise ValueError(f"{what} must be (rows, {width}), got {tuple(shape)}")
     row, col = x.stride()
-    return x if col == 1 and row >= width else x.contiguous()
+    if col == 1 and row >= width:
+        return x
+    x = x.contiguous()
+    # (a single row counts as contiguous whatever its stride: flattened and back, that is the row's length)
+    return x.view(-1).view(shape) if shape[0] < 2 else x
 
 
 def _heads(x, n_head, n_kv_head, most):
@@ -1237,6 +1241,8 @@ def window_attention_step(q, k_new, v_new, k_cache, v_cache, kv_len, n_head, n_k
     cap = shape[1]
     for c in (k_cache, v_cache):
         s0, s1, s2 = c.stride()   # sequence by sequence, or position by position
+        if cap == 1:
+            s1 = w   # (as in the call below)
         if s2 != 1 or s1 < w or s0 < 0 or (R > 1 and s0 < (cap - 1) * s1 + w and (s0 < w or s1 < (R - 1) * s0 + w)):
             raise ValueError(f"cache rows overlap or are not contiguous (strides {c.stride()})")
     if k_new is not None:

@@ -46,6 +46,18 @@ def test_frequency_refusals(kw):
         ops.RotaryFrequencies(device="cpu", **kw)
 
 
+# ------------------------------------------------------------------------------ rows
+@pytest.mark.parametrize("x", [torch.arange(8.0).view(8, 1).t(), torch.arange(8.0).expand(1, 8), torch.ones(()).expand(1, 8),
+                               torch.zeros(16)[::2].view(1, 8), torch.empty(8, 0).t(), torch.arange(8.0).view(1, 8),
+                               torch.zeros(3, 8)[1:2], torch.zeros(8, 3).t(), torch.ones(8).expand(3, 8), torch.zeros(3, 20)[:, 3:11]])
+def test_rows_have_a_stride_of_their_length_at_least(x):
+    """What torch calls contiguous may have any stride along a dimension of one."""
+    y = ops._rows(x, 8, "x")
+    assert torch.equal(x, y) and y.stride(1) == 1 and y.stride(0) >= 8
+    if x.stride(0) >= 8 and x.stride(1) == 1:
+        assert y is x
+
+
 # ------------------------------------------------------------------------------ rotary, norm
 def rotary_args(**kw):
     a = dict(q=rows(5, 64), k=rows(5, 32), pos=torch.arange(5), freqs=freqs(), n_head=4, n_kv_head=2)

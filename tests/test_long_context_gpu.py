@@ -895,3 +895,46 @@ def test_step_infinite_value(n, at, d, dtype):
     got = ops.window_attention_step(q, None, None, kc, vc, length, 1)
     want[0, 3] = math.inf
     assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------------------ one row, whose stride says nothing
+def one_row(x):
+    """The same (1, w) row with a row stride of 1, which torch calls contiguous."""
+    return x.view(-1, 1).t()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_one_row_of_any_stride(dtype):
+    g = torch.Generator().manual_seed(20)
+    H, d = 2, 64
+    f = ops.RotaryFrequencies(64, device=DEV)
+    pos = torch.tensor([7], device=DEV)
+    x, y, z, do = (rnd((1, H * d), dtype, g).to(DEV) for _ in range(4))
+    gamma = torch.ones(d, device=DEV)
+    calls = (lambda a, b, c: ops.rotary(a, b, pos, f, H)[0], lambda a, b, c: ops.qk_norm_rotary(a, b, gamma, gamma, pos, f, H)[0],
+             lambda a, b, c: ops.window_attention(a, b, c, 1, 1, 1, H))
+    for call in calls:
+        leaves = [t.clone().requires_grad_() for t in (x, y, z)]
+        want = call(*leaves)
+        (dx,) = torch.autograd.grad(want, leaves[0], do)
+        odd = [one_row(t).requires_grad_() for t in (x, y, z)]
+        assert odd[0].stride() == (1, 1)
+        got = call(*odd)
+        assert torch.equal(got, want)
+        assert torch.equal(torch.autograd.grad(got, odd[0], do)[0], dx)
+        got = call(*leaves)   # gradients as autograd hands them over: strides (1, 1) and (0, 1)
+        assert torch.equal(torch.autograd.grad(got.t().contiguous(), leaves[0], do.t())[0], dx)
+        got = call(*leaves)
+        assert torch.equal(torch.autograd.grad(got.sum(0), leaves[0], do[0])[0], dx)
+    kc, vc = rnd((1, 9, H * d), dtype, g).to(DEV), rnd((1, 9, H * d), dtype, g).to(DEV)
+    length = torch.tensor([9], dtype=torch.int32, device=DEV)
+    want = ops.window_attention_step(x, y, z, kc, vc, length, H)
+    assert torch.equal(ops.window_attention_step(one_row(x), one_row(y), one_row(z), kc, vc, length, H), want)
+    # caches of one position: its stride says nothing either
+    k1, v1 = kc[:, :1].clone(), vc[:, :1].clone()
+    length.fill_(1)
+    want = ops.window_attention_step(x, y, z, k1, v1, length, H)
+    k2, v2 = (t.reshape(1, -1, 1).transpose(1, 2) for t in (torch.zeros_like(k1), torch.zeros_like(v1)))
+    assert k2.shape == k1.shape and k2.stride(1) < H * d
+    assert torch.equal(ops.window_attention_step(x, y, z, k2, v2, length, H), want)
+    assert torch.equal(k2, k1) and torch.equal(v2, v1)
