@@ -14,6 +14,7 @@ import contextlib
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -1033,8 +1034,17 @@ def _same(first, *tensors):
             raise ValueError(f"tensors on {dev} and {t.device}")
 
 
+def _no_tangents(tensors):
+    """Refuses dual tensors: past the tape their tangents would be lost without a word."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:   # (-1: no level is open, so there are none)
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("this operator has no forward-mode derivative")
+
+
 def _run(fn, leaves, *rest):
     """fn of the tensors `leaves` that may want gradients and of the rest, without the tape where none does."""
+    _no_tangents(leaves)
     if torch.is_grad_enabled():
         for a in leaves:
             if a is not None and a.requires_grad:
@@ -1266,6 +1276,7 @@ def window_attention_step(q, k_new, v_new, k_cache, v_cache, kv_len, n_head, n_k
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or
                                     (k_new is not None and (k_new.requires_grad or v_new.requires_grad))):
         raise RuntimeError("window_attention_step has no gradient: call it under torch.no_grad() or on detached tensors")
+    _no_tangents((q, k_new, v_new, k_cache, v_cache))
     with L.on_device(q):
         return L.window_attn_step(q, k_new, v_new, k_cache, v_cache, kv_len, n_head, n_kv, d,
                                   d ** -0.5 if scale is None else float(scale), window, int(sinks))

@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from specialk_amd import _lib as L
 from specialk_amd import ops
@@ -149,6 +150,27 @@ def test_step_has_no_gradient():
         ops.window_attention_step(**step_args(q=rows(2, 64).requires_grad_()))
     with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):
         ops.window_attention_step(**step_args(q=rows(2, 64).requires_grad_()))
+
+
+# ------------------------------------------------------------------------------ forward mode
+@pytest.mark.parametrize("leaf", [False, True])
+@pytest.mark.parametrize("grad", [True, False])
+def test_tangents_are_refused(grad, leaf):
+    """A dual tensor in any place: an error, not a result without a tangent."""
+    gammas = dict(gamma_q=torch.ones(16), gamma_k=torch.ones(16))
+    calls = ((ops.rotary, rotary_args(), "qk"), (ops.qk_norm_rotary, rotary_args(**gammas), ("q", "k", "gamma_q", "gamma_k")),
+             (ops.window_attention, window_args(), "qkv"),
+             (ops.window_attention_step, step_args(), ("q", "k_new", "v_new", "k_cache", "v_cache")))
+    for fn, args, names in calls:
+        if leaf and fn is ops.window_attention_step:
+            continue
+        for name in names:
+            with torch.set_grad_enabled(grad), forward_ad.dual_level():
+                x = args[name].clone().requires_grad_(leaf)
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    fn(**{**args, name: forward_ad.make_dual(x, torch.ones_like(x))})
+                with pytest.raises(RuntimeError, match="GPU"):   # (a level alone changes nothing)
+                    fn(**args)
 
 
 # ------------------------------------------------------------------------------ the C entry points
