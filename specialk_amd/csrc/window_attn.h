@@ -94,13 +94,13 @@ struct KeyTiles {
   __device__ __forceinline__ bool holds(int j) const { return j < hi && (j >= lo || j < s_hi); }
 };
 
-// Queries that see keys j0 .. j1-1 (rows [i_lo, i_hi)): chunk < 0: through the window; else the given chunk of the
-// queries beyond it, which see only the sinks among the keys.
+// Queries that see keys j0 .. j1-1 (rows [i_lo, i_hi)): chunk < 0: through the window, and beyond it if there are sinks among
+// the keys and no chunks; else the given chunk of the queries beyond it, which see only the sinks among the keys.
 __device__ __forceinline__ void query_range(const WinParams& p, const Seq& sq, int j0, int j1, int chunk, int& i_lo, int& i_hi) {
   const int far = max(0, min(sq.Lq, j1 + p.left - sq.off));
   if (chunk < 0) {
     i_lo = max(0, min(sq.Lq, j0 - p.right - sq.off));
-    i_hi = far;
+    i_hi = !p.nst && j0 < p.sinks ? sq.Lq : far;
   } else {
     i_lo = min(sq.Lq, far + chunk * p.ch);
     i_hi = min(sq.Lq, i_lo + p.ch);

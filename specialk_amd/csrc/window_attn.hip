@@ -524,7 +524,12 @@ void set_window(WinParams& p, int window, int causal) {
   const int span = p.Lq + p.Lk;
   p.left = std::min(window - 1, span);
   p.right = causal ? 0 : p.left;
+  if (p.sinks >= p.Lk) p.left = span;   // every key stays visible
   p.sinks = std::min(p.sinks, p.Lk);
+}
+
+int64_t slab_floats(const WinParams& p, int rows) {
+  return ((int64_t)p.B * p.G * p.nst * (1 + p.nch) * 2 * slab_rows(p, rows) * p.d + 3) / 4 * 4;   // (16-byte stores behind)
 }
 
 // Parts of a key tile's window: two blocks for every CU, each with at least four tiles of queries (bf16, 2 x 4096 tokens, 8
@@ -542,6 +547,18 @@ void plan_keys(WinParams& p, int rows) {
   const int64_t less = std::max<int64_t>(64, (span / p.parts + 63) / 64 * 64);
   if (units * p.nst * (p.Lq / less + 1) <= 4 * cus) p.ch = (int)std::min<int64_t>(p.ch, p.parts > 1 ? less : p.ch);
   p.nch = far ? (p.Lq + p.ch - 1) / p.ch : 0;
+  // The sums in memory grow with sinks x Lq / ch.  Where they are large the sink tiles are many, and four blocks for every CU
+  // do: longer chunks, and no chunks where the tiles alone are that many (their blocks sweep the far queries too, query_range).
+  // At most 4096 x rows x d floats then remain, however many sinks (32768 tokens, 8 heads of 128, window 64, 4096 sinks:
+  // 4.3 GB -> 168 MB).
+  if (slab_floats(p, rows) <= 1 << 24) return;
+  const int64_t most = 4 * cus / (units * p.nst);
+  if (most >= 1) {
+    p.ch = std::max<int64_t>(p.ch, ((p.Lq + most - 1) / most + 63) / 64 * 64);
+    p.nch = (p.Lq + p.ch - 1) / p.ch;
+  } else {
+    p.nst = p.nch = 0;
+  }
 }
 
 // Cuts of a query tile's keys: two blocks for every CU, each with at least 12 tiles of 64 keys (fp32 arithmetic: 8).  64
@@ -563,9 +580,6 @@ bool grids_fit(const WinParams& p) {
          (p.nst == 0 || (int64_t)p.sinks * p.d < (1ll << 31));
 }
 
-int64_t slab_floats(const WinParams& p, int rows) {
-  return ((int64_t)p.B * p.G * p.nst * (1 + p.nch) * 2 * slab_rows(p, rows) * p.d + 3) / 4 * 4;   // (16-byte stores behind)
-}
 int64_t split_floats(const WinParams& p) { return p.parts > 1 ? 2ll * p.parts * p.B * p.Lk * p.G * p.d : 0; }
 
 template <typename T, int D>

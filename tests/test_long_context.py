@@ -231,3 +231,15 @@ def test_workspace_sizes():
                                          0, 1, ws, n, 0, None) == code
     assert lib.skhip_window_attn_step_ws_floats(65535, 8, 8, 64, 4096, 4096, 0) == 0
     assert lib.skhip_window_attn_step_ws_floats(1, 8, 8, 64, 4096, 4096, 0) > 0
+
+
+def test_backward_workspace_of_many_sinks():
+    """The sums of the first keys' far queries stay within 2 ^ 24 floats or 4 blocks a CU, however many first keys there are."""
+    lib = L.load()
+    for B, H, G, n, d, window, sinks in ((1, 8, 8, 32768, 128, 64, 4096), (1, 8, 8, 32768, 128, 1, 32768), (4, 8, 8, 8192, 64, 64, 8191),
+                                         (4, 8, 8, 8192, 64, 64, 4096), (1, 32, 8, 32768, 128, 256, 4096),
+                                         (1, 8, 8, 32768, 128, 64, 16384), (64, 8, 8, 4096, 64, 100, 500), (1, 1, 1, 1 << 20, 64, 10, 5000)):
+        got = lib.skhip_window_attn_bwd_ws_floats(B, H, G, B * n, n, n, d, window, sinks, 1)
+        rest = lib.skhip_window_attn_bwd_ws_floats(B, H, G, B * n, n, n, d, window, 0, 1)
+        # 256 CUs: 4 * 256 blocks and as many tiles' own windows, each of 128 rows of dK and dV
+        assert got - rest <= max(1 << 24, 2 * 4 * 256 * 2 * 128 * d), (got, rest)

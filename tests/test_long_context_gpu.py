@@ -938,3 +938,48 @@ def test_one_row_of_any_stride(dtype):
     assert k2.shape == k1.shape and k2.stride(1) < H * d
     assert torch.equal(ops.window_attention_step(x, y, z, k2, v2, length, H), want)
     assert torch.equal(k2, k1) and torch.equal(v2, v1)
+
+
+# ------------------------------------------------------------------------------ many first keys
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("n,m,sinks", [(200, 200, 200), (200, 200, 1000), (150, 90, 90), (70, 260, 260)])
+def test_window_all_keys_are_sinks(n, m, sinks, causal, dtype):
+    """Every key stays visible: windows no longer matter to the past."""
+    run_window([n], [m], 2, 1, 64, 5, sinks, causal, dtype, "dense", seed=9)
+
+
+def many_sinks(B, n, H, G, d, window, sinks, dtype, packed, causal=True):
+    """A few rows of every gradient in 64 bits, all of the others through the same call on fewer heads at a time."""
+    g = torch.Generator().manual_seed(22)
+    T = B * n
+    q, k, v, do = rnd((T, H * d), dtype, g), rnd((T, G * d), dtype, g), rnd((T, G * d), dtype, g), rnd((T, H * d), dtype, g)
+    off = torch.arange(0, T + 1, n, dtype=torch.int32, device=DEV) if packed else None
+    leaves = [t.to(DEV).requires_grad_() for t in (q, k, v)]
+    o = ops.window_attention(*leaves, B, n, n, H, G, window, sinks, causal, q_off=off, k_off=off)
+    grads = torch.autograd.grad(o, leaves, do.to(DEV))
+    for b, h in ((0, 0), (B - 1, H - 1)):
+        kh, rs = h // (H // G), slice(b * n, b * n + n)
+        vis = visible(n, n, window, sinks, causal)
+        want = [torch.zeros((n, d), dtype=torch.float64) for _ in range(4)]
+        bound = [torch.full((n, d), TINY, dtype=torch.float64) for _ in range(4)]
+        for hh in range(kh * (H // G), (kh + 1) * (H // G)):
+            hs, ks = slice(hh * d, hh * d + d), slice(kh * d, kh * d + d)
+            res = attention64(q[rs, hs], k[rs, ks], v[rs, ks], do[rs, hs], vis, d ** -0.5, dtype)
+            for i in range(4):
+                if i >= 2 or hh == h:
+                    want[i] += res[i][0]
+                    bound[i] += res[i][1]
+        for i, (got, x) in enumerate(zip((o,) + grads, (h, h, kh, kh))):
+            check(got[rs, x * d:x * d + d], want[i], bound[i], ("o", "dq", "dk", "dv")[i])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("case", [  # B, n, H, G, d, window, sinks: longer chunks, fewer of them, and none
+    (4, 1400, 16, 16, 128, 20, 700), (6, 1100, 16, 16, 64, 9, 1000), (24, 700, 16, 16, 128, 33, 650), (12, 1000, 32, 16, 96, 33, 777)])
+def test_window_many_sinks(case, dtype):
+    many_sinks(*case, dtype, packed=False)
+
+
+def test_window_many_sinks_packed_both_ways():
+    many_sinks(12, 1000, 16, 16, 128, 33, 990, BF, packed=True, causal=False)
