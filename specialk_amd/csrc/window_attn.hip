@@ -565,8 +565,9 @@ void plan_keys(WinParams& p, int rows) {
 // queries at the end of 32768 keys, 8 heads of 128, all visible: 8 blocks alone 649 us, cut 54, with the backward pass 1262
 // and 186 (fp32 4276 and 148, 5861 and 737); 4096 tokens, 4 heads of 64, causal: 74 and 41.  Shorter sweeps are not worth
 // the join: 2048 tokens, 8 heads of 128, window 1024 (18 tiles): uncut 30, in two 38.
+// (Partial outputs are kept for every row of Q: a packed tensor with more rows than its sequences counts whole.)
 void plan_cuts(WinParams& p, int rows) {
-  const int64_t blocks = std::max<int64_t>(1, (int64_t)p.B * p.H * ((p.Lq + rows - 1) / rows));
+  const int64_t blocks = std::max<int64_t>({1, (int64_t)p.B * p.H * ((p.Lq + rows - 1) / rows), p.H * p.Tq / rows});
   const int64_t tiles = std::min<int64_t>(p.Lk, (int64_t)rows + p.left + p.right + p.sinks) / 64;
   p.cuts = (int)std::max<int64_t>(1, std::min({2 * (int64_t)sk_num_cus() / blocks, tiles / (rows == NT ? 8 : 12), (int64_t)64}));
 }

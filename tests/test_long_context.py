@@ -243,3 +243,14 @@ def test_backward_workspace_of_many_sinks():
         rest = lib.skhip_window_attn_bwd_ws_floats(B, H, G, B * n, n, n, d, window, 0, 1)
         # 256 CUs: 4 * 256 blocks and as many tiles' own windows, each of 128 rows of dK and dV
         assert got - rest <= max(1 << 24, 2 * 4 * 256 * 2 * 128 * d), (got, rest)
+
+
+def test_workspace_of_few_queries_in_a_large_packed_tensor():
+    """Rows outside every sequence are only zeroed: their partial results are not multiplied by the cuts."""
+    lib = L.load()
+    few = lib.skhip_window_attn_fwd_ws_floats(1, 8, 8, 64, 64, 32768, 128, 32768, 0, 1)
+    assert few > 0
+    for Tq in (1 << 16, 1 << 20):
+        assert lib.skhip_window_attn_fwd_ws_floats(1, 8, 8, Tq, 64, 32768, 128, 32768, 0, 1) <= few * 2, Tq
+        back = lib.skhip_window_attn_bwd_ws_floats(1, 8, 8, Tq, 64, 32768, 128, 32768, 0, 1)
+        assert back - 2 * 8 * Tq <= 2 * lib.skhip_window_attn_bwd_ws_floats(1, 8, 8, 64, 64, 32768, 128, 32768, 0, 1), Tq

@@ -983,3 +983,29 @@ def test_window_many_sinks(case, dtype):
 
 def test_window_many_sinks_packed_both_ways():
     many_sinks(12, 1000, 16, 16, 128, 33, 990, BF, packed=True, causal=False)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows", [70, 3000])
+def test_window_queries_in_cuts_inside_a_larger_tensor(rows, dtype):
+    """Few packed queries before many keys, further rows around them: the result of the queries alone, zeros elsewhere."""
+    g = torch.Generator().manual_seed(23)
+    H, d, n, m = 2, 64, 40, 3000
+    q, do = (rnd((rows, H * d), dtype, g).to(DEV) for _ in range(2))
+    k, v = (rnd((m, H * d), dtype, g).to(DEV) for _ in range(2))
+    first = rows - n - 9
+    q_off, k_off = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([first, first + n], [0, m]))
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    o = ops.window_attention(*leaves, 1, n, m, H, q_off=q_off, k_off=k_off)
+    got = (o,) + torch.autograd.grad(o, leaves, do)
+    few = slice(first, first + n)
+    alone = [q[few].clone().requires_grad_(), k.clone().requires_grad_(), v.clone().requires_grad_()]
+    o = ops.window_attention(*alone, 1, n, m, H)
+    want = (o,) + torch.autograd.grad(o, alone, do[few])
+    for a, b, name in zip(got, want, ("o", "dq", "dk", "dv")):
+        if name in ("o", "dq"):
+            assert not a[:first].any() and not a[first + n:].any()
+            a = a[few]
+        # (cut or not: the same sums in another order; bf16 results are within a step of each other, as each is within
+        # test_window_queries_in_cuts' bounds of one exact value)
+        torch.testing.assert_close(a.float(), b.float(), rtol=2 * unit(dtype) + 1e-5, atol=(unit(dtype) + 1e-6) * b.abs().max().item())
