@@ -615,13 +615,13 @@ void launch_bwd(const WinParams& p, hipStream_t stream) {
 }  // namespace
 
 int sk_window_join(const WinParams& p, int rows, int dtype, hipStream_t stream) {
-  if (p.cuts > 1 && p.Tq) {
+  if (p.cuts > 1 && p.B && p.Lq) {
     const dim3 all((unsigned)(((int64_t)p.Lq * p.H * p.d + 255) / 256), p.B);
     if (dtype == SK_BF16) hipLaunchKernelGGL((window_cut_sum_kernel<bf16_t>), all, dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((window_cut_sum_kernel<float>), all, dim3(256), 0, stream, p);
     SK_CHECK_LAUNCH("skhip_window_attn_bwd(join)");
   }
-  if ((!p.nst && p.parts == 1) || !p.Tk) return SK_OK;
+  if ((!p.nst && p.parts == 1) || !p.B || !p.Lk) return SK_OK;   // (no sequence has keys: no grid)
   if (p.parts > 1) {
     const dim3 all((unsigned)(((int64_t)p.Lk * p.G * p.d + 255) / 256), p.B);
     if (dtype == SK_BF16) hipLaunchKernelGGL((window_split_join_kernel<bf16_t>), all, dim3(256), 0, stream, p, rows);
@@ -637,7 +637,7 @@ int sk_window_join(const WinParams& p, int rows, int dtype, hipStream_t stream) 
 }
 
 int sk_window_cut_join(const WinParams& p, int dtype, hipStream_t stream) {
-  if (p.cuts == 1) return SK_OK;
+  if (p.cuts == 1 || !p.B || !p.Lq) return SK_OK;   // (no sequence has queries: no grid)
   const dim3 all((unsigned)(((int64_t)p.Lq * p.H * p.d + 255) / 256), p.B);
   if (dtype == SK_BF16) hipLaunchKernelGGL((window_cut_join_kernel<bf16_t>), all, dim3(256), 0, stream, p);
   else hipLaunchKernelGGL((window_cut_join_kernel<float>), all, dim3(256), 0, stream, p);

@@ -1009,3 +1009,24 @@ def test_window_queries_in_cuts_inside_a_larger_tensor(rows, dtype):
         # (cut or not: the same sums in another order; bf16 results are within a step of each other, as each is within
         # test_window_queries_in_cuts' bounds of one exact value)
         torch.testing.assert_close(a.float(), b.float(), rtol=2 * unit(dtype) + 1e-5, atol=(unit(dtype) + 1e-6) * b.abs().max().item())
+
+
+# ------------------------------------------------------------------------------ batches of nothing
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_packed_rows_without_sequences(dtype):
+    """No sequence at all, or none with queries, or none with keys, before tensors that hold rows: zeros."""
+    g = torch.Generator().manual_seed(21)
+    H, d, n, m = 2, 64, 6, 5000
+    off = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    for q_off, k_off, Lq, Lk in ((off(0), off(0), n, m), (off(0, 0), off(0, m), 0, m), (off(0, n), off(0, 0), n, 0), (off(2, 2), off(9, 9), 0, 0)):
+        for n_kv, sinks in ((H, 0), (1, 300)):
+            q, do = rnd((n, H * d), dtype, g).to(DEV).requires_grad_(), rnd((n, H * d), dtype, g).to(DEV)
+            k, v = (rnd((m, n_kv * d), dtype, g).to(DEV).requires_grad_() for _ in range(2))
+            o = ops.window_attention(q, k, v, q_off.numel() - 1, Lq, Lk, H, n_kv, 4000, sinks, q_off=q_off, k_off=k_off)
+            for t in (o,) + torch.autograd.grad(o, (q, k, v), do):
+                assert not t.any(), (Lq, Lk, n_kv)
+    q, do = rnd((4000, H * d), dtype, g).to(DEV).requires_grad_(), rnd((4000, H * d), dtype, g).to(DEV)
+    k, v = (rnd((3, d), dtype, g).to(DEV).requires_grad_() for _ in range(2))
+    o = ops.window_attention(q, k, v, 1, 4000, 0, H, 1, q_off=off(0, 4000), k_off=off(0, 0))
+    for t in (o,) + torch.autograd.grad(o, (q, k, v), do):
+        assert not t.any()
