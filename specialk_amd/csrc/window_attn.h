@@ -40,6 +40,8 @@ struct WinParams {
   float *cut_o, *cut_ml;
 };
 
+constexpr int FEW = 32;   // bf16 rows that see no more keys: delta = rowsum(dO O) is not taken from the rounded O
+
 struct Seq { int64_t qbase, kbase; int Lq, Lk, off; };
 
 __device__ __forceinline__ Seq seq_of(const WinParams& p, int b) {

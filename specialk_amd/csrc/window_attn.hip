@@ -16,6 +16,7 @@
 // 100 - 1000 tokens, window 256: forward 77, dQ 101, dK and dV 154 us, 4.6 blocks of 5.5 tiles a CU in all).
 #include "window_attn.h"
 #include <algorithm>
+#include <type_traits>
 
 using namespace skwin;
 
@@ -171,15 +172,17 @@ template <typename T, int D> struct KeySweep {
     if (beg < end) load(beg);
   }
   __device__ __forceinline__ int start(int t) const { return kt.start<NT>(t); }
+  __device__ __forceinline__ int padding(int t) const { return pad ? pad[min(start(t) + (int)(threadIdx.x & 63), sq.Lk - 1)] : 0; }
+  __device__ __forceinline__ uint64_t usable(int t, int no) const { return __ballot(kt.holds(start(t) + (int)(threadIdx.x & 63)) && !no); }
   __device__ __forceinline__ void load(int t) {
     const int j0 = start(t);
-    if (pad) gone = pad[min(j0 + (int)(threadIdx.x & 63), sq.Lk - 1)];
+    gone = padding(t);
     k.load(K, p.ldk, j0, sq.Lk, p.d, p.vec);
     v.load(V, p.ldv, j0, sq.Lk, p.d, p.vec);
   }
   // tile t into LDS; the next one on its way.  Returns the keys that may be used.
   __device__ __forceinline__ uint64_t next(int t, Tile<D>& Ks, Tile<D>& Vs) {
-    const uint64_t ok = __ballot(kt.holds(start(t) + (int)(threadIdx.x & 63)) && !gone);
+    const uint64_t ok = usable(t, gone);
     __syncthreads();
     k.store(Ks, ok, p.d);
     v.store(Vs, ok, p.d);
@@ -284,6 +287,17 @@ __global__ __launch_bounds__(256, BLOCKS(D)) void window_dq_kernel(WinParams p) 
   const int i = i0 + wave * 16 + c, pos = i + sq.off;
   const int64_t row = sq.qbase + min(i, sq.Lq - 1), si = (int64_t)h * p.Tq + row;
   KeySweep<T, D> keys(p, sq, b, kh, i0, cut, p.cuts);
+  // bf16 rows of few keys: delta in fp32 from a sweep of its own, since O carries two roundings to 2^-8 (window_attn_mfma.hip)
+  bool few_row = false, few = false;
+  if constexpr (sizeof(T) == 2) {
+    int count = 0;
+    for (int t = keys.kt.n - 1; t >= 0; --t) {
+      count += __popcll(keys_seen(p, pos, keys.start(t), keys.usable(t, keys.padding(t))));
+      if (__all(count > FEW || i >= sq.Lq)) break;
+    }
+    few_row = i < sq.Lq && count <= FEW;
+    few = __syncthreads_or(few_row);
+  }
   f32x4_t fq[D / 16], fd[D / 16], dq[D / 16];
   load_own<T, D>(fq, (const T*)p.O + row * p.ldo + (int64_t)h * p.d, p.d, g, i < sq.Lq);
   load_own<T, D>(fd, (const T*)p.dO + row * p.lddo + (int64_t)h * p.d, p.d, g, i < sq.Lq);
@@ -297,21 +311,41 @@ __global__ __launch_bounds__(256, BLOCKS(D)) void window_dq_kernel(WinParams p) 
   dl = quad_sum(dl);
   load_own<T, D>(fq, (const T*)p.Q + row * p.ldq + (int64_t)h * p.d, p.d, g, i < sq.Lq);
   const float cs = p.scale * LOG2E, lse2 = p.LSE[si] * LOG2E;
-  if (i < sq.Lq && g == 0 && cut == 0) p.delta[si] = dl;
-  for (int t = keys.beg; t < keys.end; ++t) {
-    const uint64_t ok = keys.next(t, Ks, Vs), see = i < sq.Lq ? keys_seen(p, pos, keys.start(t), ok) : 0;
-    const uint64_t mk = see >> (4 * g);
+  auto sweep = [&](auto delta_only) {
+    float sum = 0.f;
+    for (int t = keys.beg; t < keys.end; ++t) {
+      const uint64_t ok = keys.next(t, Ks, Vs), see = i < sq.Lq ? keys_seen(p, pos, keys.start(t), ok) : 0;
+      const uint64_t mk = see >> (4 * g);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (!piece(see, k)) continue;
-      f32x4_t ds = dot_rows<D>(Ks, 16 * k, fq, lane);
-      const f32x4_t dp = dot_rows<D>(Vs, 16 * k, fd, lane);
+      for (int k = 0; k < 4; ++k) {
+        if (!piece(see, k)) continue;
+        f32x4_t ds = dot_rows<D>(Ks, 16 * k, fq, lane);
+        const f32x4_t dp = dot_rows<D>(Vs, 16 * k, fd, lane);
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        ds[r] = keep_or(__builtin_amdgcn_exp2f(fmaf(ds[r], cs, -lse2)) * (dp[r] - dl), mk, k, r, 0u);
-      add_cols<D>(dq, Ks, 16 * k, ds, lane);
+        for (int r = 0; r < 4; ++r) {
+          ds[r] = keep_or(__builtin_amdgcn_exp2f(fmaf(ds[r], cs, -lse2)) * (delta_only ? dp[r] : dp[r] - dl), mk, k, r, 0u);
+          if (delta_only) sum += ds[r];
+        }
+        if constexpr (!delta_only) add_cols<D>(dq, Ks, 16 * k, ds, lane);
+      }
+    }
+    return sum;
+  };
+  if constexpr (sizeof(T) == 2) {
+    if (few) {
+      const int beg = keys.beg, end = keys.end;
+      keys.beg = 0;
+      keys.end = max(0, keys.kt.n);
+      if (keys.end > 0) keys.load(0);
+      const float exact = quad_sum(sweep(std::true_type{}));
+      dl = few_row ? exact : dl;
+      keys.beg = beg;
+      keys.end = end;
+      if (beg < end) keys.load(beg);
     }
   }
+  if (i < sq.Lq && g == 0 && cut == 0) p.delta[si] = dl;
+  sweep(std::false_type{});
   if (p.cuts > 1) {
     if (i < sq.Lq) store_own<float, D>(p.cut_o + (((int64_t)cut * p.H + h) * p.Tq + row) * p.d, dq, p.scale, p.d, g);
     return;

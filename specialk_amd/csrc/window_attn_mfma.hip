@@ -306,7 +306,6 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void fwd_kernel(WinParams p, 
 // are then 1.4 instead of 1.65 times as far from the exact values as a result rounded once.  Waves without such rows
 // sit that sweep out, and two tiles or fewer stay in LDS for the second (256 causal texts of 100 tokens, 8 heads of 64: dQ
 // 47.5 -> 41.5 us).
-constexpr int FEW = 32;
 template <int D, int W>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dq_kernel(WinParams p, int qtiles) {
   __shared__ __attribute__((aligned(1024))) char lds[2][2 * tile_bytes<D>()];

@@ -1030,3 +1030,47 @@ def test_packed_rows_without_sequences(dtype):
     o = ops.window_attention(q, k, v, 1, 4000, 0, H, 1, q_off=off(0, 4000), k_off=off(0, 0))
     for t in (o,) + torch.autograd.grad(o, (q, k, v), do):
         assert not t.any()
+
+
+# ------------------------------------------------------------------------------ gradients of rows that see few keys
+def few_keys64(q, k, v, do, vis, scale, operands):
+    """dq, dk of one sequence and head with bounds that hold delta = sum_j P_j dP_j to fp32: no rounding of the output in them.
+    operands: what a value of dS loses as an operand of the last product (0: fp32 arithmetic)."""
+    q, k, v, do = (t.double() for t in (q, k, v, do))
+    n, d, u = vis.sum(1).max().item(), q.shape[1], unit(BF)
+    p = torch.softmax((q @ k.t() * scale).masked_fill(~vis, -math.inf), 1) * vis
+    dp = do @ v.t()
+    ds = p * (dp - (p * dp).sum(1, keepdim=True)) * scale
+    smax = (q.abs() @ k.abs().t() * abs(scale) * vis).max()
+    rel = (2 * (d + 6) * smax + 2 * n + 16) * E          # of a probability, as in attention64
+    edp = (d + 2) * E * (do.abs() @ v.abs().t())
+    edelta = (p * (dp.abs() * (rel + (n + 2) * E) + edp)).sum(1, keepdim=True)
+    # of a probability times a difference: its own error, that of the difference, and one step of its operands' sizes
+    eds = ds.abs() * (operands + rel + 4 * E) + p * abs(scale) * (edelta + edp + E * (dp.abs() + (p * dp).sum(1, keepdim=True).abs()))
+    acc = (max(vis.shape) + 8) * E
+    return ((ds @ k, u * (ds @ k).abs() + eds @ k.abs() + acc * ds.abs() @ k.abs()),
+            (ds.t() @ q, u * (ds.t() @ q).abs() + eds.t() @ q.abs() + acc * ds.abs().t() @ q.abs()))
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (2, 0), (1, 1), (5, 2), (8, 24)])
+@pytest.mark.parametrize("d,shift", [(64, 0), (128, 0), (37, 0), (64, 1), (100, 0)])
+def test_gradients_of_rows_with_few_keys(d, shift, window, sinks):
+    """bf16 rows of at most 32 visible keys, on whole 16-byte pieces and on odd rows."""
+    g = torch.Generator().manual_seed(24)
+    n, H, G = 170, 2, 1
+    x = torch.zeros((n, (H + 2 * G) * d + shift), dtype=BF)
+    x[:, shift:] = rnd((n, (H + 2 * G) * d), BF, g)
+    do = rnd((n, H * d), BF, g)
+    cut = lambda t: (t[:, shift:shift + H * d], t[:, shift + H * d:shift + (H + G) * d], t[:, shift + (H + G) * d:])
+    leaves = [t.detach().requires_grad_() for t in cut(x.to(DEV))]
+    o = ops.window_attention(*leaves, 1, n, n, H, G, window, sinks)
+    dq, dk, _ = torch.autograd.grad(o, leaves, do.to(DEV))
+    q, k, v = cut(x)
+    vis = visible(n, n, window, sinks, True)
+    want, bound = torch.zeros((n, d), dtype=torch.float64), torch.full((n, d), TINY, dtype=torch.float64)
+    for h in range(H):
+        s = slice(h * d, h * d + d)
+        a, b = few_keys64(q[:, s], k, v, do[:, s], vis, d ** -0.5, unit(BF) if d % 8 == 0 and shift % 8 == 0 else 0.0)
+        check(dq[:, s], a[0], a[1] + TINY, ("dq", h))
+        want, bound = want + b[0], bound + b[1]
+    check(dk, want, bound, "dk")
