@@ -6,6 +6,7 @@ stream; no arithmetic on the hot path is done by torch itself.  Parameters stay 
 bfloat16 the kernels read bf16 working copies kept by `compute_weight` and weight
 gradients are produced directly in fp32.
 """
+import decimal
 import itertools
 import math
 import weakref
@@ -967,6 +968,9 @@ class EmbedFn(torch.autograd.Function):
 
 
 # ----------------------------------------------------------------------------- rotary positions, norms of heads
+PI = "3.14159265358979323846264338327950288419716939937510582097494459"
+
+
 class RotaryFrequencies:
     """The turn per position of each pair of a head's rotated part, for `rotary` and `qk_norm_rotary`.
 
@@ -977,7 +981,8 @@ class RotaryFrequencies:
       "yarn"    pairs that turn fewer than once within trained_len are divided by factor, those that turn more than 32
                 times kept, the others blended by their number of turns; rotated pairs are scaled by 0.1 ln(factor) + 1
                 (the attention temperature that goes with it).
-    Frequencies are kept as 64-bit fractions of a turn, so any int64 position has its angle without rounding."""
+    Frequencies are kept as 64-bit fractions of a turn, each within 2^-65 of the formula's, and a position's angle is the exact
+    product: it is off by at most |position| 2^-65 turns (2 10^-13 rad a million positions on)."""
 
     def __init__(self, rot_dim, base=10000.0, scaling=None, factor=1.0, trained_len=0, device="cuda"):
         if rot_dim < 0 or rot_dim % 2:
@@ -990,18 +995,27 @@ class RotaryFrequencies:
             raise ValueError('"ntk" needs more than one pair')
         if scaling == "yarn" and (trained_len <= 0 or factor < 1):
             raise ValueError('"yarn" needs trained_len and a factor of at least 1')
-        if scaling == "ntk":
-            base = base * factor ** (rot_dim / (rot_dim - 2))
-        radians = [base ** (-2.0 * i / rot_dim) for i in range(rot_dim // 2)]
-        self.rot_dim, self.amplitude = rot_dim, 1.0
-        if scaling == "linear":
-            radians = [f / factor for f in radians]
-        elif scaling == "yarn":
-            keep = [min(1.0, max(0.0, (trained_len * f / (2 * math.pi) - 1.0) / 31.0)) for f in radians]
-            radians = [f / factor * (1.0 - g) + f * g for f, g in zip(radians, keep)]
-            self.amplitude = 0.1 * math.log(factor) + 1.0
-        words = [round(math.fmod(f / (2 * math.pi), 1.0) * 2.0 ** 64) % (1 << 64) for f in radians]
-        self.radians = radians
+        # (in doubles the frequencies' 53 bits would be half a radian off at position 2^53)
+        with decimal.localcontext(decimal.Context(prec=60, rounding=decimal.ROUND_HALF_EVEN, traps=[decimal.InvalidOperation])):
+            b, s, n = (decimal.Decimal(float(x)) for x in (base, factor, trained_len))
+            turn, rot = 2 * decimal.Decimal(PI), int(rot_dim)
+            if scaling == "ntk":
+                b *= s ** (decimal.Decimal(rot) / (rot - 2))
+            radians, step = [decimal.Decimal(1)], b ** (decimal.Decimal(-2) / max(rot, 2))
+            for _ in range(rot // 2 - 1):
+                radians.append(radians[-1] * step)
+            radians = radians[:rot // 2]
+            if scaling == "linear":
+                radians = [f / s for f in radians]
+            elif scaling == "yarn":
+                keep = [min(1, max(0, (n * f / turn - 1) / 31)) for f in radians]
+                radians = [f / s * (1 - g) + f * g for f, g in zip(radians, keep)]
+            if any(f > 1 << 64 for f in radians):
+                raise ValueError(f"base {base} and factor {factor} give more than 2^64 radians per position")
+            words = [int((f / turn % 1 * (1 << 64)).to_integral_value()) % (1 << 64) for f in radians]
+        self.rot_dim = rot_dim
+        self.amplitude = 0.1 * math.log(factor) + 1.0 if scaling == "yarn" else 1.0
+        self.radians = [float(f) for f in radians]
         self.turns = torch.tensor([w - (1 << 64) if w >> 63 else w for w in words], dtype=torch.int64).to(device)
 
 

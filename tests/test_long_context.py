@@ -1,7 +1,9 @@
 """Refusals of the rotary / query-key norm / windowed-attention operators, on the CPU, and what their frequency tables
 hold."""
+import decimal
 import math
 
+import numpy as np
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -26,6 +28,48 @@ def test_turns_are_the_frequencies_as_fractions_of_a_turn():
         # a double holds the frequency to 2^-53; the word adds at most half a unit of 2^-64 turns
         want = 10000.0 ** (-2.0 * i / 64) / (2 * math.pi)
         assert abs(w / 2.0 ** 64 - want) <= want * 2.0 ** -50 + 2.0 ** -65
+
+
+def formula(rot, base, scaling, factor, trained_len):
+    """Turns per position of every pair, to 70 digits, from the formulas: logarithms and exponentials instead of powers."""
+    with decimal.localcontext(decimal.Context(prec=70)):
+        D = decimal.Decimal
+        arctan = lambda n: sum(D((-1) ** k) / ((2 * k + 1) * D(n) ** (2 * k + 1)) for k in range(60))
+        turn = 8 * (4 * arctan(5) - arctan(239))                     # 2 pi by Machin
+        ln = D(base).ln()
+        if scaling == "ntk":
+            ln += D(factor).ln() * rot / (rot - 2)
+        out = []
+        for i in range(rot // 2):
+            f = (-ln * 2 * i / rot).exp() / turn
+            r = trained_len * f                                      # turns within the trained length
+            if scaling == "linear" or (scaling == "yarn" and r <= 1):
+                f /= D(factor)
+            elif scaling == "yarn" and r < 32:                       # between: (r - 1) of 31 parts kept
+                f *= ((r - 1) + (32 - r) / D(factor)) / 31
+            out.append(f)
+        return out
+
+
+@pytest.mark.parametrize("rot,base", [(4, 10000.0), (64, 10000.0), (36, 500000.0), (128, 1e6)])
+@pytest.mark.parametrize("scaling,factor,trained_len", [(None, 1.0, 0), ("linear", 3.7, 0), ("ntk", 8.0, 0), ("yarn", 32.0, 4096),
+                                                        ("yarn", 1.5, 131072)])
+def test_every_turn_is_its_formula_to_half_a_unit(rot, base, scaling, factor, trained_len):
+    f = freqs(rot, base=base, scaling=scaling, factor=factor, trained_len=trained_len)
+    want = formula(rot, base, scaling, factor, trained_len)
+    assert len(f.turns) == len(want) == rot // 2
+    for got, w in zip(f.turns.tolist(), want):
+        # rounded once: half a unit of 2^-64, and what 60 digits leave out
+        assert abs(got % (1 << 64) - w * (1 << 64)) <= decimal.Decimal("0.5000001")
+    assert f.radians == pytest.approx([float(w) * 2 * math.pi for w in want], rel=1e-14)
+
+
+def test_frequencies_of_other_number_types():
+    want = freqs(64, scaling="yarn", factor=4.0, trained_len=2048, base=10000.0).turns
+    for num in (int, np.float32, np.float64, np.int64):
+        assert torch.equal(freqs(np.int64(64), scaling="yarn", factor=num(4), trained_len=num(2048), base=num(10000)).turns, want)
+    with pytest.raises(ValueError, match="2\\^64"):
+        freqs(8, base=1e-300)
 
 
 @pytest.mark.parametrize("scaling", ["linear", "ntk", "yarn"])

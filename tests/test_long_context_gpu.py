@@ -3,6 +3,7 @@
 Tolerances are bounds per element, from the roundings a result goes through: U = half a step of the storage type (2^-8
 bf16, 2^-24 fp32) for every value that is stored in it, E = 2^-24 for every fp32 operation, multiplied by the absolute
 values that the rounded quantities meet on the way to the element."""
+import decimal
 import math
 
 import pytest
@@ -1074,3 +1075,30 @@ def test_gradients_of_rows_with_few_keys(d, shift, window, sinks):
         check(dq[:, s], a[0], a[1] + TINY, ("dq", h))
         want, bound = want + b[0], bound + b[1]
     check(dk, want, bound, "dk")
+
+
+# ------------------------------------------------------------------------------ very far positions
+@pytest.mark.parametrize("il", [False, True])
+@pytest.mark.parametrize("far", [1 << 32, -(1 << 45), (1 << 53) + 1, 1 << 56])
+def test_rotary_very_far_positions(far, il):
+    """Angles from the formula in 60 digits: off by at most half a unit of 2^-64 turns a position."""
+    g = torch.Generator().manual_seed(25)
+    T, H, d, rot = 20, 2, 64, 48
+    pos = torch.randint(0, 300, (T,), generator=g) + far
+    x = rnd((T, H * d), F32, g)
+    f = ops.RotaryFrequencies(rot, device=DEV)
+    out, _ = ops.rotary(x.to(DEV), None, pos.to(DEV), f, H, interleaved=il)
+    with decimal.localcontext(decimal.Context(prec=60)):
+        turn = 2 * decimal.Decimal("3.14159265358979323846264338327950288419716939937510582097494")
+        ln = decimal.Decimal(10000).ln()
+        per = [(-ln * 2 * i / rot).exp() / turn for i in range(rot // 2)]
+        ang = torch.tensor([[float(p * t % 1) * 2 * math.pi for t in per] for p in pos.tolist()], dtype=torch.float64)[:, None]
+    h = x.double().view(T, H, d)
+    a, b = (h[..., 0:rot:2], h[..., 1:rot:2]) if il else (h[..., :rot // 2], h[..., rot // 2:rot])
+    y = (a * torch.cos(ang) - b * torch.sin(ang), b * torch.cos(ang) + a * torch.sin(ang))
+    m = a.abs() + b.abs()
+    join = (lambda u, v: torch.stack((u, v), -1).flatten(-2)) if il else (lambda u, v: torch.cat((u, v), -1))
+    want = torch.cat((join(*y), h[..., rot:]), -1)
+    mag = torch.cat((join(m, m), h[..., rot:].abs()), -1)
+    off = pos.abs().max().item() * 2.0 ** -65 * 2 * math.pi + 2.0 ** -50   # (and this reference's own angles)
+    check(out, want.view(T, -1), (E * want.abs() + (ROT_E + off) * mag).view(T, -1), "far")
