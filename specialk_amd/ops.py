@@ -1016,7 +1016,8 @@ class RotaryFrequencies:
         self.rot_dim = rot_dim
         self.amplitude = 0.1 * math.log(factor) + 1.0 if scaling == "yarn" else 1.0
         self.radians = [float(f) for f in radians]
-        self.turns = torch.tensor([w - (1 << 64) if w >> 63 else w for w in words], dtype=torch.int64).to(device)
+        with torch.inference_mode(False):   # (made lazily by an evaluation, it still serves training)
+            self.turns = torch.tensor([w - (1 << 64) if w >> 63 else w for w in words], dtype=torch.int64).to(device)
 
 
 def _rows(x, width, what):
@@ -1077,19 +1078,19 @@ class QKRotaryFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, pos, freqs, n_head, n_kv, interleaved):
-        ctx.save_for_backward(pos)
-        ctx.args = (freqs.turns, freqs.amplitude, None, None, 0.0, n_head, n_kv, q.shape[1] // n_head, freqs.rot_dim, interleaved)
+        ctx.save_for_backward(pos, freqs.turns)
+        ctx.args = (freqs.amplitude, None, None, 0.0, n_head, n_kv, q.shape[1] // n_head, freqs.rot_dim, interleaved)
         with L.on_device(q):
-            return L.qk_rotary(q, k, pos, *ctx.args)
+            return L.qk_rotary(q, k, pos, freqs.turns, *ctx.args)
 
     @staticmethod
     def backward(ctx, dq, dk):
         _once()
-        (pos,) = ctx.saved_tensors
-        n_head, n_kv, d = ctx.args[5:8]
+        pos, turns = ctx.saved_tensors
+        n_head, n_kv, d = ctx.args[4:7]
         dq = _rows(dq, n_head * d, "dq")
         with L.on_device(dq):
-            dq, dk = L.qk_rotary(dq, None if dk is None else _rows(dk, n_kv * d, "dk"), pos, *ctx.args, inverse=True)
+            dq, dk = L.qk_rotary(dq, None if dk is None else _rows(dk, n_kv * d, "dk"), pos, turns, *ctx.args, inverse=True)
         return dq, dk, None, None, None, None, None
 
 
@@ -1099,23 +1100,21 @@ class QKNormRotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, gamma_q, gamma_k, pos, freqs, n_head, n_kv, eps, interleaved):
         gq, gk = gamma_q.detach(), None if gamma_k is None else gamma_k.detach()
-        rot = 0 if freqs is None else freqs.rot_dim
-        ctx.save_for_backward(q, k, gamma_q, gamma_k, pos)
-        ctx.freqs, ctx.rest = freqs, (eps, n_head, n_kv, q.shape[1] // n_head, rot, interleaved)
+        turns, ctx.amplitude, rot = (None, 1.0, 0) if freqs is None else (freqs.turns, freqs.amplitude, freqs.rot_dim)
+        ctx.save_for_backward(q, k, gamma_q, gamma_k, pos, turns)
+        ctx.rest = (eps, n_head, n_kv, q.shape[1] // n_head, rot, interleaved)
         with L.on_device(q):
-            return L.qk_rotary(q, k, pos, None if freqs is None else freqs.turns, 1.0 if freqs is None else freqs.amplitude,
-                               gq, gk, *ctx.rest)
+            return L.qk_rotary(q, k, pos, turns, ctx.amplitude, gq, gk, *ctx.rest)
 
     @staticmethod
     def backward(ctx, dq, dk):
         _once()
-        q, k, gq, gk, pos = ctx.saved_tensors
-        f, (_, n_head, n_kv, d, _, _) = ctx.freqs, ctx.rest
+        q, k, gq, gk, pos, turns = ctx.saved_tensors
+        _, n_head, n_kv, d, _, _ = ctx.rest
         dq = _rows(dq, n_head * d, "dq")
         with L.on_device(q):
-            out = L.qk_norm_rotary_bwd(q, k, dq, None if k is None else _rows(dk, n_kv * d, "dk"), pos,
-                                       None if f is None else f.turns, 1.0 if f is None else f.amplitude, gq.detach(),
-                                       None if gk is None else gk.detach(), *ctx.rest)
+            out = L.qk_norm_rotary_bwd(q, k, dq, None if k is None else _rows(dk, n_kv * d, "dk"), pos, turns, ctx.amplitude,
+                                       gq.detach(), None if gk is None else gk.detach(), *ctx.rest)
         return out + (None,) * 6
 
 

@@ -64,6 +64,12 @@ def test_every_turn_is_its_formula_to_half_a_unit(rot, base, scaling, factor, tr
     assert f.radians == pytest.approx([float(w) * 2 * math.pi for w in want], rel=1e-14)
 
 
+def test_frequencies_made_in_inference_mode_serve_training():
+    with torch.inference_mode():
+        f = freqs(8)
+    assert not f.turns.is_inference()
+
+
 def test_frequencies_of_other_number_types():
     want = freqs(64, scaling="yarn", factor=4.0, trained_len=2048, base=10000.0).turns
     for num in (int, np.float32, np.float64, np.int64):

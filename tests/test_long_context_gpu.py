@@ -1102,3 +1102,24 @@ def test_rotary_very_far_positions(far, il):
     mag = torch.cat((join(m, m), h[..., rot:].abs()), -1)
     off = pos.abs().max().item() * 2.0 ** -65 * 2 * math.pi + 2.0 ** -50   # (and this reference's own angles)
     check(out, want.view(T, -1), (E * want.abs() + (ROT_E + off) * mag).view(T, -1), "far")
+
+
+def test_frequencies_may_change_after_the_forward_pass():
+    """The gradient is that of the frequencies the forward pass used, or an error where those are gone."""
+    g = torch.Generator().manual_seed(26)
+    q = rnd((6, 32), F32, g).to(DEV).requires_grad_()
+    gamma, pos, w = torch.ones(16, device=DEV), torch.arange(6, device=DEV), rnd((6, 32), F32, g).to(DEV)
+    calls = (lambda f: ops.rotary(q, None, pos, f, 2)[0], lambda f: ops.qk_norm_rotary(q, None, gamma, None, pos, f, 2)[0])
+    make = lambda: ops.RotaryFrequencies(16, device=DEV, scaling="yarn", factor=4.0, trained_len=64)
+    other = ops.RotaryFrequencies(16, device=DEV, base=77.0)
+    for call in calls:
+        want, = torch.autograd.grad(call(make()), q, w)
+        f = make()
+        y = call(f)
+        f.turns, f.amplitude, f.rot_dim = other.turns, 9.0, 8
+        assert torch.equal(torch.autograd.grad(y, q, w)[0], want)
+        f = make()
+        y = call(f)
+        f.turns.copy_(other.turns)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y, q, w)
