@@ -288,14 +288,12 @@ __global__ __launch_bounds__(256, BLOCKS(D)) void window_dq_kernel(WinParams p) 
   const int64_t row = sq.qbase + min(i, sq.Lq - 1), si = (int64_t)h * p.Tq + row;
   KeySweep<T, D> keys(p, sq, b, kh, i0, cut, p.cuts);
   // bf16 rows of few keys: delta in fp32 from a sweep of its own, since O carries two roundings to 2^-8 (window_attn_mfma.hip)
+  __shared__ int s_few[4][2];
   bool few_row = false, few = false;
   if constexpr (sizeof(T) == 2) {
-    int count = 0;
-    for (int t = keys.kt.n - 1; t >= 0; --t) {
-      count += __popcll(keys_seen(p, pos, keys.start(t), keys.usable(t, keys.padding(t))));
-      if (__all(count > FEW || i >= sq.Lq)) break;
-    }
-    few_row = i < sq.Lq && count <= FEW;
+    const FewKeys fk = few_keys(p, keys.kt, pos, i < sq.Lq, [&](int t) { return keys.padding(t); }, [&](int t, int no) { return keys.usable(t, no); });
+    if (lane == 0) { s_few[wave][0] = fk.lo; s_few[wave][1] = fk.hi; }
+    few_row = fk.row;
     few = __syncthreads_or(few_row);
   }
   f32x4_t fq[D / 16], fd[D / 16], dq[D / 16];
@@ -334,9 +332,9 @@ __global__ __launch_bounds__(256, BLOCKS(D)) void window_dq_kernel(WinParams p) 
   if constexpr (sizeof(T) == 2) {
     if (few) {
       const int beg = keys.beg, end = keys.end;
-      keys.beg = 0;
-      keys.end = max(0, keys.kt.n);
-      if (keys.end > 0) keys.load(0);
+      keys.beg = min(min(s_few[0][0], s_few[1][0]), min(s_few[2][0], s_few[3][0]));
+      keys.end = max(max(s_few[0][1], s_few[1][1]), max(s_few[2][1], s_few[3][1]));
+      if (keys.beg < keys.end) keys.load(keys.beg);
       const float exact = quad_sum(sweep(std::true_type{}));
       dl = few_row ? exact : dl;
       keys.beg = beg;

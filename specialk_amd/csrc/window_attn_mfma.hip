@@ -309,6 +309,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void fwd_kernel(WinParams p, 
 template <int D, int W>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dq_kernel(WinParams p, int qtiles) {
   __shared__ __attribute__((aligned(1024))) char lds[2][2 * tile_bytes<D>()];
+  __shared__ int s_few[4][2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, hf = lane >> 5;
   const Work work = work_of_block(p, qtiles * p.cuts, p.H / p.G, true);
   if (work.none) return;
@@ -352,12 +353,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dq_kernel(WinParams p, i
     load_tile<D>(buf, K + j0 * p.ldk, p.ldk, p.d, ok, wave, lane);
     load_tile<D>(buf + tile_bytes<D>(), V + j0 * p.ldv, p.ldv, p.d, ok, wave, lane);
   };
-  int count = 0;
-  for (int t = kt.n - 1; t >= 0; --t) {
-    count += __popcll(keys_seen(p, pos, kt.start<NT>(t), usable(t, padding(t))));
-    if (__all(count > FEW || i >= sq.Lq)) break;
-  }
-  const bool few_row = i < sq.Lq && count <= FEW, few_wave = __any(few_row), few = __syncthreads_or(few_row);
+  const FewKeys fk = few_keys(p, kt, pos, i < sq.Lq, padding, usable);
+  if (lane == 0) { s_few[wave][0] = fk.lo; s_few[wave][1] = fk.hi; }
+  const bool few_row = fk.row, few_wave = __any(few_row), few = __syncthreads_or(few_row);
   // one half tile: scores and dP; then the half's part of delta, or dS and its product
   auto half_tile = [&](auto delta_only, bool whole, const char* Ks, const char* Vs, int k, uint32_t mk) {
     f32x16_t sc = zero16(), dp = zero16();
@@ -424,7 +422,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void dq_kernel(WinParams p, i
   const int n = max(0, kt.n);
   const bool both = few && n <= 2 && p.cuts == 1;   // (the tiles are then all in LDS when the first sweep ends)
   if (few) {
-    const float exact = other_sum(sweep(std::true_type{}, false, 0, n));
+    const int lo = min(min(s_few[0][0], s_few[1][0]), min(s_few[2][0], s_few[3][0]));
+    const int hi = max(max(s_few[0][1], s_few[1][1]), max(s_few[2][1], s_few[3][1]));
+    const float exact = other_sum(sweep(std::true_type{}, false, both ? 0 : lo, both ? n : hi));
     dl = few_row ? exact : dl;
     if (!both) __syncthreads();   // every wave is done with the tiles
   }

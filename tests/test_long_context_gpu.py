@@ -1123,3 +1123,29 @@ def test_frequencies_may_change_after_the_forward_pass():
         f.turns.copy_(other.turns)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             torch.autograd.grad(y, q, w)
+
+
+@pytest.mark.parametrize("live", [range(0, 9), range(1990, 2000), range(3, 1990, 150), [700], [], range(1200, 1240)])
+@pytest.mark.parametrize("d", [64, 128, 37])
+def test_gradients_where_padding_leaves_few_keys(d, live):
+    """Few queries before keys that are nearly all padding: the keys are cut, and rows of few keys keep their delta."""
+    g = torch.Generator().manual_seed(27)
+    n, m, H = 40, 2000, 1
+    q, do, k, v = (rnd((r, d), BF, g) for r in (n, n, m, m))
+    pads = torch.ones((1, m), dtype=torch.uint8)
+    pads[0, list(live)] = 0
+    leaves = [t.to(DEV).requires_grad_() for t in (q, k, v)]
+    o = ops.window_attention(*leaves, 1, n, m, H, causal=False, key_pad=pads.to(DEV))
+    dq, dk, _ = torch.autograd.grad(o, leaves, do.to(DEV))
+    if len(live) == 0:
+        assert not dq.any() and not dk.any()
+        return
+    keep = list(live)
+    vis = torch.ones((n, len(keep)), dtype=torch.bool)
+    if len(keep) <= 32:
+        a, b = few_keys64(q, k[keep], v[keep], do, vis, d ** -0.5, unit(BF) if d % 8 == 0 else 0.0)
+    else:
+        _, a, b, _ = attention64(q, k[keep], v[keep], do, vis, d ** -0.5, BF)
+    check(dq, a[0], a[1] + TINY, "dq")
+    check(dk[keep], b[0], b[1] + TINY, "dk")
+    assert not dk[pads[0].bool().to(DEV)].any()
