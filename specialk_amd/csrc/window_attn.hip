@@ -27,6 +27,7 @@ constexpr int NT = 64;     // rows per LDS tile
 // tokens, 8 heads, 2 key heads, window 512: 530 us alone, 428 by two; dQ 448 and 327).
 constexpr int BLOCKS(int D) { return D <= 64 ? 3 : 2; }
 constexpr int MAXD = 128;
+constexpr int MAX_LEN = 1 << 29;   // positions, plus a window of both sequences' lengths, stay within 32 bits
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr int MFMA_ROWS = 128;   // key rows of a block of the bf16 path
 
@@ -542,7 +543,7 @@ int check(const char* who, const WinParams& p, int window, int dtype) {
   SK_CHECK_ARG(p.H % p.G == 0, "%s: %d query heads do not share %d key heads evenly", who, p.H, p.G);
   SK_CHECK_ARG(p.d > 0 && p.d <= MAXD, "%s: head size %d must be in 1..%d", who, p.d, MAXD);
   SK_CHECK_ARG(p.H <= 65535 && p.B <= 65534, "%s: more than 65535 heads or 65534 sequences", who);
-  SK_CHECK_ARG(p.Lq <= (1 << 29) && p.Lk <= (1 << 29), "%s: sequences of more than 2^29 positions", who);
+  SK_CHECK_ARG(p.Lq <= MAX_LEN && p.Lk <= MAX_LEN, "%s: sequences of more than 2^29 positions", who);
   SK_CHECK_ARG(window >= 1 && p.sinks >= 0, "%s: window %d must be >= 1 and sinks %d >= 0", who, window, p.sinks);
   SK_CHECK_ARG(!p.q_off == !p.k_off, "%s: one offset array without the other", who);
   SK_CHECK_ARG(!(p.q_off && p.key_pad), "%s: packed rows take no padding mask", who);
@@ -677,9 +678,15 @@ int sk_window_cut_join(const WinParams& p, int dtype, hipStream_t stream) {
   return SK_OK;
 }
 
+// sizes that a call would take (the size queries answer 0 for others)
+static bool sizes_fit(int B, int n_head, int n_kv, int64_t Tq, int Lq, int Lk, int d, int window, int sinks) {
+  return B >= 0 && n_head > 0 && n_kv > 0 && n_head % n_kv == 0 && Tq >= 0 && Lq >= 0 && Lq <= MAX_LEN && Lk >= 0 && Lk <= MAX_LEN &&
+         d > 0 && d <= MAXD && window >= 1 && sinks >= 0;
+}
+
 extern "C" int64_t skhip_window_attn_fwd_ws_floats(int B, int n_head, int n_kv, int64_t Tq, int Lq, int Lk, int d, int window,
                                                    int sinks, int causal) {
-  if (B < 0 || n_head <= 0 || n_kv <= 0 || Tq < 0 || Lq < 0 || Lk < 0 || d <= 0 || window < 1 || sinks < 0) return 0;
+  if (!sizes_fit(B, n_head, n_kv, Tq, Lq, Lk, d, window, sinks)) return 0;
   WinParams p = {};
   p.B = B; p.H = n_head; p.G = n_kv; p.Tq = Tq; p.Lq = Lq; p.Lk = Lk; p.d = d; p.sinks = sinks;
   set_window(p, window, causal);
@@ -692,7 +699,7 @@ extern "C" int64_t skhip_window_attn_fwd_ws_floats(int B, int n_head, int n_kv, 
 
 extern "C" int64_t skhip_window_attn_bwd_ws_floats(int B, int n_head, int n_kv, int64_t Tq, int Lq, int Lk, int d, int window,
                                                    int sinks, int causal) {
-  if (B < 0 || n_head <= 0 || n_kv <= 0 || Tq < 0 || Lq < 0 || Lk < 0 || d <= 0 || window < 1 || sinks < 0) return 0;
+  if (!sizes_fit(B, n_head, n_kv, Tq, Lq, Lk, d, window, sinks)) return 0;
   WinParams p = {};
   p.B = B; p.H = n_head; p.G = n_kv; p.Tq = Tq; p.Lq = Lq; p.Lk = Lk; p.d = d; p.sinks = sinks;
   set_window(p, window, causal);

@@ -304,3 +304,12 @@ def test_workspace_of_few_queries_in_a_large_packed_tensor():
         assert lib.skhip_window_attn_fwd_ws_floats(1, 8, 8, Tq, 64, 32768, 128, 32768, 0, 1) <= few * 2, Tq
         back = lib.skhip_window_attn_bwd_ws_floats(1, 8, 8, Tq, 64, 32768, 128, 32768, 0, 1)
         assert back - 2 * 8 * Tq <= 2 * lib.skhip_window_attn_bwd_ws_floats(1, 8, 8, 64, 64, 32768, 128, 32768, 0, 1), Tq
+
+
+def test_workspace_sizes_of_refused_calls():
+    """0, as for every size that a call refuses, not what is left of an overflow."""
+    lib, M = L.load(), (1 << 31) - 1
+    for q in (lib.skhip_window_attn_fwd_ws_floats, lib.skhip_window_attn_bwd_ws_floats):
+        for Lq, Lk, d, H, G in ((M, M, 64, 8, 8), (100, M, 64, 8, 8), ((1 << 29) + 1, 5, 64, 8, 8), (100, 100, 129, 8, 8), (100, 100, 64, 8, 3)):
+            for window, sinks in ((M, 0), (M, 3), (60, M), (60, 5)):
+                assert q(1, H, G, 100, Lq, Lk, d, window, sinks, 1) == 0, (Lq, Lk, d, H, G, window, sinks)
