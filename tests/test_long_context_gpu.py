@@ -5,6 +5,7 @@ bf16, 2^-24 fp32) for every value that is stored in it, E = 2^-24 for every fp32
 values that the rounded quantities meet on the way to the element."""
 import decimal
 import math
+import threading
 
 import pytest
 import torch
@@ -1149,3 +1150,93 @@ def test_gradients_where_padding_leaves_few_keys(d, live):
     check(dq, a[0], a[1] + TINY, "dq")
     check(dk[keep], b[0], b[1] + TINY, "dk")
     assert not dk[pads[0].bool().to(DEV)].any()
+
+
+# ------------------------------------------------------------------------------ calls side by side
+def test_threads_and_streams_side_by_side():
+    """Four threads, each on a stream of its own, run the operators on their own tensors at once: each gets what it gets alone."""
+    H, G, d, sinks, cap = 4, 2, 64, 3, 5000
+    f = ops.RotaryFrequencies(64, device=DEV)
+
+    def case(seed):
+        g = torch.Generator().manual_seed(seed)
+        n, window, dtype = 150 + 40 * seed, 30 + seed, (BF, F32)[seed % 2]
+        x, do = rnd((n, (H + 2 * G) * d), dtype, g).to(DEV), rnd((n, H * d), dtype, g).to(DEV)
+        gq, gk = (1 + 0.1 * torch.randn(d, generator=g)).to(DEV), torch.ones(d, device=DEV)
+        kc, vc = rnd((1, cap, G * d), dtype, g).to(DEV), rnd((1, cap, G * d), dtype, g).to(DEV)
+        length, pos = torch.tensor([4500 + seed], dtype=torch.int32, device=DEV), torch.arange(n, device=DEV)
+
+        def work():
+            leaf = x.detach().requires_grad_()
+            q, k, v, o = block(leaf, pos, window, f, H, G, d, gq, gk, B=1, Lq=n, Lk=n, sinks=sinks)
+            few = ops.window_attention(q[-5:], k.repeat(20, 1), v.repeat(20, 1), 1, 5, 20 * n, H, G)   # keys cut over blocks
+            grad, = torch.autograd.grad((o, few), leaf, (do, do[-5:]))
+            with torch.no_grad():
+                return o.detach(), few.detach(), grad, ops.window_attention_step(q[:1], k[:1], v[:1], kc, vc, length, H, G, 4096, sinks)
+
+        return work
+
+    works = [case(s) for s in range(4)]
+    want = [w() for w in works]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def thread(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(10):
+                got = works[i]()
+                stream.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    wrong.append(i)
+        stream.synchronize()
+
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("d", [64, 80, 128, 37])
+def test_window_scores_of_minus_infinity(d, dtype):
+    """Keys whose score is -inf to every query count for nothing, whole tiles of them and single ones."""
+    g = torch.Generator().manual_seed(28)
+    n, m = 90, 400
+    q, k, v = rnd((n, d), dtype, g).abs() + 0.1, rnd((m, d), dtype, g), rnd((m, d), dtype, g)
+    alive = torch.ones(m, dtype=torch.bool)
+    alive[list(range(64, 200)) + list(range(201, 399, 2)) + [0, 399]] = False
+    k[~alive, 0] = -math.inf
+    o = ops.window_attention(q.to(DEV), k.to(DEV), v.to(DEV), 1, n, m, 1, causal=False)
+    vis = torch.ones((n, int(alive.sum())), dtype=torch.bool)
+    (want, bound), *_ = attention64(q, k[alive], v[alive], q, vis, d ** -0.5, dtype)
+    check(o, want, bound + TINY, "o")
+
+
+@pytest.mark.parametrize("n,window,sinks,causal", [(150, 30, 2, True), (260, 70, 0, False), (64, None, 0, True)])
+@pytest.mark.parametrize("shift", [1, 3, 4])
+def test_window_bf16_rows_off_their_pieces(shift, n, window, sinks, causal):
+    """bf16 heads of 64 in rows that are not 16-byte aligned: the bounds of test_window_attention."""
+    g = torch.Generator().manual_seed(29)
+    H, G, d = 4, 2, 64
+    x = torch.zeros((n, (H + 2 * G) * d + shift), dtype=BF)
+    x[:, shift:] = rnd((n, (H + 2 * G) * d), BF, g)
+    do = torch.zeros((n, H * d + shift), dtype=BF)
+    do[:, shift:] = rnd((n, H * d), BF, g)
+    cut = lambda t: (t[:, shift:shift + H * d], t[:, shift + H * d:shift + (H + G) * d], t[:, shift + (H + G) * d:])
+    leaves = [t.detach().requires_grad_() for t in cut(x.to(DEV))]
+    o = ops.window_attention(*leaves, 1, n, n, H, G, window, sinks, causal)
+    got = (o,) + torch.autograd.grad(o, leaves, do.to(DEV)[:, shift:])
+    q, k, v = cut(x)
+    want = [torch.zeros((n, w * d), dtype=torch.float64) for w in (H, H, G, G)]
+    bound = [torch.full_like(t, TINY) for t in want]
+    for h in range(H):
+        hs, ks = slice(h * d, h * d + d), slice(h // 2 * d, h // 2 * d + d)
+        res = attention64(q[:, hs], k[:, ks], v[:, ks], do[:, shift:][:, hs], visible(n, n, window or 1 << 30, sinks, causal), d ** -0.5, BF)
+        for i, cs in enumerate((hs, hs, ks, ks)):
+            want[i][:, cs] += res[i][0]
+            bound[i][:, cs] += res[i][1]
+    for a, w, b, name in zip(got, want, bound, ("o", "dq", "dk", "dv")):
+        check(a, w, b, name)
