@@ -103,9 +103,20 @@ struct KeyTiles {
 struct FewKeys { bool row; int lo, hi; };
 template <typename Padding, typename Usable>
 __device__ __forceinline__ FewKeys few_keys(const WinParams& p, const KeyTiles& kt, int pos, bool on, Padding padding, Usable usable) {
-  constexpr int GROUP = 4;   // tiles whose padding is on its way at a time: where little is left the whole text is walked
-  FewKeys f = {false, 0x7fffffff, 0};
+  FewKeys f = {false, 0, kt.n};
   int count = 0;
+  auto enough = [&]() { return __all(count > FEW || !on); };
+  if (!p.key_pad) {   // (the tiles are then those of the rows' windows, and few)
+    for (int t = kt.n - 1; t >= 0; --t) {
+      count += __popcll(keys_seen(p, pos, kt.start<64>(t), usable(t, 0)));
+      if (enough()) break;
+    }
+    f.row = on && count <= FEW;
+    return f;
+  }
+  constexpr int GROUP = 4;   // tiles whose padding is on its way at a time: where little is left the whole text is walked
+  f.lo = kt.n;
+  f.hi = 0;
   bool more = true;
   for (int t0 = kt.n - 1; more && t0 >= 0; t0 -= GROUP) {
     int gone[GROUP];
@@ -123,11 +134,11 @@ __device__ __forceinline__ FewKeys few_keys(const WinParams& p, const KeyTiles& 
         f.lo = t;
         f.hi = max(f.hi, t + 1);
       }
-      more = !__all(count > FEW || !on);
+      more = !enough();
     }
   }
   f.row = on && count <= FEW;
-  if (!__any(f.row)) f = {false, 0x7fffffff, 0};
+  if (!__any(f.row)) f = {false, kt.n, 0};
   return f;
 }
 
