@@ -8,8 +8,8 @@
 //   dgamma = sum over rows and heads of g * xhat, xhat = x * rstd;   dx = rstd (g gamma - xhat mean(g gamma xhat)).
 // Without the norm backward IS the forward kernel with the angles negated.
 //
-// Angles: a frequency is a 64-bit fraction of a turn, so  position * frequency mod 2^64  is the exact phase of any 64-bit
-// position in one integer product (in 32-bit floats position 10^6 would already be off by 0.06 rad).  Its top bits give
+// Angles: a frequency is a 64-bit fraction of a turn, so  position * frequency mod 2^64  is the exact phase at that frequency
+// of any 64-bit position in one integer product (in 32-bit floats position 10^6 would already be off by 0.06 rad).  Its top bits give
 // the quadrant and a remainder of at most 1/8 turn, which the Taylor polynomials of sine and cosine take to fp32
 // accuracy.  A block computes the (cos, sin) of its tokens once into LDS and uses them for all heads.
 //

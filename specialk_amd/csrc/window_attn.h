@@ -98,7 +98,7 @@ struct KeyTiles {
 
 // Whether the row at position pos (on: it exists) sees few keys, and the tiles [lo, hi) in which such rows of the wave see any:
 // the sweep for their delta, which every cut of the keys makes, needs no others (64 queries before 32768 keys, 8 heads of 128,
-// all but 20 keys padding, forward and backward: 232 us, sweeping every tile for delta 545; nothing padded 171).
+// all but 20 keys padding, forward and backward: 234 us, sweeping every tile for delta 545; nothing padded 172).
 // padding(t), usable(t, padding): tile t's keys, lane by lane and as bits.
 struct FewKeys { bool row; int lo, hi; };
 template <typename Padding, typename Usable>

@@ -11,9 +11,11 @@
 // next product as they stand (k = 4 (lane / 16) + r, taken for r = 0 .. 3 in turn).  Scores never reach memory; tiles
 // outside the window are never visited; dQ and dK / dV come from separate launches, so that no sum depends on the order
 // of blocks.  Shared key heads: the dK / dV block walks the query heads of its group.
-// Bound by the fp32 matrix rate (1/16 of bf16's): 8192 tokens, 8 heads of 64, causal: 0.79 ms forward, 87 TFLOP/s of the 154
-// that a product of two 8192 x 8192 matrices reaches; where the blocks are few by the latency of a tile (16 packed texts of
-// 100 - 1000 tokens, window 256: forward 77, dQ 101, dK and dV 154 us, 4.6 blocks of 5.5 tiles a CU in all).
+// 8192 tokens, 8 heads of 64, causal: 0.79 ms forward, 87 TFLOP/s of the 154 that a product of two 8192 x 8192 matrices
+// reaches: the matrix unit (1/16 of bf16's rate) is busy 55 % of the launch, 2.5 waves a SIMD spend 64 % of their time waiting
+// to issue and 19 % waiting for LDS or memory, and a CU is without waves for 12 %.  Where the blocks are few (16 packed texts
+// of 100 - 1000 tokens, window 256: forward 82, dQ 108, dK and dV 155 us, 4.6 blocks of 5.5 tiles a CU in all) it is busy 31 -
+// 35 %, with 1.6 waves.
 #include "window_attn.h"
 #include <algorithm>
 #include <type_traits>
@@ -595,8 +597,8 @@ void plan_keys(WinParams& p, int rows) {
 }
 
 // Cuts of a query tile's keys: two blocks for every CU, each with at least 12 tiles of 64 keys (fp32 arithmetic: 8).  64
-// queries at the end of 32768 keys, 8 heads of 128, all visible: 8 blocks alone 649 us, cut 54, with the backward pass 1262
-// and 186 (fp32 4276 and 148, 5861 and 737); 4096 tokens, 4 heads of 64, causal: 74 and 41.  Shorter sweeps are not worth
+// queries at the end of 32768 keys, 8 heads of 128, all visible: 8 blocks alone 649 us, cut 46, with the backward pass 1262
+// and 172 (fp32 4276 and 144, 5861 and 724); 4096 tokens, 4 heads of 64, causal: 74 and 36.  Shorter sweeps are not worth
 // the join: 2048 tokens, 8 heads of 128, window 1024 (18 tiles): uncut 30, in two 38.
 // (Partial outputs are kept for every row of Q: a packed tensor with more rows than its sequences counts whole.)
 void plan_cuts(WinParams& p, int rows) {

@@ -161,8 +161,8 @@ __device__ __forceinline__ float keep_or(float v, uint32_t m, uint32_t other) {
 // cycles and some 100 vector instructions, 16 of them exponentials, and the two units' busy times add up to all of the
 // kernel's (50 + 52 % at d = 128, 34 + 71 % at 64).  Dealing the matrix instructions out among the vector ones (scores of
 // the next half tile beside the probabilities of this one) does not help: the chip, at 1.8 of 2.4 GHz in this kernel, is
-// held by power as well (32771 tokens of 32 / 8 heads of 128, window 4096: 2.05 ms, 1000 TFLOP/s; so dealt 2.2; a product of
-// two 8192 x 8192 matrices reaches 1214).  So the arithmetic itself is kept small: the scale goes into the exponent's
+// held by power as well (32771 tokens of 32 / 8 heads of 128, window 4096: 2.10 - 2.19 ms by box, 940 - 980 TFLOP/s; so dealt
+// a twentieth to an eighth more; a product of two 8192 x 8192 matrices reaches 1214).  So the arithmetic itself is kept small: the scale goes into the exponent's
 // multiply-add, and the accumulators are rescaled only when a row's maximum has grown by more than 2^8 since the last
 // time: until then probabilities stay below 256, which bf16 holds as precisely as values below one.
 // Small windows are bound by the rows' way from memory instead: 256 packed sentences of 3 - 400 tokens, 8 heads of 64,
