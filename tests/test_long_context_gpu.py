@@ -1240,3 +1240,38 @@ def test_window_bf16_rows_off_their_pieces(shift, n, window, sinks, causal):
             bound[i][:, cs] += res[i][1]
     for a, w, b, name in zip(got, want, bound, ("o", "dq", "dk", "dv")):
         check(a, w, b, name)
+
+
+@pytest.mark.parametrize("dtype,n,sinks", [(BF, 5000, 3300), (F32, 4500, 4100)])
+def test_window_many_sinks_under_few_key_heads(dtype, n, sinks):
+    """Key tiles in parts and bounded chunks of far queries at once."""
+    H, G, d, window = 4, 1, 128, 20
+    g = torch.Generator().manual_seed(30)
+    q, do = (rnd((n, H * d), dtype, g).to(DEV) for _ in range(2))
+    k, v = (rnd((n, d), dtype, g).to(DEV) for _ in range(2))
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    o = ops.window_attention(*leaves, 1, n, n, H, G, window, sinks)
+    dq, dk, dv = torch.autograd.grad(o, leaves, do)
+    vis = visible(n, n, window, sinks, True).to(DEV)
+    sums = [torch.zeros((n, d), dtype=torch.float64, device=DEV) for _ in range(4)]
+    for h in range(H):
+        s = slice(h * d, h * d + d)
+        res = attention64(q[:, s], k, v, do[:, s], vis, d ** -0.5, dtype)
+        check(o[:, s], *res[0], ("o", h))
+        check(dq[:, s], *res[1], ("dq", h))
+        for i, x in enumerate(res[2] + res[3]):
+            sums[i] += x
+    check(dk, sums[0], sums[1], "dk")
+    check(dv, sums[2], sums[3], "dv")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("B,Lq,Lk", [(0, 5, 5), (3, 0, 5), (3, 5, 0), (3, 0, 0), (0, 0, 0)])
+def test_padded_batches_of_nothing(B, Lq, Lk, dtype):
+    q, do = torch.ones((B * Lq, 128), dtype=dtype, device=DEV).requires_grad_(), torch.ones((B * Lq, 128), dtype=dtype, device=DEV)
+    k, v = (torch.ones((B * Lk, 64), dtype=dtype, device=DEV).requires_grad_() for _ in range(2))
+    pad = torch.zeros((B, Lk), dtype=torch.bool, device=DEV)
+    o = ops.window_attention(q, k, v, B, Lq, Lk, 2, 1, 3, 2, key_pad=pad)
+    assert o.shape == (B * Lq, 128)
+    for t in (o,) + torch.autograd.grad(o, (q, k, v), do):
+        assert not t.any()
